@@ -17,7 +17,10 @@ CSRC = os.path.join(HERE, "csrc")
 OBJDIR = os.path.join(CSRC, "_build")
 OUT = os.path.join(HERE, "libseg_hip.so")
 STAMP = OUT + ".srchash"          # fingerprint of the sources the shipped .so was built from
-BASE_CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-fno-slp-vectorize"]
+# packed fp32 arithmetic (v_pk_add / mul / fma_f32) stays off altogether: -fno-slp-vectorize keeps the vectoriser from forming it, the
+# target feature keeps instruction selection from doing so for explicit vector types (the host pass warns that it does not know it)
+BASE_CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-fno-slp-vectorize",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 ABI_HEADER = os.path.join(ROOT, "include", "seg_hip.h")
 
 
