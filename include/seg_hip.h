@@ -581,6 +581,138 @@ int seg_pack_input_f32(const float* x, void* y, int64_t npix, int32_t C, int32_t
 int seg_unpack_f32_f32(const void* x, float* y, int64_t npix, int32_t C, int32_t cs, int32_t coff, seg_stream_t stream);
 
 
+/* ---- sequence operators -------------------------------------------------------------------------------------------
+ * A layer normalisation, a matrix product with its epilogue, a short causal convolution and a selective state space scan over rows
+ * of channels ([B][L][C], channels innermost): the pieces of a sequence mixer for 1D signals and flattened bottlenecks, beside the
+ * BatchNormalization, convolution and (T = 1) ConvLSTM entry points above.  They stand outside the storage modes: elements are plain
+ * fp16, bf16 or fp32 (`dtype`), never split pairs (seg_unpack_f32_f32 / seg_pack_input_f32 convert), and rows need no channel
+ * padding.  Row strides (`_ld`) and batch strides (`_bs`) are in ELEMENTS, the channel axis is contiguous; strides may describe
+ * slices of wider tensors.  Parameters, statistics, states of the scan and gradients of parameters are fp32, every sum is held in
+ * fp32.  Results do not depend on the order of blocks: two runs give the same bits.  Nothing is allocated: workspaces are asked
+ * for (`*_workspace_bytes`), need no initialisation and belong to one call in flight.  Inputs and outputs must not overlap unless
+ * an entry point says so.  Extents of zero are calls without work.                                                           */
+enum { SEG_DT_F16 = 0, SEG_DT_BF16 = 1, SEG_DT_F32 = 2 };
+/* activations of the sequence operators: SEG_ACT_NONE / RELU / LEAKY / SIGMOID and                                             */
+enum { SEG_ACT_SILU = 5, SEG_ACT_GELU = 6 };                       /* v sigmoid(v);  v Phi(v) (the error function, no tanh form) */
+
+/* Layer normalisation over the C channels of every row: y = (x - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps), biased
+ * variance.  gamma / beta NULL = 1 / 0; mean / rstd (fp32 [rows]) NULL = not wanted.  y may be x.                              */
+int seg_layernorm_fwd(const void* x, int64_t x_ld, void* y, int64_t y_ld, int64_t rows, int32_t C, int32_t dtype, const float* gamma,
+                      const float* beta, float eps, float* mean, float* rstd, seg_stream_t stream);
+/* its gradients: with xhat = (x - mean) * rstd and g = dy * gamma
+ *   dx = rstd * (g - mean_C(g) - xhat * mean_C(g * xhat)),  dgamma = sum_rows dy * xhat,  dbeta = sum_rows dy   (stored, not added)
+ * dx / dgamma / dbeta NULL = not wanted; dx may be dy or x.                                                                    */
+int64_t seg_layernorm_bwd_workspace_bytes(int64_t rows, int32_t C, int32_t dtype);
+int seg_layernorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, void* dx, int64_t dx_ld, int64_t rows, int32_t C,
+                      int32_t dtype, const float* mean, const float* rstd, const float* gamma, float* dgamma, float* dbeta,
+                      void* workspace, seg_stream_t stream);
+
+/* Matrix product with its epilogue.  x [M][K], w [N][K] (one row per output unit), y [M][N]:
+ *   seg_linear_fwd          z = x w^T + bias;  y = act(z) + residual            (z stored when z != NULL; bias, residual may be NULL)
+ *   seg_linear_bwd_data     y = (x w) * act'(z) + residual with x = the incoming gradient [M][K], w [K][N] as the layer stores it
+ *                           ([units][inputs]: K = units, N = inputs), z [M][N] the pre-activation of the layer in FRONT (NULL: no
+ *                           activation there), residual [M][N] another gradient of the same tensor (a skip connection's).  bias NULL
+ *   seg_linear_bwd_weight   dw [N][K] (fp32) = dy^T x, db [N] = sum_rows dy; x [M][K], dy [M][N]; dw / db NULL = not wanted
+ * fp16 / bf16 products are exact in the fp32 accumulators of the matrix cores; fp32 operands are contracted by the fp32 matrix
+ * instructions.  y may be residual (same strides), nothing else may overlap.                                                    */
+typedef struct seg_linear_args {
+  int64_t M;
+  int32_t N, K, dtype, act;
+  float alpha;                   /* slope of SEG_ACT_LEAKY */
+  const void* x; int64_t x_ld;
+  const void* w; int64_t w_ld;
+  const float* bias;
+  const void* residual; int64_t residual_ld;
+  void* z; int64_t z_ld;         /* written by fwd, read by bwd_data */
+  void* y; int64_t y_ld;
+  const void* dy; int64_t dy_ld; /* bwd_weight only */
+  float* dw; int64_t dw_ld;
+  float* db;
+  void* workspace;               /* seg_linear_workspace_bytes(args, pass) bytes */
+} seg_linear_args;
+enum { SEG_LINEAR_FWD = 0, SEG_LINEAR_BWD_DATA = 1, SEG_LINEAR_BWD_WEIGHT = 2 };
+int64_t seg_linear_workspace_bytes(const seg_linear_args* a, int32_t pass);
+int seg_linear_fwd(const seg_linear_args* a, seg_stream_t stream);
+int seg_linear_bwd_data(const seg_linear_args* a, seg_stream_t stream);
+int seg_linear_bwd_weight(const seg_linear_args* a, seg_stream_t stream);
+/* dx = dy * act'(z) on [rows][C] (an activation with no product behind it); dx may be dy                                       */
+int seg_linear_act_bwd(const void* dy, int64_t dy_ld, const void* z, int64_t z_ld, void* dx, int64_t dx_ld, int64_t rows, int32_t C,
+                       int32_t dtype, int32_t act, float alpha, seg_stream_t stream);
+
+/* Short causal convolution per channel: v[t] = bias + sum_k w[k] * xx[t + k], xx = [state (K - 1 rows); x], y[t] = act(v[t]).
+ * w fp32 [K][D], 1 <= K <= 8; bias fp32 [D] or NULL; act NONE or SILU; state [B][K-1][D] of dtype (dense) or NULL = zeros;
+ * lengths int32 [B] or NULL: rows t >= lengths[b] (clamped to [0, L]) are not read, their y is 0.  state_out (NULL: not wanted)
+ * = the last K - 1 rows of xx in front of lengths[b]; it may not be state.
+ * bwd: from dy (rows behind a length not read) and dstate_out (gradient of state_out, NULL = 0): dx (0 behind a length), dw, db (fp32,
+ * stored), dstate (gradient of state); each may be NULL.  step: one row per sequence, x / y [B][D], state_out may be state.     */
+typedef struct seg_causal_conv_args {
+  int32_t B, L, D, K, dtype, act;
+  const void* x; int64_t x_bs, x_ld;
+  const float* w;
+  const float* bias;
+  const void* state;
+  const int32_t* lengths;
+  void* y; int64_t y_bs, y_ld;
+  void* state_out;
+  const void* dy; int64_t dy_bs, dy_ld;
+  const void* dstate_out;
+  void* dx; int64_t dx_bs, dx_ld;
+  float* dw;
+  float* db;
+  void* dstate;
+  void* workspace;               /* seg_causal_conv_bwd only */
+} seg_causal_conv_args;
+int64_t seg_causal_conv_bwd_workspace_bytes(const seg_causal_conv_args* a);
+int seg_causal_conv_fwd(const seg_causal_conv_args* a, seg_stream_t stream);
+int seg_causal_conv_bwd(const seg_causal_conv_args* a, seg_stream_t stream);
+int seg_causal_conv_step(const seg_causal_conv_args* a, seg_stream_t stream);
+
+/* Selective state space scan.  Per sequence b, channel d and state s (1 <= S <= 64), with delta = softplus(dt + dt_bias) (softplus
+ * == 0: dt + dt_bias itself):
+ *   h[t] = exp(delta[t] A[d][s]) h[t-1] + delta[t] Bm[t][s] u[t],   y[t] = (sum_s Cm[t][s] h[t] + D[d] u[t]) * silu(z[t])
+ * u, dt, z, y [B][L][D], Bm, Cm [B][L][S] of dtype; A fp32 [D][S]; D, dt_bias fp32 [D] or NULL; z NULL = no gate; state fp32
+ * [B][D][S] = h in front of the first row (NULL: zeros); lengths as above: rows behind a length are not read, their y is 0 and the
+ * state stays; state_out (NULL: not wanted) may not be state.  saved (NULL: inference) receives what the backward pass needs:
+ * seg_selective_scan_saved_bytes() bytes.
+ * bwd: dy, dstate_out (NULL = 0), saved -> du, ddt, dz, dBm, dCm (of dtype, 0 behind a length), dA, dD, ddt_bias (fp32, stored),
+ * dstate; u, dt, z, Bm, Cm, A, D, dt_bias, softplus, lengths as in the forward call.  Gradients that are NULL are not wanted.
+ * step: one row per sequence (L = 1, strides _bs; lengths ignored), state_out may be state.                                      */
+typedef struct seg_scan_args {
+  int32_t B, L, D, S, dtype, softplus;
+  const void* u; int64_t u_bs, u_ld;
+  const void* dt; int64_t dt_bs, dt_ld;
+  const void* z; int64_t z_bs, z_ld;
+  const void* Bm; int64_t Bm_bs, Bm_ld;
+  const void* Cm; int64_t Cm_bs, Cm_ld;
+  const float* A;
+  const float* Dskip;
+  const float* dt_bias;
+  const float* state;
+  const int32_t* lengths;
+  void* y; int64_t y_bs, y_ld;
+  float* state_out;
+  float* saved;
+  const void* dy; int64_t dy_bs, dy_ld;
+  const float* dstate_out;
+  void* du; int64_t du_bs, du_ld;
+  void* ddt; int64_t ddt_bs, ddt_ld;
+  void* dz; int64_t dz_bs, dz_ld;
+  void* dBm; int64_t dBm_bs, dBm_ld;
+  void* dCm; int64_t dCm_bs, dCm_ld;
+  float* dA;
+  float* dD;
+  float* ddt_bias;
+  float* dstate;
+  void* workspace;
+} seg_scan_args;
+int64_t seg_selective_scan_saved_bytes(const seg_scan_args* a);
+int64_t seg_selective_scan_fwd_workspace_bytes(const seg_scan_args* a);
+int64_t seg_selective_scan_bwd_workspace_bytes(const seg_scan_args* a);
+int seg_selective_scan_fwd(const seg_scan_args* a, seg_stream_t stream);
+int seg_selective_scan_bwd(const seg_scan_args* a, seg_stream_t stream);
+int seg_selective_scan_step(const seg_scan_args* a, seg_stream_t stream);
+
+
 #ifdef __cplusplus
 }
 #endif

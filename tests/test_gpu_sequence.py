@@ -1,0 +1,586 @@
+"""GPU: the sequence operators (sequence.py) against their definitions in 64 bits (tests/sequence_ref.py), with bounds that count
+roundings; strides, lengths, empty and single rows, graphs, streams, and a whole mixer block forward, backward and row by row."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs an MI355X", allow_module_level=True)
+
+import sequence_ref as R
+from segamd import sequence as seq
+
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+IDS = ["f16", "bf16", "f32"]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rnd(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def dev(t):
+    return None if t is None else t.cuda()
+
+
+def wide(t, left, right):
+    """t's values as a slice of a wider device tensor whose other columns are NaN."""
+    o = torch.full(t.shape[:-1] + (left + t.shape[-1] + right,), float("nan"), dtype=t.dtype, device="cuda")
+    o[..., left:left + t.shape[-1]] = t.cuda()
+    return o[..., left:left + t.shape[-1]]
+
+
+# ------------------------------------------------------------------------------------------------------- layer normalisation
+LN_SHAPES = [(1, 1), (3, 7), (5, 8), (70, 64), (9, 120), (33, 200), (7, 512), (6, 1000), (2, 2048), (5, 2056), (3, 4100), (2, 8192), (2, 16384), (2, 16390)]
+
+
+def ln_ref(x, gamma, beta, eps, dy):
+    x64 = x.double().requires_grad_()
+    g64 = (torch.ones(x.shape[1]) if gamma is None else gamma).double().requires_grad_()
+    b64 = (torch.zeros(x.shape[1]) if beta is None else beta).double().requires_grad_()
+    mean = x64.mean(1, keepdim=True)
+    rstd = (((x64 - mean) ** 2).mean(1, keepdim=True) + eps) ** -0.5
+    y = (x64 - mean) * rstd * g64 + b64
+    dx, dg, db = torch.autograd.grad(y, (x64, g64, b64), dy.double())
+    return y.detach(), mean.detach()[:, 0], rstd.detach()[:, 0], dx, dg, db
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,C", LN_SHAPES)
+def test_layer_norm(rows, C, dtype):
+    g = gen(rows * 7 + C)
+    x = (rnd(g, rows, C) * (torch.rand(rows, 1, generator=g) + 0.3) + rnd(g, rows, 1)).to(dtype)
+    dy, gamma, beta = rnd(g, rows, C, dtype=dtype), torch.rand(C, generator=g) + 0.5, rnd(g, C)
+    y, mean, rstd, dx, dgamma, dbeta = ln_ref(x, gamma, beta, 1e-3, dy)
+    # longest chain of a sum over the row: a lane's own channels (64 at most; C / 256 where rows are walked), 8 to combine them
+    n = max(64, C // 256 + 1) + 8
+    x64, r = x.double(), rstd[:, None]
+    xm = x64.abs().mean(1, keepdim=True)
+    xh = ((x64 - mean[:, None]) * r).abs()
+    xs = xh + xm * r                                         # xhat with the cancelled mean's terms
+    # rstd: half of the variance's relative error, whose terms are (x - mean)^2 with a cancelled mean
+    cond = (xs * xs).mean(1, keepdim=True)
+    gy, gm, gr = seq.layer_norm(x.cuda(), gamma.cuda(), beta.cuda(), eps=1e-3, stats=True)
+    R.assert_close(gm, mean, xm[:, 0], n, "mean")
+    R.assert_close(gr, rstd, rstd * (1 + cond[:, 0]), n + 4, "rstd")
+    R.assert_close(gy, y, (xs + xh * (1 + cond)) * gamma.double() + beta.double().abs(), n + 8, "y")
+    assert torch.equal(gy, seq.layer_norm(x.cuda(), gamma.cuda(), beta.cuda(), eps=1e-3))
+    gdx, gdg, gdb = seq.layer_norm_backward(dy.cuda(), x.cuda(), gm, gr, gamma.cuda())
+    d64 = dy.double().abs()
+    # the backward pass takes mean / rstd as they are in 32 bits: their errors (bounded above) enter xhat
+    xe = xs + xh * (1 + cond)
+    s = d64 * gamma.double()
+    R.assert_close(gdx, dx, r * (s + s.mean(1, keepdim=True) + xe * (s * xe).mean(1, keepdim=True) * 2), 2 * n + 16, "dx")
+    R.assert_close(gdb, dbeta, d64.sum(0), rows + 16, "dbeta")
+    R.assert_close(gdg, dgamma, (d64 * xe).sum(0), rows + n + 16, "dgamma")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_layer_norm_many_rows_reduce_in_order(dtype):
+    """Enough rows for every block to walk several of them: two runs give the same bits, gradients of the parameters hold."""
+    g = gen(5)
+    rows, C = 40001, 24
+    x, dy = rnd(g, rows, C, dtype=dtype), rnd(g, rows, C, dtype=dtype)
+    _y, mean, rstd, dx, dgamma, dbeta = ln_ref(x, None, None, 1e-3, dy)
+    args = (dy.cuda(), x.cuda(), mean.float().cuda(), rstd.float().cuda())
+    a, b = seq.layer_norm_backward(*args), seq.layer_norm_backward(*args)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    xh = ((x.double() - mean[:, None]) * rstd[:, None]).abs() + 1
+    d64 = dy.double().abs()
+    # a thread adds at most rows / (32 rows per block x 313 blocks) + the block's and the blocks' sums, far below the count used here
+    R.assert_close(a[1], dgamma, (d64 * xh).sum(0), 400, "dgamma")
+    R.assert_close(a[2], dbeta, d64.sum(0), 400, "dbeta")
+    R.assert_close(a[0], dx, rstd[:, None] * (d64 + 2 * xh * (d64 * xh).mean(1, keepdim=True) + d64.mean(1, keepdim=True)), 64, "dx")
+
+
+def test_layer_norm_slices_and_offsets():
+    """Slices of wider tensors (aligned or not), NaN beside them; no gamma / beta; leading axes; nothing outside is written."""
+    g = gen(6)
+    for left, right, C in ((8, 8, 64), (3, 2, 64), (1, 0, 37)):
+        x = rnd(g, 2, 9, C, dtype=torch.float16)
+        y, mean, rstd = seq.layer_norm(wide(x, left, right), stats=True)
+        assert y.shape == x.shape and mean.shape == (2, 9)
+        w = seq.layer_norm(x.cuda())
+        R.assert_close(y, w.double().cpu(), torch.ones(2, 9, C, dtype=torch.float64), 64, "slice")      # (another lane order: 32-bit error only)
+        dy = rnd(g, 2, 9, C, dtype=torch.float16)
+        for p, q in zip(seq.layer_norm_backward(wide(dy, left, right), wide(x, left, right), mean, rstd), seq.layer_norm_backward(dy.cuda(), x.cuda(), mean, rstd)):
+            R.assert_close(p, q.double().cpu(), 64 * torch.ones(q.shape, dtype=torch.float64), 64, "slice backward")
+
+
+def test_layer_norm_no_rows_and_constant_rows():
+    y, mean, rstd = seq.layer_norm(torch.empty(0, 40, device="cuda"), stats=True)
+    assert y.shape == (0, 40) and mean.shape == (0,)
+    dx, dg, db = seq.layer_norm_backward(y, y, mean, rstd)
+    assert dx.shape == (0, 40) and not dg.any() and not db.any() and dg.shape == (40,)
+    x = torch.full((3, 72), 1.25, device="cuda", dtype=torch.bfloat16)
+    y, mean, rstd = seq.layer_norm(x, eps=1e-3, stats=True)
+    assert not y.any() and torch.equal(mean, torch.full_like(mean, 1.25))
+
+
+def test_layer_norm_non_finite_rows_stay_in_their_row():
+    x = torch.randn(4, 256, generator=gen(8)).cuda()
+    want = seq.layer_norm(x)
+    x[1, 3], x[2, 5] = float("inf"), float("nan")
+    y = seq.layer_norm(x)
+    assert torch.equal(y[0], want[0]) and torch.equal(y[3], want[3]) and torch.isnan(y[1:3]).any(1).all()
+
+
+# --------------------------------------------------------------------------------------------------------------------- linear
+LIN = [(1, 8, 8), (1, 1, 1), (3, 5, 7), (16, 64, 64), (64, 64, 32), (65, 130, 100), (17, 33, 257), (129, 256, 512), (300, 200, 1000), (2, 1000, 4096),
+       (256, 256, 64), (257, 264, 72), (512, 384, 640)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", LIN)
+def test_linear_epilogue(M, N, K, dtype):
+    g = gen(M + 3 * N + 5 * K)
+    x, w, b, r = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5), rnd(g, N), rnd(g, M, N, dtype=dtype)
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64.t() + b.double()
+    s = x64.abs() @ w64.abs().t() + b.double().abs()
+    for k, name in enumerate([None, "relu", "leaky_relu", "sigmoid", "silu", "gelu"]):
+        if k % 3 != (M + N + K) % 3 and (M, N, K) != (65, 130, 100):
+            continue
+        y, gz = seq.linear(x.cuda(), w.cuda(), b.cuda(), activation=name, residual=r.cuda(), preactivation=True)
+        R.assert_close(gz, z, s, K + 4, "z")
+        # every activation here has a slope of at most 1.13; its own evaluation: 16 roundings of a value of at most |z| + 1
+        R.assert_close(y, R.act(z, name) + r.double(), 1.13 * s + r.double().abs() + z.abs() + 1, K + 24, f"y {name}")
+    y = seq.linear(x.cuda(), w.cuda())
+    R.assert_close(y, x64 @ w64.t(), s, K + 4, "plain")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", LIN + [(4096, 24, 40), (5000, 136, 72)])
+def test_linear_backward(M, N, K, dtype):
+    g = gen(M + 3 * N + 7 * K)
+    x, w, dy, z, r = (rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=N ** -0.5), rnd(g, M, N, dtype=dtype), rnd(g, M, K, dtype=dtype),
+                      rnd(g, M, K, dtype=dtype))
+    d64, w64, x64 = dy.double(), w.double(), x.double()
+    name = ["relu", "gelu", "silu", "leaky_relu", "sigmoid"][(M + N + K) % 5]
+    dx, dw, db = seq.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z=z.cuda(), activation=name, residual=r.cuda())
+    slope = R.act_slope(z.double(), name)
+    s = d64.abs() @ w64.abs()
+    R.assert_close(dx, (d64 @ w64) * slope + r.double(), 1.13 * s + (d64 @ w64).abs() * (1 + z.double().abs()) + r.double().abs(), N + 24, "dx")
+    R.assert_close(dw, d64.t() @ x64, d64.abs().t() @ x64.abs(), M + 4, "dw")
+    R.assert_close(db, d64.sum(0), d64.abs().sum(0), M + 4, "db")
+    dx, none, db2 = seq.linear_backward(dy.cuda(), x.cuda(), w.cuda(), need_dw=False)
+    assert none is None and torch.equal(db, db2)
+    R.assert_close(dx, d64 @ w64, s, N + 4, "dx plain")
+
+
+def test_linear_backward_is_the_difference_quotient():
+    """f32: a two-layer perceptron's loss moved along every gradient agrees with the central difference (error of the quotient: step^2 of
+    the third derivative, plus the loss' own rounding over the step)."""
+    g = gen(11)
+    x, w1, b1, w2 = rnd(g, 20, 24), rnd(g, 40, 24, scale=0.2), rnd(g, 40), rnd(g, 16, 40, scale=0.2)
+    dy = rnd(g, 20, 16)
+
+    def loss(x, w1, b1, w2):
+        h = R.act(x.double() @ w1.double().t() + b1.double(), "gelu")
+        return float(((h @ w2.double().t()) * dy.double()).sum())
+    h, z = seq.linear(x.cuda(), w1.cuda(), b1.cuda(), activation="gelu", preactivation=True)
+    dz, dw2, _ = seq.linear_backward(dy.cuda(), h, w2.cuda(), z=z, activation="gelu", need_db=False)
+    dx, dw1, db1 = seq.linear_backward(dz, x.cuda(), w1.cuda())
+    for i, grad in enumerate((dx, dw1, db1, dw2)):
+        args = [x, w1, b1, w2]
+        v = rnd(g, *args[i].shape).double()
+        up, down = list(args), list(args)
+        up[i], down[i] = args[i].double() + 1e-4 * v, args[i].double() - 1e-4 * v
+        quotient = (loss(*up) - loss(*down)) / 2e-4
+        got = float((grad.double().cpu() * v).sum())
+        assert abs(got - quotient) <= 1e-4 * float((grad.double().cpu() * v).abs().sum()), (i, got, quotient)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_linear_slices(dtype):
+    """Operands as slices of wider tensors, aligned or not, NaN beside them - also behind the last input of a row, where a tile ends."""
+    g = gen(12)
+    for left, right, (M, N, K) in ((8, 8, (70, 72, 40)), (8, 24, (130, 256, 136)), (3, 1, (33, 40, 48)), (4, 4, (33, 40, 44))):
+        x, w, dy, z = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype), rnd(g, M, N, dtype=dtype), rnd(g, M, K, dtype=dtype)
+        X, W, DY, Z = (wide(t, left, right) for t in (x, w, dy, z))
+        s = x.double().abs() @ w.double().abs().t()
+        R.assert_close(seq.linear(X, W), x.double() @ w.double().t(), s, K + 4, "fwd")
+        dx, dw, db = seq.linear_backward(DY, X, W, z=Z, activation="relu")
+        R.assert_close(dx, (dy.double() @ w.double()) * (z.double() > 0), dy.double().abs() @ w.double().abs(), N + 4, "dx")
+        R.assert_close(dw, dy.double().t() @ x.double(), dy.double().abs().t() @ x.double().abs(), M + 4, "dw")
+        R.assert_close(db, dy.double().sum(0), dy.double().abs().sum(0), M + 4, "db")
+
+
+def test_linear_no_rows_and_leading_axes():
+    w = torch.randn(6, 10, generator=gen(1)).cuda()
+    y = seq.linear(torch.empty(0, 10, device="cuda"), w)
+    assert y.shape == (0, 6)
+    dx, dw, db = seq.linear_backward(y, torch.empty(0, 10, device="cuda"), w)
+    assert dx.shape == (0, 10) and not dw.any() and not db.any()
+    x = torch.randn(2, 3, 10, generator=gen(2)).cuda()
+    assert torch.equal(seq.linear(x, w).reshape(6, 6), seq.linear(x.reshape(6, 10), w))
+    assert torch.equal(seq.linear(x[0, 0], w), seq.linear(x[0, :1], w)[0])
+
+
+@pytest.mark.parametrize("name", ["relu", "leaky_relu", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_activation_backward(name, dtype):
+    g = gen(13)
+    for shape in ((5, 33), (3, 7, 64)):
+        z, dy = rnd(g, *shape, dtype=dtype, scale=3.0), rnd(g, *shape, dtype=dtype)
+        R.assert_close(seq.activation_backward(dy.cuda(), z.cuda(), name), dy.double() * R.act_slope(z.double(), name), dy.double().abs() * (1 + z.double().abs()), 24, name)
+
+
+@pytest.mark.parametrize("name", ["silu", "gelu", "sigmoid"])
+def test_activations_at_the_ends(name):
+    """Large arguments of either sign: finite, and the limits."""
+    z = torch.tensor([[-3e38, -1e5, -200.0, -88.0, 0.0, 88.0, 200.0, 1e5]]).cuda()
+    one = torch.eye(8).cuda()
+    y = seq.linear(z, one, activation=name)
+    want = R.act(z.double().cpu(), name)
+    assert torch.isfinite(y).all() and torch.allclose(y.double().cpu(), want, rtol=1e-5, atol=1e-30)
+
+
+# --------------------------------------------------------------------------------------------------------- causal convolution
+CONV = [(1, 1, 1, 1), (2, 1, 8, 4), (3, 5, 16, 3), (2, 17, 40, 4), (2, 33, 7, 2), (1, 130, 264, 4), (2, 300, 24, 8), (3, 16, 12, 5), (1, 3, 8, 6), (2, 2, 16, 7)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("silu", [False, True], ids=["none", "silu"])
+@pytest.mark.parametrize("B,L,D,K", CONV)
+def test_causal_conv(B, L, D, K, silu, dtype):
+    g = gen(B + 3 * L + 5 * D + 7 * K)
+    x, dy, st, dst = rnd(g, B, L, D, dtype=dtype), rnd(g, B, L, D, dtype=dtype), rnd(g, B, K - 1, D, dtype=dtype), rnd(g, B, K - 1, D, dtype=dtype)
+    w, bias = rnd(g, K, D), rnd(g, D)
+    for ragged in (False, True):
+        lengths = torch.randint(-1, L + 2, (B,), generator=g, dtype=torch.int32) if ragged else None
+        if ragged:
+            lengths[0] = 0
+        args = [t.double().requires_grad_() for t in (x, w, bias, st)]
+        y, so = R.conv(*args, lengths, silu)
+        gx, gw, gb, gst = torch.autograd.grad((y, so), args, (dy.double(), dst.double()), allow_unused=True)
+        act = "silu" if silu else None
+        xd, dyd = x.cuda(), dy.cuda()
+        if ragged:                                            # what stands behind a length is not read
+            for b in range(B):
+                xd[b, max(int(lengths[b]), 0):] = float("nan")
+                dyd[b, max(int(lengths[b]), 0):] = float("inf")
+        ln = dev(lengths)
+        gy, gso = seq.causal_conv(xd, w.cuda(), bias.cuda(), activation=act, state=st.cuda(), lengths=ln)
+        assert torch.equal(gso.cpu(), so.detach().to(dtype))
+        ya, _ = R.conv(x.double().abs(), w.double().abs(), bias.double().abs(), st.double().abs(), lengths, False)
+        R.assert_close(gy, y, 1.13 * ya + y.detach().abs(), K + 16, "y")
+        dx, dw, db, dst_in = seq.causal_conv_backward(dyd, xd, w.cuda(), bias.cuda(), activation=act, state=st.cuda(), lengths=ln, dstate=dst.cuda())
+        # gradients: dv = dy act'(v), |act'| <= 1.13 with a slope of at most 0.5 towards v's error
+        dv = (1.2 * dy.double().abs() * (1 + ya))
+        if ragged:
+            for b in range(B):
+                dv[b, max(int(lengths[b]), 0):] = 0
+        sx = torch.zeros(B, L + K - 1, D, dtype=torch.float64)
+        sw = torch.zeros(K, D, dtype=torch.float64)
+        xx = torch.cat([st.double().abs(), x.double().abs()], 1)
+        for k in range(K):
+            sx[:, k:k + L] += dv * w[k].double().abs()
+            sw[k] = (dv * xx[:, k:k + L]).sum((0, 1))
+        for b in range(B):
+            m = L if lengths is None else min(max(int(lengths[b]), 0), L)
+            sx[b, m:m + K - 1] += dst[b].double().abs()
+        R.assert_close(dx, gx, sx[:, K - 1:], 4 * K + 24, "dx")
+        R.assert_close(dst_in, gst if gst is not None else torch.zeros_like(st).double(), sx[:, :K - 1], 4 * K + 24, "dstate")
+        R.assert_close(dw, gw, sw, B * L + 2 * K + 24, "dw")
+        R.assert_close(db, gb, dv.sum((0, 1)), B * L + 2 * K + 24, "db")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_causal_conv_steps_are_the_prompt(dtype):
+    """A prompt, then row by row from its state: the same outputs as the whole prompt; in place and through a second buffer."""
+    g = gen(21)
+    B, L, D, K = 3, 9, 40, 4
+    x, w, bias = rnd(g, B, L, D, dtype=dtype).cuda(), rnd(g, K, D).cuda(), rnd(g, D).cuda()
+    y, last = seq.causal_conv(x, w, bias, activation="silu")
+    first, state = seq.causal_conv(x[:, :4], w, bias, activation="silu")
+    assert torch.equal(first, y[:, :4])
+    other = torch.empty_like(state)
+    for t in range(4, L):
+        keep = state.clone()
+        yt = seq.causal_conv_step(x[:, t], state, w, bias, activation="silu", new_state=other)
+        assert torch.equal(state, keep)
+        assert torch.equal(yt, seq.causal_conv_step(x[:, t], state, w, bias, activation="silu"))
+        assert torch.equal(state, other)
+        assert torch.equal(yt, y[:, t])
+    assert torch.equal(state, last)
+
+
+# ------------------------------------------------------------------------------------------------------- selective state space
+SCAN = [(1, 1, 1, 1), (2, 3, 8, 4), (1, 31, 5, 3), (2, 33, 24, 16), (1, 64, 64, 16), (2, 70, 72, 8), (2, 100, 16, 32), (1, 65, 20, 64), (2, 40, 9, 61), (1, 260, 8, 16),
+        (3, 50, 130, 6)]
+
+
+def scan_inputs(seed, B, L, D, S, dtype):
+    g = gen(seed)
+    i = dict(u=rnd(g, B, L, D, dtype=dtype), dt=rnd(g, B, L, D, dtype=dtype, scale=0.7), A=-(torch.rand(D, S, generator=g) * 4 + 0.05),
+             B=rnd(g, B, L, S, dtype=dtype), C=rnd(g, B, L, S, dtype=dtype), D=rnd(g, D), z=rnd(g, B, L, D, dtype=dtype), dt_bias=rnd(g, D) - 2.0,
+             state=rnd(g, B, D, S))
+    return i, rnd(g, B, L, D, dtype=dtype), rnd(g, B, D, S), g
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("B,L,D,S", SCAN)
+def test_selective_scan(B, L, D, S, dtype):
+    i, dy, dstate, g = scan_inputs(B + 3 * L + 5 * D + 7 * S, B, L, D, S, dtype)
+    for ragged, bare, sp in ((False, False, True), (True, False, True), (False, True, True), (True, True, False)):
+        k = dict(i)
+        if not sp:
+            k["dt"] = k["dt"].abs()                            # the step itself, as a caller's own softplus leaves it
+        if bare:
+            k["D"] = k["z"] = k["dt_bias"] = k["state"] = None
+        lengths = torch.randint(-1, L + 2, (B,), generator=g, dtype=torch.int32) if ragged else torch.full((B,), L, dtype=torch.int32)
+        if ragged and B > 1:
+            lengths[0] = 0
+        ds = None if bare else dstate
+        v = {n: None if t is None else t.double().requires_grad_() for n, t in k.items()}
+        y, last = R.scan(**v, softplus=sp, lengths=lengths)
+        names = [n for n in v if v[n] is not None]
+        gr = torch.autograd.grad((y, last), [v[n] for n in names], (dy.double(), torch.zeros_like(last) if ds is None else ds.double()), allow_unused=True)
+        gr = {n: torch.zeros_like(v[n]) if t is None else t for n, t in zip(names, gr)}
+        d64 = {n: None if t is None else t.double() for n, t in k.items()}
+        sc = R.scan_scales(*(d64[n] for n in ("u", "dt", "A", "B", "C", "D", "z", "dt_bias")), sp, d64["state"], lengths.clamp(0, L), dy.double(),
+                           None if ds is None else ds.double())
+        # a row's step: 8 roundings, the exponent's argument (known to 12 roundings) times its error; every term passes at most L rows, forward
+        # and again backward
+        n = int((8 + 12 * (1 + sc["arg"])) * (L + 8)) + 64
+        c = {m: dev(t) for m, t in k.items()}
+        dyd = dy.cuda()
+        if ragged:
+            for b in range(B):
+                for m in ("u", "dt", "B", "C", "z"):
+                    if c[m] is not None:
+                        c[m][b, max(int(lengths[b]), 0):] = float("nan")
+                dyd[b, max(int(lengths[b]), 0):] = float("nan")
+        ln = dev(lengths) if ragged else None
+        state = c.pop("state")
+        gy, gl, saved = seq.selective_scan(**c, softplus=sp, state=state, lengths=ln, training=True)
+        R.assert_close(gy, y, sc["y"], n, "y")
+        R.assert_close(gl, last, sc["state"], n, "state")
+        y2, l2 = seq.selective_scan(**c, softplus=sp, state=state, lengths=ln)
+        assert torch.equal(gy, y2) and torch.equal(gl, l2)
+        d = seq.selective_scan_backward(dyd, c["u"], c["dt"], c["A"], c["B"], c["C"], saved, D=c["D"], z=c["z"], dt_bias=c["dt_bias"], softplus=sp,
+                                        lengths=ln, dstate=dev(ds))
+        nb = n + D + B * L
+        for name, got in (("u", d.du), ("dt", d.ddt), ("A", d.dA), ("B", d.dB), ("C", d.dC), ("D", d.dD), ("z", d.dz), ("dt_bias", d.ddt_bias)):
+            if k[name] is None:
+                assert got is None
+                continue
+            R.assert_close(got, gr[name], sc["d" + name], nb, "d" + name)
+        if state is not None:
+            R.assert_close(d.dstate, gr["state"], sc["dstate"], n, "dstate")
+        again = seq.selective_scan_backward(dyd, c["u"], c["dt"], c["A"], c["B"], c["C"], saved, D=c["D"], z=c["z"], dt_bias=c["dt_bias"], softplus=sp,
+                                            lengths=ln, dstate=dev(ds))
+        assert all(p is q or torch.equal(p, q) for p, q in zip(d, again))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_selective_scan_slices(dtype):
+    """B, C next to each other in one projection's output, u and z halves of another, at aligned and odd columns."""
+    B, L, D, S = 2, 45, 40, 16
+    i, dy, dstate, g = scan_inputs(77, B, L, D, S, dtype)
+    c = {m: dev(t) for m, t in i.items()}
+    want = seq.selective_scan(**c, training=True)
+    dw = seq.selective_scan_backward(dy.cuda(), c["u"], c["dt"], c["A"], c["B"], c["C"], want[2], D=c["D"], z=c["z"], dt_bias=c["dt_bias"])
+    for left, right in ((8, 8), (5, 3)):
+        s = dict(c)
+        for m in ("u", "dt", "B", "C", "z"):
+            s[m] = wide(i[m], left, right)
+        got = seq.selective_scan(**s, training=True)
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+        dg = seq.selective_scan_backward(wide(dy, left, right), s["u"], s["dt"], s["A"], s["B"], s["C"], got[2], D=s["D"], z=s["z"], dt_bias=s["dt_bias"])
+        assert all(torch.equal(p, q) for p, q in zip(dw, dg))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("S", [3, 16, 40])
+def test_selective_scan_steps_are_the_prompt(S, dtype):
+    B, L, D = 3, 8, 24
+    i, _dy, _ds, _g = scan_inputs(31 + S, B, L, D, S, dtype)
+    c = {m: dev(t) for m, t in i.items()}
+    y, last = seq.selective_scan(**c)
+    state = c["state"].clone()
+    other = torch.empty_like(state)
+    v = {m: None if t is None else t.double() for m, t in i.items()}
+    sc = R.scan_scales(*(v[n] for n in ("u", "dt", "A", "B", "C", "D", "z", "dt_bias")), True, v["state"], torch.full((B,), L), torch.zeros(B, L, D).double(), None)
+    n = int((8 + 12 * (1 + sc["arg"])) * (L + 8)) + 64
+    want, _ = R.scan(**v)
+    for t in range(L):
+        at = dict(u=c["u"][:, t], dt=c["dt"][:, t], A=c["A"], B=c["B"][:, t], C=c["C"][:, t], D=c["D"], z=c["z"][:, t], dt_bias=c["dt_bias"])
+        keep = state.clone()
+        yt = seq.selective_scan_step(state=state, new_state=other, **at)
+        assert torch.equal(state, keep)
+        assert torch.equal(yt, seq.selective_scan_step(state=state, **at)) and torch.equal(state, other)
+        R.assert_close(yt, want[:, t], sc["y"][:, t], n, f"row {t}")
+    R.assert_close(state, last.double().cpu(), sc["state"], 2 * n, "state")
+
+
+def test_selective_scan_no_rows():
+    B, L, D, S = 2, 0, 8, 16
+    i, _dy, _ds, g = scan_inputs(3, B, L, D, S, torch.float32)
+    c = {m: dev(t) for m, t in i.items()}
+    y, last, saved = seq.selective_scan(**c, training=True)
+    assert y.shape == (2, 0, 8) and torch.equal(last, c["state"]) and saved.numel() == 0
+    ds = rnd(g, B, D, S).cuda()
+    d = seq.selective_scan_backward(y, c["u"], c["dt"], c["A"], c["B"], c["C"], saved, D=c["D"], z=c["z"], dt_bias=c["dt_bias"], dstate=ds)
+    assert torch.equal(d.dstate, ds) and not d.dA.any() and not d.dD.any() and not d.ddt_bias.any()
+    e = torch.empty(0, 5, 8, device="cuda")
+    y, last = seq.selective_scan(e, e, c["A"], torch.empty(0, 5, 16, device="cuda"), torch.empty(0, 5, 16, device="cuda"))
+    assert y.shape == (0, 5, 8) and last.shape == (0, 8, 16)
+
+
+# ------------------------------------------------------------------------------------------------------------- a run together
+class Mixer:
+    """norm -> two projections -> causal convolution -> step / B / C projection -> gated scan -> projection + residual."""
+
+    def __init__(self, g, D, H, S, Rk, K, dtype):
+        def p(*s):
+            return rnd(g, *s, scale=s[-1] ** -0.5).to(dtype)
+        self.gamma, self.beta = torch.rand(D, generator=g) + 0.5, rnd(g, D, scale=0.1)
+        self.w_in, self.w_x, self.w_dt, self.w_out = p(2 * H, D), p(Rk + 2 * S, H), p(H, Rk), p(D, H)
+        self.cw, self.cb = rnd(g, K, H, scale=0.5), rnd(g, H, scale=0.1)
+        self.A, self.D, self.bias = -(torch.rand(H, S, generator=g) * 3 + 0.1), rnd(g, H), rnd(g, H) - 2.0
+        self.H, self.S, self.R = H, S, Rk
+
+    def names(self):
+        return ("gamma", "beta", "w_in", "w_x", "w_dt", "w_out", "cw", "cb", "A", "D", "bias")
+
+    def to(self, f):
+        m = object.__new__(Mixer)
+        m.__dict__.update({k: f(v) if torch.is_tensor(v) else v for k, v in self.__dict__.items()})
+        return m
+
+    def reference(self, x):
+        B, L, D = x.shape
+        mean = x.mean(-1, keepdim=True)
+        n = (x - mean) * (((x - mean) ** 2).mean(-1, keepdim=True) + 1e-3) ** -0.5 * self.gamma + self.beta
+        xz = n @ self.w_in.t()
+        c, _ = R.conv(xz[..., :self.H], self.cw, self.cb, None, None, True)
+        q = c @ self.w_x.t()
+        dt = q[..., :self.R] @ self.w_dt.t()
+        y, last = R.scan(c, dt, self.A, q[..., self.R:self.R + self.S], q[..., self.R + self.S:], self.D, xz[..., self.H:], self.bias)
+        return y @ self.w_out.t() + x, last
+
+    def prompt(self, x):
+        s = {}
+        s["x"] = x
+        s["n"], s["mean"], s["rstd"] = seq.layer_norm(x, self.gamma, self.beta, stats=True)
+        s["xz"] = seq.linear(s["n"], self.w_in)
+        s["c"], s["conv"] = seq.causal_conv(s["xz"][..., :self.H], self.cw, self.cb, activation="silu")
+        s["q"] = seq.linear(s["c"], self.w_x)
+        s["dt"] = seq.linear(s["q"][..., :self.R], self.w_dt)
+        s["y"], s["h"], s["saved"] = seq.selective_scan(s["c"], s["dt"], self.A, s["q"][..., self.R:self.R + self.S], s["q"][..., self.R + self.S:], D=self.D,
+                                                        z=s["xz"][..., self.H:], dt_bias=self.bias, training=True)
+        return seq.linear(s["y"], self.w_out, residual=x), s
+
+    def backward(self, dout, s):
+        H, Rk, S = self.H, self.R, self.S
+        g = {}
+        dy, g["w_out"], _ = seq.linear_backward(dout, s["y"], self.w_out, need_db=False)
+        q, z = s["q"], s["xz"][..., H:]
+        d = seq.selective_scan_backward(dy, s["c"], s["dt"], self.A, q[..., Rk:Rk + S], q[..., Rk + S:], s["saved"], D=self.D, z=z, dt_bias=self.bias)
+        g["A"], g["D"], g["bias"] = d.dA, d.dD, d.ddt_bias
+        dlow, g["w_dt"], _ = seq.linear_backward(d.ddt, q[..., :Rk], self.w_dt, need_db=False)
+        dc, g["w_x"], _ = seq.linear_backward(torch.cat([dlow, d.dB, d.dC], -1), s["c"], self.w_x, residual=d.du, need_db=False)
+        dx, g["cw"], g["cb"], _ = seq.causal_conv_backward(dc, s["xz"][..., :H], self.cw, self.cb, activation="silu")
+        dn, g["w_in"], _ = seq.linear_backward(torch.cat([dx, d.dz], -1), s["n"], self.w_in, need_db=False)
+        dx, g["gamma"], g["beta"] = seq.layer_norm_backward(dn, s["x"], s["mean"], s["rstd"], self.gamma)
+        return dx + dout, g
+
+    def step(self, x, conv, h):
+        xz = seq.linear(seq.layer_norm(x, self.gamma, self.beta), self.w_in)
+        c = seq.causal_conv_step(xz[:, :self.H], conv, self.cw, self.cb, activation="silu")
+        q = seq.linear(c, self.w_x)
+        dt = seq.linear(q[:, :self.R], self.w_dt)
+        y = seq.selective_scan_step(c, dt, self.A, q[:, self.R:self.R + self.S], q[:, self.R + self.S:], h, D=self.D, z=xz[:, self.H:], dt_bias=self.bias)
+        return seq.linear(y, self.w_out, residual=x)
+
+
+def test_mixer_block_forward_backward_and_row_by_row():
+    """The operators in a row, in 32 bits: outputs, all gradients, and a prompt continued row by row."""
+    g = gen(41)
+    B, L, D = 2, 37, 24
+    m = Mixer(g, D, 48, 16, 8, 4, torch.float32)
+    x, dout = rnd(g, B, L, D), rnd(g, B, L, D)
+    m64 = m.to(lambda t: t.double().requires_grad_())
+    x64 = x.double().requires_grad_()
+    out, last = m64.reference(x64)
+    want = torch.autograd.grad(out, [x64] + [getattr(m64, n) for n in m.names()], dout.double())
+    mc = m.to(lambda t: t.cuda())
+    got, s = mc.prompt(x.cuda())
+    # about 400 roundings stand on the longest path (the sums of 24 .. 64 terms of six products, 37 rows of 20 each), each carried on by
+    # factors of order one between stages: 2^-24 x 400 x 8 = 2e-4 of the largest value
+    def near(a, b, what):
+        a, b = a.detach().double().cpu(), b.detach()
+        assert float((a - b).abs().max()) <= 2e-4 * float(b.abs().max()), (what, float((a - b).abs().max()), float(b.abs().max()))
+    near(got, out, "out")
+    near(s["h"], last, "state")
+    dx, gr = mc.backward(dout.cuda(), s)
+    near(dx, want[0], "dx")
+    for n, w in zip(m.names(), want[1:]):
+        near(gr[n], w, n)
+    head, s2 = mc.prompt(x[:, :20].contiguous().cuda())
+    near(head, out[:, :20], "prompt")
+    conv, h = s2["conv"], s2["h"]
+    for t in range(20, L):
+        near(mc.step(x[:, t].cuda(), conv, h), out[:, t], f"row {t}")
+    near(h, last, "state row by row")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_mixer_block_in_a_graph(dtype):
+    """Forward and backward captured once and replayed on changing inputs, eager work of the same kind between the replays; and two graphs
+    of the same operators that replay in turn (their workspaces are their own)."""
+    g = gen(43)
+    B, L, D = 2, 130, 64
+    m = Mixer(g, D, 128, 16, 8, 4, dtype).to(lambda t: t.cuda())
+    xs = [rnd(g, B, L, D, dtype=dtype).cuda() for _ in range(4)]
+    douts = [rnd(g, B, L, D, dtype=dtype).cuda() for _ in range(4)]
+
+    def work(x, dout):
+        out, s = m.prompt(x)
+        dx, gr = m.backward(dout, s)
+        return [out, s["h"], dx] + [gr[n] for n in m.names()]
+    want = [[t.clone() for t in work(x, d)] for x, d in zip(xs, douts)]
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        x, d = xs[0].clone(), douts[0].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            work(x, d)
+        torch.cuda.current_stream().wait_stream(side)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = work(x, d)
+        graphs.append((gr, x, d, res))
+    for k in range(8):
+        gr, x, d, res = graphs[k % 2]
+        x.copy_(xs[k % 4])
+        d.copy_(douts[k % 4])
+        gr.replay()
+        if k % 3 == 0:
+            work(xs[(k + 1) % 4], douts[(k + 1) % 4])
+            torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(res, want[k % 4])), k
+
+
+def test_two_streams_at_once():
+    g = gen(44)
+    m = Mixer(g, 64, 128, 16, 8, 4, torch.float16).to(lambda t: t.cuda())
+    xs = [rnd(g, 2, 200, 64, dtype=torch.float16).cuda() for _ in range(2)]
+    want = [m.prompt(x)[0].clone() for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(m.prompt(xs[k])[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[k]) for k in range(2) for y in got[k])

@@ -22,5 +22,13 @@ from .harness import (EarlyStopping, ModelCheckpoint, ReduceLROnPlateau, fit, ma
 __all__ = ["Graph", "Node", "ParamSpec", "Sym", "unet_model_builder", "model_selector", "ENCODER_METHODS",
            "SUPPORTED_DECODERS", "builders1d", "BCDUNet", "UNet1D", "harness", "EarlyStopping", "ModelCheckpoint",
            "ReduceLROnPlateau", "fit", "masks_from_predictions", "mask_grey_levels", "predict_directory", "data",
-           "CustomDataGenerator", "prepare_train_dict", "create_patches", "patchify", "unpatchify", "keras_map", "keras_file", "keras_import", "h5lite", "load_model"]
+           "CustomDataGenerator", "prepare_train_dict", "create_patches", "patchify", "unpatchify", "keras_map", "keras_file", "keras_import", "h5lite", "load_model", "sequence"]
 __version__ = "0.1.0"
+
+
+def __getattr__(name):
+    """`sequence` (the sequence operators) works on torch tensors: it is imported on first use, graph construction needs no torch."""
+    if name == "sequence":
+        import importlib
+        return importlib.import_module(".sequence", __name__)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

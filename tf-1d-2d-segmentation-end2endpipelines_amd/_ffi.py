@@ -16,6 +16,10 @@ MAX_SEG, MAX_TAPS, MAX_CLS = 8, 32, 4
 SEG_VARIANT_A_HI = SEG_VARIANT_IN_HI = 0x1000          # include/seg_hip.h
 SEG_VARIANT_DZ_HI = SEG_VARIANT_B_HI = 0x2000
 ACT = {None: 0, "none": 0, "linear": 0, "relu": 1, "leaky_relu": 2, "sigmoid": 3, "softmax": 4}
+# the sequence operators (sequence.py): SEG_ACT_SILU / SEG_ACT_GELU exist there only
+SEQ_ACT = {None: 0, "none": 0, "linear": 0, "relu": 1, "leaky_relu": 2, "sigmoid": 3, "silu": 5, "gelu": 6}
+DT_F16, DT_BF16, DT_F32 = 0, 1, 2
+LINEAR_FWD, LINEAR_BWD_DATA, LINEAR_BWD_WEIGHT = 0, 1, 2
 LOSS = {"mse": 0, "bce": 1, "cce": 2, "mae": 3, "mape": 4, "msle": 5, "huber": 6, "logcosh": 7, "poisson": 8, "hinge": 9,
         "squared_hinge": 10, "binary_focal": 11, "kld": 12, "categorical_hinge": 13, "cosine": 14, "sparse_cce": 15}
 # the names `TFOptimizers(name, lr).optimizer()` takes (2DCNN/utils/tf_optimizers.py:10-26); Adam has its own entry points
@@ -97,6 +101,32 @@ class HeadInject(C.Structure):
 
 i32, i64, f32, vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
 
+
+class LinearArgs(C.Structure):
+    """seg_linear_args (include/seg_hip.h), field order as declared."""
+    _fields_ = [("M", i64), ("N", i32), ("K", i32), ("dtype", i32), ("act", i32), ("alpha", f32), ("x", vp), ("x_ld", i64), ("w", vp), ("w_ld", i64),
+                ("bias", vp), ("residual", vp), ("residual_ld", i64), ("z", vp), ("z_ld", i64), ("y", vp), ("y_ld", i64), ("dy", vp), ("dy_ld", i64),
+                ("dw", vp), ("dw_ld", i64), ("db", vp), ("workspace", vp)]
+
+
+class CausalConvArgs(C.Structure):
+    """seg_causal_conv_args."""
+    _fields_ = [("B", i32), ("L", i32), ("D", i32), ("K", i32), ("dtype", i32), ("act", i32), ("x", vp), ("x_bs", i64), ("x_ld", i64), ("w", vp),
+                ("bias", vp), ("state", vp), ("lengths", vp), ("y", vp), ("y_bs", i64), ("y_ld", i64), ("state_out", vp), ("dy", vp), ("dy_bs", i64),
+                ("dy_ld", i64), ("dstate_out", vp), ("dx", vp), ("dx_bs", i64), ("dx_ld", i64), ("dw", vp), ("db", vp), ("dstate", vp), ("workspace", vp)]
+
+
+def _strided(*names):
+    return [f for n in names for f in ((n, vp), (n + "_bs", i64), (n + "_ld", i64))]
+
+
+class ScanArgs(C.Structure):
+    """seg_scan_args."""
+    _fields_ = ([(n, i32) for n in ("B", "L", "D", "S", "dtype", "softplus")] + _strided("u", "dt", "z", "Bm", "Cm") +
+                [(n, vp) for n in ("A", "Dskip", "dt_bias", "state", "lengths")] + _strided("y") + [("state_out", vp), ("saved", vp)] + _strided("dy") +
+                [("dstate_out", vp)] + _strided("du", "ddt", "dz", "dBm", "dCm") + [(n, vp) for n in ("dA", "dD", "ddt_bias", "dstate", "workspace")])
+
+
 _PROTOS = {
     "seg_abi_version": ([], C.c_int),
     "seg_igemm_fwd": ([C.POINTER(IgemmFwdArgs), vp], C.c_int),
@@ -159,6 +189,24 @@ _PROTOS = {
     "seg_cast_f32_split": ([vp, vp, i64, vp], C.c_int),
     "seg_pack_input": ([vp, vp, i64, i32, i32, vp, vp], C.c_int),
     "seg_unpack_f32": ([vp, vp, i64, i32, i32, i32, vp], C.c_int),
+    "seg_layernorm_fwd": ([vp, i64, vp, i64, i64, i32, i32, vp, vp, f32, vp, vp, vp], C.c_int),
+    "seg_layernorm_bwd_workspace_bytes": ([i64, i32, i32], C.c_int64),
+    "seg_layernorm_bwd": ([vp, i64, vp, i64, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp], C.c_int),
+    "seg_linear_workspace_bytes": ([C.POINTER(LinearArgs), i32], C.c_int64),
+    "seg_linear_fwd": ([C.POINTER(LinearArgs), vp], C.c_int),
+    "seg_linear_bwd_data": ([C.POINTER(LinearArgs), vp], C.c_int),
+    "seg_linear_bwd_weight": ([C.POINTER(LinearArgs), vp], C.c_int),
+    "seg_linear_act_bwd": ([vp, i64, vp, i64, vp, i64, i64, i32, i32, i32, f32, vp], C.c_int),
+    "seg_causal_conv_fwd": ([C.POINTER(CausalConvArgs), vp], C.c_int),
+    "seg_causal_conv_bwd_workspace_bytes": ([C.POINTER(CausalConvArgs)], C.c_int64),
+    "seg_causal_conv_bwd": ([C.POINTER(CausalConvArgs), vp], C.c_int),
+    "seg_causal_conv_step": ([C.POINTER(CausalConvArgs), vp], C.c_int),
+    "seg_selective_scan_saved_bytes": ([C.POINTER(ScanArgs)], C.c_int64),
+    "seg_selective_scan_fwd_workspace_bytes": ([C.POINTER(ScanArgs)], C.c_int64),
+    "seg_selective_scan_bwd_workspace_bytes": ([C.POINTER(ScanArgs)], C.c_int64),
+    "seg_selective_scan_fwd": ([C.POINTER(ScanArgs), vp], C.c_int),
+    "seg_selective_scan_bwd": ([C.POINTER(ScanArgs), vp], C.c_int),
+    "seg_selective_scan_step": ([C.POINTER(ScanArgs), vp], C.c_int),
 }
 
 # entry points that touch activation tensors exist twice: fp16 (throughput mode) and *_f32 (parity mode: split fp16 pairs, 4 B per element)

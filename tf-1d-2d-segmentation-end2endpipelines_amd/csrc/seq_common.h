@@ -1,0 +1,126 @@
+// Shared pieces of the sequence operators (seq_norm.hip, seq_linear.hip, seq_scan.hip): element types fp16 / bf16 / fp32, vector
+// access with a scalar form for rows that no 16-byte access fits, activations, and the ordered reduction of per-block partial rows.
+#pragma once
+#include "seg_common.h"
+#include <math.h>
+#include <type_traits>
+
+namespace {
+
+typedef __bf16 bf16_t;
+typedef bf16_t b8 __attribute__((ext_vector_type(8)));
+
+// eight consecutive elements <-> eight floats.  VEC: 16-byte accesses (32 bytes in fp32: two); else one element at a time, of which
+// the first n (<= 8) exist - the others read as zero and are not written
+template <typename T> __device__ __forceinline__ void vload8(const T* p, float* f) {
+  if constexpr (std::is_same<T, float>::value) {
+    load8<float>(p, f);
+  } else if constexpr (std::is_same<T, half_t>::value) {
+    unpack8(ld16(p), f);
+  } else {
+    const u4 v = ld16(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(v[i] << 16);
+      f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ void vstore8(T* p, const float* f) {
+  if constexpr (std::is_same<T, float>::value) {
+    store8<float>(p, f);
+  } else if constexpr (std::is_same<T, half_t>::value) {
+    st16(p, pack8(f));
+  } else {
+    b8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (bf16_t)f[i];
+    st16(p, __builtin_bit_cast(u4, v));
+  }
+}
+template <typename T, bool VEC> __device__ __forceinline__ void row_load8(const T* p, int n, float* f) {
+  if constexpr (VEC) {
+    if (n > 0) {
+      vload8(p, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < n ? (float)p[i] : 0.f;
+  }
+}
+template <typename T, bool VEC> __device__ __forceinline__ void row_store8(T* p, int n, const float* f) {
+  if constexpr (VEC) {
+    if (n > 0) vstore8(p, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (T)f[i];
+  }
+}
+
+__device__ __forceinline__ float sigmoid_f(float v) { return 1.f / (1.f + __expf(-v)); }
+
+__device__ __forceinline__ float seq_act(float v, int act, float alpha) {
+  switch (act) {
+    case SEG_ACT_RELU: return v > 0.f ? v : 0.f;
+    case SEG_ACT_LEAKY: return v > 0.f ? v : v * alpha;
+    case SEG_ACT_SIGMOID: return sigmoid_f(v);
+    case SEG_ACT_SILU: return v * sigmoid_f(v);
+    case SEG_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    default: return v;
+  }
+}
+// derivative from the activation's INPUT
+__device__ __forceinline__ float seq_act_slope(float v, int act, float alpha) {
+  switch (act) {
+    case SEG_ACT_RELU: return v > 0.f ? 1.f : 0.f;
+    case SEG_ACT_LEAKY: return v > 0.f ? 1.f : alpha;
+    case SEG_ACT_SIGMOID: { const float s = sigmoid_f(v); return s * (1.f - s); }
+    case SEG_ACT_SILU: { const float s = sigmoid_f(v); return s * (1.f + v * (1.f - s)); }
+    case SEG_ACT_GELU: return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * __expf(-0.5f * v * v) * 0.39894228040143268f;
+    default: return 1.f;
+  }
+}
+
+// out[c] = sum over parts of part[p][c], fixed order: 16 columns x 16 parts per 256 threads, each thread its parts in turn
+constexpr int CR_COLS = 16;
+__global__ __launch_bounds__(256) void colsum_parts_kernel(const float* part, int64_t nparts, int64_t ld, int64_t cols, float* out) {
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * CR_COLS + c;
+  float s = 0.f;
+  if (col < cols)
+    for (int64_t p = r; p < nparts; p += 16) s += part[p * ld + col];
+  __shared__ float sh[16][17];
+  sh[r][c] = s;
+  __syncthreads();
+  if (r == 0 && col < cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += sh[i][c];
+    out[col] = t;
+  }
+}
+inline void launch_colsum_parts(const float* part, int64_t nparts, int64_t ld, int64_t cols, float* out, hipStream_t st) {
+  hipLaunchKernelGGL(colsum_parts_kernel, dim3((unsigned)((cols + CR_COLS - 1) / CR_COLS)), dim3(256), 0, st, part, nparts, ld, cols, out);
+}
+
+inline size_t dt_size(int dt) { return dt == SEG_DT_F32 ? 4 : 2; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// whether 8-element vector accesses fit a tensor's rows (NULL: not there, fits)
+inline bool vec_ok(const void* p, int64_t ld, int64_t bs, int dt) {
+  const int64_t u = dt == SEG_DT_F32 ? 4 : 8;
+  return p == nullptr || (aligned16(p) && ld % u == 0 && bs % u == 0);
+}
+
+template <typename F>
+inline int seq_dispatch_dtype(int dt, F&& f) {
+  if (dt == SEG_DT_F16) f((half_t*)nullptr);
+  else if (dt == SEG_DT_BF16) f((bf16_t*)nullptr);
+  else f((float*)nullptr);
+  return 0;
+}
+
+}  // namespace

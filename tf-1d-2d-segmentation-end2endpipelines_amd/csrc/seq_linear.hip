@@ -1,0 +1,383 @@
+// Matrix product with its epilogue and its two gradients (seg_linear_fwd / _bwd_data / _bwd_weight).  All three are
+//   C[i][j] = sum_k A(i, k) B(j, k)
+// with the operands as the caller stores them:
+//   pass            i        j        k       A             B
+//   fwd             rows     units    inputs  x  [i][k]     w [j][k]      z = C + bias, y = act(z) + residual
+//   bwd_data        rows     inputs   units   dy [i][k]     w [k][j]      y = C act'(z) + residual
+//   bwd_weight      units    inputs   rows    dy [k][i]     x [k][j]      dw = C (fp32)
+#include "seq_common.h"
+#include "igemm_common.h"
+
+namespace {
+
+constexpr int TPB = 256;
+
+struct GemmArgs {
+  const void *A, *B;
+  int64_t a_ld, b_ld;
+  int64_t I, Kd;
+  int J;
+  int ti, tj;                    // tiles along i and j
+  int splits;                    // ranges of k contracted by different blocks
+  int64_t kper;                  // their length (a multiple of the K step)
+  float* part;                   // [splits][I][J] when splits > 1
+  int act;
+  float alpha;
+  const float* bias;
+  const void* res; int64_t res_ld;
+  void* z; int64_t z_ld;
+  void* out; int64_t out_ld;
+};
+
+// one element of the result through the pass's epilogue
+template <int PASS, typename T> __device__ __forceinline__ void epilogue1(const GemmArgs& p, int64_t i, int j, float v) {
+  if constexpr (PASS == SEG_LINEAR_BWD_WEIGHT) {
+    ((float*)p.out)[i * p.out_ld + j] = v;
+  } else {
+    if constexpr (PASS == SEG_LINEAR_FWD) {
+      if (p.bias != nullptr) v += p.bias[j];
+      if (p.z != nullptr) ((T*)p.z)[i * p.z_ld + j] = (T)v;
+      v = seq_act(v, p.act, p.alpha);
+    } else {
+      if (p.z != nullptr) v *= seq_act_slope((float)((const T*)p.z)[i * p.z_ld + j], p.act, p.alpha);
+    }
+    if (p.res != nullptr) v += (float)((const T*)p.res)[i * p.res_ld + j];
+    ((T*)p.out)[i * p.out_ld + j] = (T)v;
+  }
+}
+
+// ---- the kernel for every size, stride and type: 64 x 64 tiles, operands through registers into k-contiguous LDS rows (an operand
+// whose memory is contiguous along i / j is transposed on its way), four waves of one 32 x 32 tile each.  VEC: elements per memory
+// access - what the addresses' alignment allows; the ends of rows and of k go element by element.
+template <typename T> struct AnyStep { static constexpr int BK = 32, EPT = 8, LD = 40; };
+template <> struct AnyStep<float> { static constexpr int BK = 16, EPT = 4, LD = 20; };
+
+template <typename T, int VEC> __device__ __forceinline__ void load_elems(const T* p, int64_t n, T* r) {
+  constexpr int EPT = AnyStep<T>::EPT;
+  typedef T vec __attribute__((ext_vector_type(VEC)));
+  if (VEC > 1 && n >= EPT) {
+#pragma unroll
+    for (int q = 0; q < EPT / VEC; ++q) {
+      const vec v = *reinterpret_cast<const vec*>(p + q * VEC);
+#pragma unroll
+      for (int t = 0; t < VEC; ++t) r[q * VEC + t] = v[t];
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < EPT; ++t) r[t] = t < n ? p[t] : (T)0.f;
+  }
+}
+
+template <int PASS, typename T, int VEC>
+__global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
+  typedef AnyStep<T> S;
+  constexpr bool AKC = PASS != SEG_LINEAR_BWD_WEIGHT, BKC = PASS == SEG_LINEAR_FWD;
+  __shared__ __align__(16) T smem[2][2][64 * S::LD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 31, fh = lane >> 5;
+  const int t = xcd_remap(blockIdx.x, p.ti * p.tj);
+  const int64_t i0 = (int64_t)(t / p.tj) * 64;
+  const int j0 = (t % p.tj) * 64;
+  const int64_t kbeg = blockIdx.y * p.kper, kend = kbeg + p.kper < p.Kd ? kbeg + p.kper : p.Kd;
+  constexpr int KCH = S::BK / S::EPT, ICH = 64 / S::EPT;       // chunks per k-contiguous / i-contiguous row
+  const T *A = (const T*)p.A, *B = (const T*)p.B;
+  T ra[S::EPT], rb[S::EPT];
+  auto fetch = [&](const T* base, int64_t ld, bool kc, int64_t r0, int64_t rend, int64_t k, T* r) {
+    if (kc) {
+      const int64_t row = r0 + tid / KCH, kk = k + (tid % KCH) * S::EPT;
+      load_elems<T, VEC>(base + row * ld + kk, row < rend ? kend - kk : 0, r);
+    } else {
+      const int64_t kk = k + tid / ICH, row = r0 + (tid % ICH) * S::EPT;
+      load_elems<T, VEC>(base + kk * ld + row, kk < kend ? rend - row : 0, r);
+    }
+  };
+  auto put = [&](T* s, bool kc, const T* r) {
+    if (kc) {
+      T* d = s + (tid / KCH) * S::LD + (tid % KCH) * S::EPT;
+#pragma unroll
+      for (int e = 0; e < S::EPT; ++e) d[e] = r[e];
+    } else {
+      T* d = s + (tid % ICH) * S::EPT * S::LD + tid / ICH;
+#pragma unroll
+      for (int e = 0; e < S::EPT; ++e) d[e * S::LD] = r[e];
+    }
+  };
+  f16v acc;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) acc[q] = 0.f;
+  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+  fetch(A, p.a_ld, AKC, i0, p.I, kbeg, ra);
+  fetch(B, p.b_ld, BKC, j0, p.J, kbeg, rb);
+  int buf = 0;
+  for (int64_t k = kbeg; k < kend; k += S::BK, buf ^= 1) {
+    put(smem[buf][0], AKC, ra);
+    put(smem[buf][1], BKC, rb);
+    __syncthreads();
+    if (k + S::BK < kend) {
+      fetch(A, p.a_ld, AKC, i0, p.I, k + S::BK, ra);
+      fetch(B, p.b_ld, BKC, j0, p.J, k + S::BK, rb);
+    }
+    const T *sa = smem[buf][0] + (wi + fr) * S::LD, *sb = smem[buf][1] + (wj + fr) * S::LD;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int ks = 0; ks < S::BK / 2; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(sa[2 * ks + fh], sb[2 * ks + fh], acc, 0, 0, 0);
+    } else if constexpr (std::is_same<T, half_t>::value) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8*>(sa + ks * 16 + fh * 8), *reinterpret_cast<const h8*>(sb + ks * 16 + fh * 8), acc, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const b8*>(sa + ks * 16 + fh * 8), *reinterpret_cast<const b8*>(sb + ks * 16 + fh * 8), acc, 0, 0, 0);
+    }
+    // the buffer written next is the one whose readers passed the barrier above
+  }
+  const int j = j0 + wj + fr;
+  if (j < p.J) {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const int64_t i = i0 + wi + (q & 3) + 8 * (q >> 2) + 4 * fh;
+      if (i < p.I) {
+        if (p.splits > 1) p.part[((int64_t)blockIdx.y * p.I + i) * p.J + j] = acc[q];
+        else epilogue1<PASS, T>(p, i, j, acc[q]);
+      }
+    }
+  }
+}
+
+// the split ranges of k added in order, then the epilogue
+template <int PASS, typename T>
+__global__ __launch_bounds__(TPB) void gemm_join_kernel(const GemmArgs p) {
+  const int64_t n = p.I * p.J;
+  for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < n; e += (int64_t)gridDim.x * TPB) {
+    float v = 0.f;
+    for (int s = 0; s < p.splits; ++s) v += p.part[s * n + e];
+    const int64_t i = e / p.J;
+    epilogue1<PASS, T>(p, i, (int)(e - i * p.J), v);
+  }
+}
+
+// ---- bias gradient: column sums of dy, rows in ranges of blocks (part[range][N], added up in order by colsum_parts_kernel)
+template <typename T, bool VEC>
+__global__ __launch_bounds__(TPB) void colsum_rows_kernel(const T* dy, int64_t ld, int64_t rows, int cols, int64_t per, float* part) {
+  const int l = threadIdx.x & 31, r = threadIdx.x >> 5, c = (blockIdx.x * 32 + l) * 8;
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = 0.f;
+  const int64_t beg = blockIdx.y * per, end = beg + per < rows ? beg + per : rows;
+  if (c < cols)
+    for (int64_t i = beg + r; i < end; i += 8) {
+      float f[8];
+      row_load8<T, VEC>(dy + i * ld + c, cols - c, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += f[j];
+    }
+  __shared__ float sh[8][32][9];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sh[r][l][j] = s[j];
+  __syncthreads();
+  const int ol = threadIdx.x >> 3, oj = threadIdx.x & 7, oc = (blockIdx.x * 32 + ol) * 8 + oj;
+  if (oc < cols) {
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += sh[q][ol][oj];
+    part[(int64_t)blockIdx.y * cols + oc] = v;
+  }
+}
+struct ColsumPlan { int64_t per, parts; };
+inline ColsumPlan colsum_plan(int64_t rows, int cols) {
+  const int64_t cb = (cols + 255) / 256, want = (1024 + cb - 1) / cb;
+  int64_t per = (rows + want - 1) / want;
+  per = (per + 31) / 32 * 32;
+  return {per, (rows + per - 1) / per};
+}
+
+// ---- plans
+struct GemmPlan { int tile; int ti, tj, splits; int64_t kper; };
+inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype) {
+  GemmPlan g;
+  g.tile = 64;
+  g.ti = (int)((I + 63) / 64);
+  g.tj = (J + 63) / 64;
+  const int64_t tiles = (int64_t)g.ti * g.tj;
+  // fewer tiles than the card has room for: k is split, down to 256 of it per block
+  int64_t s = tiles >= 512 || tiles == 0 ? 1 : 1024 / tiles;
+  if (s > Kd / 256) s = Kd / 256;
+  if (s > 32) s = 32;
+  if (s < 1) s = 1;
+  const int64_t step = dtype == SEG_DT_F32 ? 16 : 32;
+  g.kper = ((Kd + s - 1) / s + step - 1) / step * step;
+  g.splits = g.kper > 0 ? (int)((Kd + g.kper - 1) / g.kper) : 1;
+  if (g.splits < 1) g.splits = 1;
+  return g;
+}
+
+struct Extents { int64_t I, Kd; int J; };
+inline Extents extents(const seg_linear_args& a, int pass) {
+  if (pass == SEG_LINEAR_BWD_WEIGHT) return {a.N, a.M, a.K};
+  return {a.M, a.K, a.N};
+}
+
+inline int vec_of(const void* A, int64_t a_ld, const void* B, int64_t b_ld, int dt) {
+  const int es = (int)dt_size(dt);
+  for (int v = dt == SEG_DT_F32 ? 4 : 8; v > 1; v >>= 1) {
+    if (v == 2) break;
+    if ((uintptr_t)A % (v * es) == 0 && (uintptr_t)B % (v * es) == 0 && a_ld % v == 0 && b_ld % v == 0) return v;
+  }
+  return 1;
+}
+
+template <int PASS>
+int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
+  const Extents e = extents(a, PASS);
+  const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a.dtype);
+  p.I = e.I; p.J = e.J; p.Kd = e.Kd;
+  p.ti = g.ti; p.tj = g.tj; p.splits = g.splits; p.kper = g.kper;
+  p.part = (float*)a.workspace;
+  p.act = a.act; p.alpha = a.alpha;
+  const dim3 grid((unsigned)(g.ti * g.tj), (unsigned)g.splits);
+  const int vec = vec_of(p.A, p.a_ld, p.B, p.b_ld, a.dtype);
+  seq_dispatch_dtype(a.dtype, [&](auto* tp) {
+    typedef typename std::remove_pointer<decltype(tp)>::type T;
+    if (vec == 4) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 4>), grid, dim3(TPB), 0, st, p);
+    else if (vec == 8) {
+      if constexpr (!std::is_same<T, float>::value) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 8>), grid, dim3(TPB), 0, st, p);
+    } else hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 1>), grid, dim3(TPB), 0, st, p);
+    if (g.splits > 1) {
+      const int64_t blocks = (p.I * p.J + TPB - 1) / TPB;
+      hipLaunchKernelGGL((gemm_join_kernel<PASS, T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(TPB), 0, st, p);
+    }
+  });
+  return SEG_OK;
+}
+
+int check_linear(const seg_linear_args* a, int pass, const char* name) {
+  SEG_CHECK_ARG(a != nullptr, "%s: args is NULL", name);
+  SEG_CHECK_ARG(a->dtype >= SEG_DT_F16 && a->dtype <= SEG_DT_F32, "%s: dtype %d", name, a->dtype);
+  SEG_CHECK_ARG(a->M >= 0 && a->N > 0 && a->K > 0, "%s: M %lld, N %d, K %d", name, (long long)a->M, a->N, a->K);
+  SEG_CHECK_ARG(a->act == SEG_ACT_NONE || a->act == SEG_ACT_RELU || a->act == SEG_ACT_LEAKY || a->act == SEG_ACT_SIGMOID || a->act == SEG_ACT_SILU || a->act == SEG_ACT_GELU,
+                "%s: activation %d", name, a->act);
+  const Extents e = extents(*a, pass);
+  SEG_CHECK_ARG(((e.I + 63) / 64) * ((int64_t)(e.J + 63) / 64) < (int64_t)1 << 24, "%s: result of %lld x %d is too large for one call", name, (long long)e.I, e.J);
+  const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a->dtype);
+  SEG_CHECK_ARG(a->M == 0 || g.splits <= 1 || a->workspace != nullptr, "%s: workspace is NULL (%lld bytes are needed)", name, (long long)seg_linear_workspace_bytes(a, pass));
+  return SEG_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t seg_linear_workspace_bytes(const seg_linear_args* a, int32_t pass) {
+  if (a == nullptr || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
+  const Extents e = extents(*a, pass);
+  const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a->dtype);
+  int64_t b = g.splits > 1 ? (int64_t)g.splits * e.I * e.J * 4 : 0;
+  if (pass == SEG_LINEAR_BWD_WEIGHT) {
+    const int64_t c = colsum_plan(a->M, a->N).parts * a->N * 4;
+    b = (b + 15) / 16 * 16 + c;
+  }
+  return b;
+}
+
+extern "C" int seg_linear_fwd(const seg_linear_args* a, seg_stream_t stream) {
+  if (int rc = check_linear(a, SEG_LINEAR_FWD, "linear_fwd")) return rc;
+  if (a->M == 0) return SEG_OK;
+  SEG_CHECK_ARG(a->x != nullptr && a->w != nullptr && a->y != nullptr, "linear_fwd: x / w / y is NULL");
+  SEG_CHECK_ARG((a->M == 1 || a->x_ld >= a->K) && (a->N == 1 || a->w_ld >= a->K), "linear_fwd: row strides below K = %d", a->K);
+  SEG_CHECK_ARG(a->M == 1 || (a->y_ld >= a->N && (a->z == nullptr || a->z_ld >= a->N) && (a->residual == nullptr || a->residual_ld >= 0)),
+                "linear_fwd: row strides below N = %d", a->N);
+  GemmArgs p = {};
+  p.A = a->x; p.a_ld = a->x_ld; p.B = a->w; p.b_ld = a->w_ld;
+  p.bias = a->bias; p.res = a->residual; p.res_ld = a->residual_ld; p.z = a->z; p.z_ld = a->z_ld; p.out = a->y; p.out_ld = a->y_ld;
+  run_gemm<SEG_LINEAR_FWD>(*a, p, (hipStream_t)stream);
+  SEG_CHECK_LAUNCH("linear_fwd");
+  return SEG_OK;
+}
+
+extern "C" int seg_linear_bwd_data(const seg_linear_args* a, seg_stream_t stream) {
+  if (int rc = check_linear(a, SEG_LINEAR_BWD_DATA, "linear_bwd_data")) return rc;
+  SEG_CHECK_ARG(a->bias == nullptr, "linear_bwd_data: takes no bias");
+  if (a->M == 0) return SEG_OK;
+  SEG_CHECK_ARG(a->x != nullptr && a->w != nullptr && a->y != nullptr, "linear_bwd_data: x / w / y is NULL");
+  SEG_CHECK_ARG((a->M == 1 || a->x_ld >= a->K) && (a->K == 1 || a->w_ld >= a->N), "linear_bwd_data: row strides of x below %d or of w below %d", a->K, a->N);
+  SEG_CHECK_ARG(a->M == 1 || (a->y_ld >= a->N && (a->z == nullptr || a->z_ld >= a->N) && (a->residual == nullptr || a->residual_ld >= 0)),
+                "linear_bwd_data: row strides below N = %d", a->N);
+  GemmArgs p = {};
+  p.A = a->x; p.a_ld = a->x_ld; p.B = a->w; p.b_ld = a->w_ld;
+  p.res = a->residual; p.res_ld = a->residual_ld; p.z = a->z; p.z_ld = a->z_ld; p.out = a->y; p.out_ld = a->y_ld;
+  run_gemm<SEG_LINEAR_BWD_DATA>(*a, p, (hipStream_t)stream);
+  SEG_CHECK_LAUNCH("linear_bwd_data");
+  return SEG_OK;
+}
+
+extern "C" int seg_linear_bwd_weight(const seg_linear_args* a, seg_stream_t stream) {
+  if (int rc = check_linear(a, SEG_LINEAR_BWD_WEIGHT, "linear_bwd_weight")) return rc;
+  SEG_CHECK_ARG(a->M == 0 || (a->dy != nullptr && (a->dw == nullptr || a->x != nullptr)), "linear_bwd_weight: dy / x is NULL");
+  SEG_CHECK_ARG(a->M <= 1 || (a->dy_ld >= a->N && (a->dw == nullptr || a->x_ld >= a->K)), "linear_bwd_weight: row strides below N = %d / K = %d", a->N, a->K);
+  SEG_CHECK_ARG(a->dw == nullptr || a->N == 1 || a->dw_ld >= a->K, "linear_bwd_weight: dw_ld below K = %d", a->K);
+  SEG_CHECK_ARG(a->db == nullptr || a->M == 0 || a->workspace != nullptr, "linear_bwd_weight: db needs the workspace");
+  hipStream_t st = (hipStream_t)stream;
+  if (a->dw != nullptr) {
+    GemmArgs p = {};
+    p.A = a->dy; p.a_ld = a->dy_ld; p.B = a->x; p.b_ld = a->x_ld; p.out = a->dw; p.out_ld = a->dw_ld;
+    run_gemm<SEG_LINEAR_BWD_WEIGHT>(*a, p, st);       // (M = 0: an empty sum, zeros are stored)
+  }
+  if (a->db != nullptr) {
+    const Extents e = extents(*a, SEG_LINEAR_BWD_WEIGHT);
+    const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a->dtype);
+    const int64_t off = g.splits > 1 ? ((int64_t)g.splits * e.I * e.J * 4 + 15) / 16 * 16 : 0;
+    float* part = (float*)((char*)a->workspace + off);
+    const ColsumPlan c = a->M > 0 ? colsum_plan(a->M, a->N) : ColsumPlan{0, 0};
+    if (a->M > 0)
+      seq_dispatch_dtype(a->dtype, [&](auto* tp) {
+        typedef typename std::remove_pointer<decltype(tp)>::type T;
+        const dim3 grid((a->N + 255) / 256, (unsigned)c.parts);
+        if (a->N % 8 == 0 && vec_ok(a->dy, a->dy_ld, 0, a->dtype))
+          hipLaunchKernelGGL((colsum_rows_kernel<T, true>), grid, dim3(TPB), 0, st, (const T*)a->dy, a->dy_ld, a->M, a->N, c.per, part);
+        else
+          hipLaunchKernelGGL((colsum_rows_kernel<T, false>), grid, dim3(TPB), 0, st, (const T*)a->dy, a->dy_ld, a->M, a->N, c.per, part);
+      });
+    launch_colsum_parts(part, c.parts, a->N, a->N, a->db, st);
+  }
+  SEG_CHECK_LAUNCH("linear_bwd_weight");
+  return SEG_OK;
+}
+
+namespace {
+template <typename T, bool VEC>
+__global__ __launch_bounds__(TPB) void act_bwd_kernel(const T* dy, int64_t dy_ld, const T* z, int64_t z_ld, T* dx, int64_t dx_ld, int64_t rows, int C,
+                                                      int act, float alpha) {
+  const int chunks = (C + 7) / 8;
+  const int64_t n = rows * chunks;
+  for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < n; e += (int64_t)gridDim.x * TPB) {
+    const int64_t r = e / chunks;
+    const int c = (int)(e - r * chunks) * 8;
+    float d[8], v[8];
+    row_load8<T, VEC>(dy + r * dy_ld + c, C - c, d);
+    row_load8<T, VEC>(z + r * z_ld + c, C - c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] *= seq_act_slope(v[j], act, alpha);
+    row_store8<T, VEC>(dx + r * dx_ld + c, C - c, d);
+  }
+}
+}  // namespace
+
+extern "C" int seg_linear_act_bwd(const void* dy, int64_t dy_ld, const void* z, int64_t z_ld, void* dx, int64_t dx_ld, int64_t rows, int32_t C,
+                                  int32_t dtype, int32_t act, float alpha, seg_stream_t stream) {
+  SEG_CHECK_ARG(dtype >= SEG_DT_F16 && dtype <= SEG_DT_F32, "linear_act_bwd: dtype %d", dtype);
+  SEG_CHECK_ARG(rows >= 0 && C > 0, "linear_act_bwd: rows %lld, C %d", (long long)rows, C);
+  SEG_CHECK_ARG(act == SEG_ACT_NONE || act == SEG_ACT_RELU || act == SEG_ACT_LEAKY || act == SEG_ACT_SIGMOID || act == SEG_ACT_SILU || act == SEG_ACT_GELU,
+                "linear_act_bwd: activation %d", act);
+  if (rows == 0) return SEG_OK;
+  SEG_CHECK_ARG(dy != nullptr && z != nullptr && dx != nullptr, "linear_act_bwd: dy / z / dx is NULL");
+  SEG_CHECK_ARG(rows == 1 || (dy_ld >= C && z_ld >= C && dx_ld >= C), "linear_act_bwd: row strides below the %d channels", C);
+  seq_dispatch_dtype(dtype, [&](auto* tp) {
+    typedef typename std::remove_pointer<decltype(tp)>::type T;
+    const int64_t blocks = (rows * ((C + 7) / 8) + TPB - 1) / TPB;
+    const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
+    if (C % 8 == 0 && vec_ok(dy, dy_ld, 0, dtype) && vec_ok(z, z_ld, 0, dtype) && vec_ok(dx, dx_ld, 0, dtype))
+      hipLaunchKernelGGL((act_bwd_kernel<T, true>), grid, dim3(TPB), 0, (hipStream_t)stream, (const T*)dy, dy_ld, (const T*)z, z_ld, (T*)dx, dx_ld, rows, C, act, alpha);
+    else
+      hipLaunchKernelGGL((act_bwd_kernel<T, false>), grid, dim3(TPB), 0, (hipStream_t)stream, (const T*)dy, dy_ld, (const T*)z, z_ld, (T*)dx, dx_ld, rows, C, act, alpha);
+  });
+  SEG_CHECK_LAUNCH("linear_act_bwd");
+  return SEG_OK;
+}

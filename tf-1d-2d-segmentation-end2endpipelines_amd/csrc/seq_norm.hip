@@ -1,0 +1,403 @@
+// Layer normalisation of rows of channels, forward and backward (seg_layernorm_fwd / _bwd).
+//
+//   mean = sum x / C,  var = sum (x - mean)^2 / C,  y = (x - mean) rstd gamma + beta
+//   dx = rstd (g - sum g / C - xhat sum (g xhat) / C),  g = dy gamma;   dgamma = sum_rows dy xhat,  dbeta = sum_rows dy
+//
+// Bandwidth bounds both: the row is read ONCE and kept in registers, so the variance is the two-pass one (no cancellation of
+// sum x^2 - mean^2) at no traffic.  LPR lanes share a row - 8 lanes for the 64-channel rows of a full-resolution level, a wave, or
+// the whole block - with NCH chunks of 8 channels per lane; rows longer than a block's registers are walked in a loop.
+#include "seq_common.h"
+
+namespace {
+
+constexpr int TPB = 256;
+constexpr int64_t LN_REG_MAX = 256 * 8 * 8;      // longest row held in registers: 256 lanes x 8 chunks x 8 channels
+
+// sum over the LPR lanes of a row (LPR <= 64: inside the wave; 256: the block, through `sh`)
+template <int LPR> __device__ __forceinline__ float row_sum(float v, float* sh) {
+#pragma unroll
+  for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if constexpr (LPR > 64) {
+    const int w = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[w] = v;
+    __syncthreads();
+    v = sh[0] + sh[1] + sh[2] + sh[3];
+  }
+  return v;
+}
+template <int LPR> __device__ __forceinline__ void row_sum2(float& a, float& b, float* sh) {
+#pragma unroll
+  for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o);
+    b += __shfl_xor(b, o);
+  }
+  if constexpr (LPR > 64) {
+    const int w = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { sh[w] = a; sh[4 + w] = b; }
+    __syncthreads();
+    a = sh[0] + sh[1] + sh[2] + sh[3];
+    b = sh[4] + sh[5] + sh[6] + sh[7];
+  }
+}
+
+// chunk i of a lane covers channels c0 .. c0 + n: with VEC 8 consecutive ones per lane, else the lanes' channels interleave (j LPR apart)
+// so that scalar accesses of neighbouring lanes stay neighbours
+template <typename T, bool VEC, int LPR> struct Chunk {
+  int l;
+  __device__ __forceinline__ int chan(int i, int j) const { return VEC ? (l + LPR * i) * 8 + j : l + LPR * (i * 8 + j); }
+  __device__ __forceinline__ void load(const T* row, int i, int C, float* f) const {
+    if constexpr (VEC) {
+      row_load8<T, true>(row + (l + LPR * i) * 8, C - (l + LPR * i) * 8, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = chan(i, j) < C ? (float)row[chan(i, j)] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void loadf(const float* p, float none, int i, int C, float* f) const {
+    if (p == nullptr) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = none;
+    } else if constexpr (VEC) {
+      const int c = (l + LPR * i) * 8;
+      if (c < C) {
+        load8<float>(p + c, f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = chan(i, j) < C ? p[chan(i, j)] : 0.f;
+    }
+  }
+  template <typename U> __device__ __forceinline__ void store(U* row, int i, int C, const float* f) const {
+    if constexpr (VEC) {
+      row_store8<U, true>(row + (l + LPR * i) * 8, C - (l + LPR * i) * 8, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (chan(i, j) < C) row[chan(i, j)] = (U)f[j];
+    }
+  }
+};
+
+template <typename T, bool VEC, int LPR, int NCH>
+__global__ __launch_bounds__(TPB) void ln_fwd_kernel(const T* x, int64_t x_ld, T* y, int64_t y_ld, int64_t rows, int C, const float* gamma,
+                                                     const float* beta, float eps, float* mean_o, float* rstd_o) {
+  constexpr int RPB = TPB / LPR;
+  __shared__ float sh[8];
+  const Chunk<T, VEC, LPR> ck{(int)(threadIdx.x % LPR)};
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + threadIdx.x / LPR;
+    const bool live = row < rows;                 // (always where a row takes the whole block)
+    float v[NCH][8];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      ck.load(x + row * x_ld, i, live ? C : 0, v[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[i][j];
+    }
+    const float mean = row_sum<LPR>(s, sh) / (float)C;          // (divided, not times 1 / C: a constant row's mean is exact)
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[i][j] -= mean;
+        if (ck.chan(i, j) < C) q = fmaf(v[i][j], v[i][j], q);
+      }
+    const float rstd = 1.f / sqrtf(row_sum<LPR>(q, sh) / (float)C + eps);
+    if (live) {
+      if (ck.l == 0) {
+        if (mean_o != nullptr) mean_o[row] = mean;
+        if (rstd_o != nullptr) rstd_o[row] = rstd;
+      }
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        float g[8], b[8];
+        ck.loadf(gamma, 1.f, i, C, g);
+        ck.loadf(beta, 0.f, i, C, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = fmaf(v[i][j] * rstd, g[j], b[j]);
+        ck.store(y + row * y_ld, i, C, g);
+      }
+    }
+  }
+}
+
+// rows longer than LN_REG_MAX: one block per row, three walks over it (the second and third from the L2)
+template <typename T>
+__global__ __launch_bounds__(TPB) void ln_fwd_long_kernel(const T* x, int64_t x_ld, T* y, int64_t y_ld, int64_t rows, int C, const float* gamma,
+                                                          const float* beta, float eps, float* mean_o, float* rstd_o) {
+  __shared__ float sh[8];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * x_ld;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < C; c += TPB) s += (float)xr[c];
+    const float mean = row_sum<256>(s, sh) / (float)C;
+    float q = 0.f;
+    for (int c = threadIdx.x; c < C; c += TPB) {
+      const float d = (float)xr[c] - mean;
+      q = fmaf(d, d, q);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<256>(q, sh) / (float)C + eps);
+    if (threadIdx.x == 0) {
+      if (mean_o != nullptr) mean_o[row] = mean;
+      if (rstd_o != nullptr) rstd_o[row] = rstd;
+    }
+    T* yr = y + row * y_ld;
+    for (int c = threadIdx.x; c < C; c += TPB)
+      yr[c] = (T)fmaf(((float)xr[c] - mean) * rstd, gamma != nullptr ? gamma[c] : 1.f, beta != nullptr ? beta[c] : 0.f);
+  }
+}
+
+// A block walks rows blockIdx.x * RPB + gridDim.x * RPB * k and keeps its share of dgamma / dbeta in registers: one partial row pair
+// per block at the end, part[block][2][C], added up in order by a second launch.
+template <typename T, bool VEC, int LPR, int NCH>
+__global__ __launch_bounds__(TPB) void ln_bwd_kernel(const T* dy, int64_t dy_ld, const T* x, int64_t x_ld, T* dx, int64_t dx_ld, int64_t rows, int C,
+                                                     const float* mean_i, const float* rstd_i, const float* gamma, float* part) {
+  constexpr int RPB = TPB / LPR;
+  __shared__ float sh[8];
+  __shared__ float comb[LPR < 256 ? (LPR <= 64 ? 4 * LPR * 16 : 1) : 1];
+  const Chunk<T, VEC, LPR> ck{(int)(threadIdx.x % LPR)};
+  const float inv = 1.f / (float)C;
+  float g[NCH][8], dg[NCH][8], db[NCH][8];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    ck.loadf(gamma, 1.f, i, C, g[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dg[i][j] = db[i][j] = 0.f;
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + threadIdx.x / LPR;
+    const bool live = row < rows;
+    const float mean = live ? mean_i[row] : 0.f, rstd = live ? rstd_i[row] : 0.f;
+    float xh[NCH][8], d[NCH][8];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      ck.load(x + row * x_ld, i, live ? C : 0, xh[i]);
+      ck.load(dy + row * dy_ld, i, live ? C : 0, d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xh[i][j] = (xh[i][j] - mean) * rstd;
+        dg[i][j] = fmaf(d[i][j], xh[i][j], dg[i][j]);        // (a channel that is not there has d = 0)
+        db[i][j] += d[i][j];
+        d[i][j] *= g[i][j];
+        s1 += d[i][j];
+        s2 = fmaf(d[i][j], xh[i][j], s2);
+      }
+    if (dx != nullptr) {                                     // (kernel-uniform)
+      row_sum2<LPR>(s1, s2, sh);
+      s1 *= inv;
+      s2 *= inv;
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[i][j] = rstd * (d[i][j] - s1 - xh[i][j] * s2);
+          ck.store(dx + row * dx_ld, i, C, d[i]);
+        }
+      }
+    }
+  }
+  if (part == nullptr) return;
+  // rows of one wave, then the four waves (LPR = 256: a channel has one owner)
+  float* out = part + (int64_t)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    if constexpr (LPR <= 64) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int o = LPR; o < 64; o <<= 1) {
+          dg[i][j] += __shfl_xor(dg[i][j], o);
+          db[i][j] += __shfl_xor(db[i][j], o);
+        }
+      __syncthreads();
+      if ((threadIdx.x & 63) < LPR) {
+        float* c = comb + ((threadIdx.x >> 6) * LPR + ck.l) * 16;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { c[j] = dg[i][j]; c[8 + j] = db[i][j]; }
+      }
+      __syncthreads();
+      if (threadIdx.x < LPR) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          dg[i][j] = db[i][j] = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            dg[i][j] += comb[(w * LPR + ck.l) * 16 + j];
+            db[i][j] += comb[(w * LPR + ck.l) * 16 + 8 + j];
+          }
+        }
+      }
+    }
+    if (LPR == 256 || threadIdx.x < LPR) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (ck.chan(i, j) < C) {
+          out[ck.chan(i, j)] = dg[i][j];
+          out[C + ck.chan(i, j)] = db[i][j];
+        }
+    }
+  }
+}
+
+// rows longer than LN_REG_MAX: dx by one block per row; dgamma / dbeta by columns, a block takes 256 channels x a range of rows
+template <typename T>
+__global__ __launch_bounds__(TPB) void ln_bwd_long_dx_kernel(const T* dy, int64_t dy_ld, const T* x, int64_t x_ld, T* dx, int64_t dx_ld, int64_t rows,
+                                                             int C, const float* mean_i, const float* rstd_i, const float* gamma) {
+  __shared__ float sh[8];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float mean = mean_i[row], rstd = rstd_i[row], inv = 1.f / (float)C;
+    const T *xr = x + row * x_ld, *dr = dy + row * dy_ld;
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < C; c += TPB) {
+      const float g = (float)dr[c] * (gamma != nullptr ? gamma[c] : 1.f);
+      s1 += g;
+      s2 = fmaf(g, ((float)xr[c] - mean) * rstd, s2);
+    }
+    row_sum2<256>(s1, s2, sh);
+    s1 *= inv;
+    s2 *= inv;
+    T* o = dx + row * dx_ld;
+    for (int c = threadIdx.x; c < C; c += TPB) {
+      const float g = (float)dr[c] * (gamma != nullptr ? gamma[c] : 1.f);
+      o[c] = (T)(rstd * (g - s1 - ((float)xr[c] - mean) * rstd * s2));
+    }
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(TPB) void ln_bwd_long_param_kernel(const T* dy, int64_t dy_ld, const T* x, int64_t x_ld, int64_t rows, int C,
+                                                                const float* mean_i, const float* rstd_i, float* part) {
+  const int c = blockIdx.x * TPB + threadIdx.x;
+  if (c >= C) return;
+  float dg = 0.f, db = 0.f;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const float d = (float)dy[r * dy_ld + c];
+    db += d;
+    dg = fmaf(d, ((float)x[r * x_ld + c] - mean_i[r]) * rstd_i[r], dg);
+  }
+  part[((int64_t)blockIdx.y * 2) * C + c] = dg;
+  part[((int64_t)blockIdx.y * 2 + 1) * C + c] = db;
+}
+
+// lanes per row and chunks per lane for C channels: the fewest lanes that keep a row's chunks at four or fewer, a wave first
+struct LnShape { int lpr, nch; };
+inline LnShape ln_shape(int C) {
+  const int chunks = (C + 7) / 8;
+  for (int lpr : {8, 16, 32, 64})
+    if (chunks <= lpr) return {lpr, 1};
+  if (chunks <= 128) return {64, 2};
+  if (chunks <= 256) return {64, 4};
+  if (chunks <= 512) return {256, 2};
+  if (chunks <= 1024) return {256, 4};
+  return {256, 8};
+}
+template <typename F>
+inline void ln_dispatch(const LnShape& s, F&& f) {
+  using std::integral_constant;
+#define LN_CASE(L, N) \
+  if (s.lpr == L && s.nch == N) return f(integral_constant<int, L>{}, integral_constant<int, N>{});
+  LN_CASE(8, 1) LN_CASE(16, 1) LN_CASE(32, 1) LN_CASE(64, 1) LN_CASE(64, 2) LN_CASE(64, 4) LN_CASE(256, 2) LN_CASE(256, 4) LN_CASE(256, 8)
+#undef LN_CASE
+}
+// the kernels walk rows with the grid as stride: more blocks than this gain nothing
+inline unsigned ln_grid(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20); }
+inline int64_t ln_bwd_blocks(int64_t rows, int C) {
+  if (C > LN_REG_MAX) return rows < 64 ? rows : 64;
+  const int64_t rpb = TPB / ln_shape(C).lpr, groups = (rows + rpb - 1) / rpb;
+  // at least four row groups per block: the partial rows are then at most a tenth of the traffic
+  const int64_t most = 1024, want = (groups + 3) / 4;
+  return want < most ? want : most;
+}
+
+bool ln_vec(std::initializer_list<const void*> ps, std::initializer_list<int64_t> lds, int C, int dt) {
+  if (C % 8 != 0) return false;
+  for (const void* p : ps)
+    if (p != nullptr && !aligned16(p)) return false;
+  for (int64_t l : lds)
+    if (l % (dt == SEG_DT_F32 ? 4 : 8) != 0) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" int seg_layernorm_fwd(const void* x, int64_t x_ld, void* y, int64_t y_ld, int64_t rows, int32_t C, int32_t dtype, const float* gamma,
+                                 const float* beta, float eps, float* mean, float* rstd, seg_stream_t stream) {
+  SEG_CHECK_ARG(dtype >= SEG_DT_F16 && dtype <= SEG_DT_F32, "layernorm_fwd: dtype %d", dtype);
+  SEG_CHECK_ARG(rows >= 0 && C > 0, "layernorm_fwd: rows %lld, C %d", (long long)rows, C);
+  SEG_CHECK_ARG(rows <= 1 || (x_ld >= C && y_ld >= C), "layernorm_fwd: row strides below the %d channels", C);
+  if (rows == 0) return SEG_OK;
+  SEG_CHECK_ARG(x != nullptr && y != nullptr, "layernorm_fwd: x / y is NULL");
+  hipStream_t st = (hipStream_t)stream;
+  seq_dispatch_dtype(dtype, [&](auto* tp) {
+    typedef typename std::remove_pointer<decltype(tp)>::type T;
+    if (C > LN_REG_MAX) {
+      hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3(ln_grid(rows)), dim3(TPB), 0, st, (const T*)x, x_ld, (T*)y, y_ld, rows, C, gamma, beta, eps, mean, rstd);
+      return;
+    }
+    const LnShape s = ln_shape(C);
+    const unsigned grid = ln_grid((rows + TPB / s.lpr - 1) / (TPB / s.lpr));
+    ln_dispatch(s, [&](auto L, auto N) {
+      if (ln_vec({x, y, gamma, beta}, {x_ld, y_ld}, C, dtype))
+        hipLaunchKernelGGL((ln_fwd_kernel<T, true, L(), N()>), dim3(grid), dim3(TPB), 0, st, (const T*)x, x_ld, (T*)y, y_ld, rows, C, gamma, beta, eps, mean, rstd);
+      else
+        hipLaunchKernelGGL((ln_fwd_kernel<T, false, L(), N()>), dim3(grid), dim3(TPB), 0, st, (const T*)x, x_ld, (T*)y, y_ld, rows, C, gamma, beta, eps, mean, rstd);
+    });
+  });
+  SEG_CHECK_LAUNCH("layernorm_fwd");
+  return SEG_OK;
+}
+
+extern "C" int64_t seg_layernorm_bwd_workspace_bytes(int64_t rows, int32_t C, int32_t dtype) {
+  (void)dtype;
+  if (rows <= 0 || C <= 0) return 0;
+  return ln_bwd_blocks(rows, C) * 2 * C * 4 + 2 * (int64_t)C * 4;
+}
+
+extern "C" int seg_layernorm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, void* dx, int64_t dx_ld, int64_t rows, int32_t C,
+                                 int32_t dtype, const float* mean, const float* rstd, const float* gamma, float* dgamma, float* dbeta,
+                                 void* workspace, seg_stream_t stream) {
+  SEG_CHECK_ARG(dtype >= SEG_DT_F16 && dtype <= SEG_DT_F32, "layernorm_bwd: dtype %d", dtype);
+  SEG_CHECK_ARG(rows >= 0 && C > 0, "layernorm_bwd: rows %lld, C %d", (long long)rows, C);
+  SEG_CHECK_ARG(rows <= 1 || (x_ld >= C && dy_ld >= C && (dx == nullptr || dx_ld >= C)), "layernorm_bwd: row strides below the %d channels", C);
+  const bool params = dgamma != nullptr || dbeta != nullptr;
+  SEG_CHECK_ARG(rows == 0 || (dy != nullptr && x != nullptr && mean != nullptr && rstd != nullptr), "layernorm_bwd: dy / x / mean / rstd is NULL");
+  SEG_CHECK_ARG(rows == 0 || !params || workspace != nullptr, "layernorm_bwd: dgamma / dbeta need the workspace");
+  hipStream_t st = (hipStream_t)stream;
+  float* part = params ? (float*)workspace : nullptr;
+  const int64_t nblk = rows > 0 ? ln_bwd_blocks(rows, C) : 0;
+  if (rows > 0 && (params || dx != nullptr))
+    seq_dispatch_dtype(dtype, [&](auto* tp) {
+      typedef typename std::remove_pointer<decltype(tp)>::type T;
+      if (C > LN_REG_MAX) {
+        if (params)                               // (in front of dx, which may be dy or x)
+          hipLaunchKernelGGL((ln_bwd_long_param_kernel<T>), dim3((C + TPB - 1) / TPB, (unsigned)nblk), dim3(TPB), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, rows, C, mean, rstd, part);
+        if (dx != nullptr)
+          hipLaunchKernelGGL((ln_bwd_long_dx_kernel<T>), dim3(ln_grid(rows)), dim3(TPB), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (T*)dx, dx_ld, rows, C, mean, rstd, gamma);
+        return;
+      }
+      ln_dispatch(ln_shape(C), [&](auto L, auto N) {
+        if (ln_vec({x, dy, dx, gamma}, {x_ld, dy_ld, dx == nullptr ? 0 : dx_ld}, C, dtype))
+          hipLaunchKernelGGL((ln_bwd_kernel<T, true, L(), N()>), dim3((unsigned)nblk), dim3(TPB), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (T*)dx, dx_ld, rows, C, mean, rstd, gamma, part);
+        else
+          hipLaunchKernelGGL((ln_bwd_kernel<T, false, L(), N()>), dim3((unsigned)nblk), dim3(TPB), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (T*)dx, dx_ld, rows, C, mean, rstd, gamma, part);
+      });
+    });
+  if (dgamma != nullptr && dbeta == dgamma + C) {            // one buffer for both: one launch
+    launch_colsum_parts(part, nblk, 2 * (int64_t)C, 2 * (int64_t)C, dgamma, st);
+    dgamma = dbeta = nullptr;
+  }
+  if (dgamma != nullptr) launch_colsum_parts(part, nblk, 2 * (int64_t)C, C, dgamma, st);
+  if (dbeta != nullptr) launch_colsum_parts(part == nullptr ? nullptr : part + C, nblk, 2 * (int64_t)C, C, dbeta, st);
+  SEG_CHECK_LAUNCH("layernorm_bwd");
+  return SEG_OK;
+}
