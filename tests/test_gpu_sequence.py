@@ -210,6 +210,29 @@ def test_linear_slices(dtype):
         R.assert_close(db, dy.double().sum(0), dy.double().abs().sum(0), M + 4, "db")
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+def test_linear_large_tiles(dtype):
+    """Results that fill the card with the largest tiles, ragged against them in every direction (reference: 64-bit products on the device)."""
+    g = gen(14)
+    M, N, K = 12360, 1032, 136
+    x, w, b, r, z, dy = (rnd(g, *s, dtype=t).cuda() for s, t in (((M, K), dtype), ((N, K), dtype), ((N,), torch.float32), ((M, N), dtype), ((M, N), dtype), ((M, N), dtype)))
+    y, pre = seq.linear(x, w, b, activation="gelu", residual=r, preactivation=True)
+    z64, s = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t() + b.double().abs()
+    R.assert_close(pre, z64.cpu(), s.cpu(), K + 4, "z")
+    R.assert_close(y, (R.act(z64, "gelu") + r.double()).cpu(), (1.13 * s + r.double().abs() + z64.abs() + 1).cpu(), K + 24, "y")
+    # as the second layer of a perceptron: inputs N, units K
+    wb = rnd(g, K, N, dtype=dtype).cuda()
+    dx, none, _db = seq.linear_backward(x, y, wb, z=z, activation="gelu", residual=r, need_dw=False)
+    p, s = x.double() @ wb.double(), x.double().abs() @ wb.double().abs()
+    R.assert_close(dx, (p * R.act_slope(z.double(), "gelu") + r.double()).cpu(), (1.13 * s + p.abs() * (1 + z.double().abs()) + r.double().abs()).cpu(), K + 24, "dx")
+    M, N, K = 131080, 520, 264
+    x, dy = rnd(g, M, K, dtype=dtype).cuda(), rnd(g, M, N, dtype=dtype).cuda()
+    _dx, dw, db = seq.linear_backward(dy, x, torch.zeros(N, K, dtype=dtype, device="cuda"), need_dx=False)
+    R.assert_close(dw, (dy.double().t() @ x.double()).cpu(), (dy.double().abs().t() @ x.double().abs()).cpu(), M, "dw")
+    R.assert_close(db, dy.double().sum(0).cpu(), dy.double().abs().sum(0).cpu(), M, "db")
+    assert torch.equal(dw, seq.linear_backward(dy, x, torch.zeros(N, K, dtype=dtype, device="cuda"), need_dx=False, need_db=False)[1])
+
+
 def test_linear_no_rows_and_leading_axes():
     w = torch.randn(6, 10, generator=gen(1)).cuda()
     y = seq.linear(torch.empty(0, 10, device="cuda"), w)

@@ -27,6 +27,7 @@ struct GemmArgs {
   const void* res; int64_t res_ld;
   void* z; int64_t z_ld;
   void* out; int64_t out_ld;
+  int vecio;                     // rows of z, residual and out take 16-byte accesses
 };
 
 // one element of the result through the pass's epilogue
@@ -144,6 +145,217 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   }
 }
 
+// ---- the tile kernel for 16-bit operands whose rows take 16-byte accesses: BM x BN tiles, 64 of k per step, both operands by LDS-DMA in
+// the layout they have in memory - k-contiguous rows of 128 bytes, or rows of one k with BM / BN columns, which the transposing LDS
+// reads turn into the same fragments - two stages in a ring: a step's loads are in flight while the step before is contracted.
+//
+// LDS swizzle (the DMA writes lane i's 16 bytes at 16 i, so the lane chooses the memory chunk instead): k-contiguous rows keep chunk
+// c of row r at c ^ ((r >> 1) & 7), so that the 16 rows a ds_read_b128 group touches lie on 16 different 16-byte slots; rows of one k
+// keep it at c ^ ((k & 3) << 2), so that the four k rows of a transposing read lie in four different 64-byte quarters.
+typedef short s4v __attribute__((__vector_size__(4 * sizeof(short))));
+typedef __attribute__((address_space(3))) s4v* lds_s4v_ptr;
+typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
+
+constexpr int BK = 64;
+
+// one operand's side of the ring: ROWS tile rows (along i or j), loaded by NWV waves
+template <bool KC, int ROWS, int NWV> struct TileLoader {
+  static constexpr int NI = ROWS / 8 / NWV;                    // DMA instructions (1 KiB) per wave and step
+  unsigned voff[NI];
+  int kchunk[2];                                               // KC: the k chunk a lane fetches in even / odd instructions
+  i4v rsrc;
+  const unsigned char* base;
+  int64_t ld2;
+  int cols2;
+  __device__ __forceinline__ void init(const void* ptr, int64_t ld, int64_t r0, int64_t rend, int64_t Kd, int wave, int lane) {
+    ld2 = ld * 2;
+    const int64_t left = rend - r0;
+    const int rows = left < ROWS ? (int)left : ROWS;
+    if constexpr (KC) {
+      base = (const unsigned char*)ptr + r0 * ld2;
+      rsrc = make_rsrc(base, (int)((rows - 1) * ld2 + Kd * 2));          // rows behind the operand's end start behind this
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int row = (wave * NI + i) * 8 + (lane >> 3);
+        const int ch = (lane & 7) ^ ((row >> 1) & 7);
+        kchunk[i & 1] = ch;
+        voff[i] = (unsigned)(row * ld2 + ch * 16);
+      }
+    } else {
+      base = (const unsigned char*)ptr + r0 * 2;
+      cols2 = (int)left * 2;
+      constexpr int RPI = 512 / ROWS, LPR = 64 / RPI;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int k = (wave * NI + i) * RPI + lane / LPR;
+        const int ch = (lane % LPR) ^ ((k & 3) << 2);
+        voff[i] = (unsigned)(k * ld2 + ch * 16);
+      }
+    }
+  }
+  // rows k0 .. k0 + 64 (to kend) into the LDS at dst; what is not there reads as zero (the buffer's bounds, or a masked offset)
+  __device__ __forceinline__ void issue(unsigned dst, int64_t k0, int64_t kend, int wave) {
+    if constexpr (KC) {
+      const bool tail = kend - k0 < BK;
+      const int rem = (int)(kend - k0);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        unsigned v = voff[i];
+        if (tail && kchunk[i & 1] * 8 >= rem) v = 0x80000000u;
+        lds_dma16(rsrc, dst + (wave * NI + i) * 1024, v, (int)(k0 * 2));
+      }
+    } else {
+      const int64_t left = kend - k0;
+      const int rows = left < BK ? (int)left : BK;
+      const i4v r = make_rsrc(base + k0 * ld2, (int)((rows - 1) * ld2 + cols2));
+#pragma unroll
+      for (int i = 0; i < NI; ++i) lds_dma16(r, dst + (wave * NI + i) * 1024, voff[i], 0);
+    }
+  }
+};
+// fragment t of a wave's tile (32 rows from row0 = first row + 32 t), k step ks
+template <bool KC, int ROWS> __device__ __forceinline__ u4 tile_frag(const unsigned char* s, int row0, int ks, int lane) {
+  if constexpr (KC) {
+    const int fr = lane & 31, fh = lane >> 5;
+    return *reinterpret_cast<const u4*>(s + (row0 + fr) * 128 + (((ks * 2 + fh) ^ ((fr >> 1) & 7)) << 4));
+  } else {
+    const int tg = lane >> 4, tt = lane & 15, tq = tt >> 2, tp = tt & 3;
+    const int ch = (row0 >> 3) + 2 * (tg & 1) + (tp >> 1);
+    const unsigned char* a = s + (ks * 16 + 8 * (tg >> 1) + tq) * (ROWS * 2) + ((ch ^ (tq << 2)) << 4) + (tp & 1) * 8;
+    const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_ptr)a);
+    const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_ptr)(a + 4 * ROWS * 2));
+    const u2 l = __builtin_bit_cast(u2, lo), h = __builtin_bit_cast(u2, hi);
+    return u4{l[0], l[1], h[0], h[1]};
+  }
+}
+template <typename T> __device__ __forceinline__ f16v mfma16(u4 a, u4 b, f16v c) {
+  if constexpr (std::is_same<T, half_t>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// eight neighbouring elements of the result through the pass's epilogue; vec: every row of z, residual and out takes 16-byte accesses
+template <int PASS, typename T> __device__ __forceinline__ void epilogue8(const GemmArgs& p, int64_t i, int j, const float* bias, float* v, bool vec) {
+  if constexpr (PASS == SEG_LINEAR_BWD_WEIGHT) {
+    float* o = (float*)p.out + i * p.out_ld + j;
+    if (vec) store8<float>(o, v);
+    else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) o[t] = v[t];
+    }
+  } else {
+    float f[8];
+    if constexpr (PASS == SEG_LINEAR_FWD) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] += bias[t];
+      if (p.z != nullptr) {
+        if (vec) row_store8<T, true>((T*)p.z + i * p.z_ld + j, 8, v);
+        else row_store8<T, false>((T*)p.z + i * p.z_ld + j, 8, v);
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = seq_act(v[t], p.act, p.alpha);
+    } else if (p.z != nullptr) {
+      if (vec) row_load8<T, true>((const T*)p.z + i * p.z_ld + j, 8, f);
+      else row_load8<T, false>((const T*)p.z + i * p.z_ld + j, 8, f);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] *= seq_act_slope(f[t], p.act, p.alpha);
+    }
+    if (p.res != nullptr) {
+      if (vec) row_load8<T, true>((const T*)p.res + i * p.res_ld + j, 8, f);
+      else row_load8<T, false>((const T*)p.res + i * p.res_ld + j, 8, f);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] += f[t];
+    }
+    if (vec) row_store8<T, true>((T*)p.out + i * p.out_ld + j, 8, v);
+    else row_store8<T, false>((T*)p.out + i * p.out_ld + j, 8, v);
+  }
+}
+
+template <int PASS, typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(const GemmArgs p) {
+  constexpr bool AKC = PASS != SEG_LINEAR_BWD_WEIGHT, BKC = PASS == SEG_LINEAR_FWD;
+  constexpr int NWV = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 128, SLAB = 32 * 68 * 4;
+  static_assert(TN % 2 == 0 && NWV * SLAB <= 2 * STAGE, "the epilogue's slabs take 64 columns and fit the ring");
+  __shared__ __align__(1024) unsigned char smem[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // tiles in groups of eight rows of tiles, column by column: the blocks of one XCD share operand panels in both directions
+  const int t = xcd_remap(blockIdx.x, p.ti * p.tj);
+  const int grp = t / (8 * p.tj), in = t - grp * 8 * p.tj, gh = p.ti - grp * 8 < 8 ? p.ti - grp * 8 : 8;
+  const int64_t i0 = (int64_t)(grp * 8 + in % gh) * BM;
+  const int j0 = in / gh * BN;
+  const int64_t kbeg = blockIdx.y * p.kper, kend = kbeg + p.kper < p.Kd ? kbeg + p.kper : p.Kd;
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_byte_ptr)smem);
+  TileLoader<AKC, BM, NWV> la;
+  TileLoader<BKC, BN, NWV> lb;
+  la.init(p.A, p.a_ld, i0, p.I, p.Kd, wave, lane);
+  lb.init(p.B, p.b_ld, j0, p.J, p.Kd, wave, lane);
+  f16v acc[TM][TN];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
+  const int wr = (wave / WN) * TM * 32, wc = (wave % WN) * TN * 32;
+  int stage = 0;
+  la.issue(lds0, kbeg, kend, wave);
+  lb.issue(lds0 + BM * 128, kbeg, kend, wave);
+  for (int64_t k = kbeg; k < kend; k += BK, stage ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    ring_release_barrier();                                    // this step has landed for every wave, the other stage has no readers left
+    if (k + BK < kend) {
+      const unsigned d = lds0 + (stage ^ 1) * STAGE;
+      la.issue(d, k + BK, kend, wave);
+      lb.issue(d + BM * 128, k + BK, kend, wave);
+    }
+    const unsigned char *sa = smem + stage * STAGE, *sb = sa + BM * 128;
+#pragma unroll
+    for (int ks = 0; ks < BK / 16; ++ks) {
+      u4 af[TM], bf[TN];
+#pragma unroll
+      for (int a = 0; a < TM; ++a) af[a] = tile_frag<AKC, BM>(sa, wr + a * 32, ks, lane);
+#pragma unroll
+      for (int b = 0; b < TN; ++b) bf[b] = tile_frag<BKC, BN>(sb, wc + b * 32, ks, lane);
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) acc[a][b] = mfma16<T>(af[a], bf[b], acc[a][b]);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  ring_release_barrier();                                      // the ring becomes the epilogue's slabs: 32 rows x 64 columns per wave
+  float* slab = reinterpret_cast<float*>(smem + wave * SLAB);
+  const int fr = lane & 31, fh = lane >> 5;
+#pragma unroll
+  for (int bp = 0; bp < TN / 2; ++bp) {
+    const int j = j0 + wc + bp * 64 + (lane & 7) * 8;
+    float bias[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) bias[q] = (PASS == SEG_LINEAR_FWD && p.bias != nullptr && j < p.J) ? p.bias[j + q] : 0.f;
+#pragma unroll
+    for (int a = 0; a < TM; ++a) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) slab[((q & 3) + 8 * (q >> 2) + 4 * fh) * 68 + h * 32 + fr] = acc[a][2 * bp + h][q];
+      __builtin_amdgcn_wave_barrier();
+      const int64_t ib = i0 + wr + a * 32 + (lane >> 3);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t i = ib + r * 8;
+        float v[8];
+        load8<float>(slab + ((lane >> 3) + r * 8) * 68 + (lane & 7) * 8, v);
+        if (i < p.I && j < p.J) {
+          if (p.splits > 1) store8<float>(p.part + ((int64_t)blockIdx.y * p.I + i) * p.J + j, v);
+          else epilogue8<PASS, T>(p, i, j, bias, v, p.vecio != 0);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
 // the split ranges of k added in order, then the epilogue
 template <int PASS, typename T>
 __global__ __launch_bounds__(TPB) void gemm_join_kernel(const GemmArgs p) {
@@ -192,19 +404,22 @@ inline ColsumPlan colsum_plan(int64_t rows, int cols) {
 }
 
 // ---- plans
-struct GemmPlan { int tile; int ti, tj, splits; int64_t kper; };
-inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype) {
+enum { TILE_ANY = 0, TILE_128 = 1, TILE_256 = 2 };
+struct GemmPlan { int kind; int ti, tj, splits; int64_t kper; };
+inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   GemmPlan g;
-  g.tile = 64;
-  g.ti = (int)((I + 63) / 64);
-  g.tj = (J + 63) / 64;
-  const int64_t tiles = (int64_t)g.ti * g.tj;
+  const int64_t t256 = ((I + 255) / 256) * ((J + 255) / 256);
+  g.kind = !dma ? TILE_ANY : t256 * ((Kd + 4095) / 4096) >= 192 ? TILE_256 : TILE_128;
+  const int side = g.kind == TILE_ANY ? 64 : g.kind == TILE_128 ? 128 : 256;
+  g.ti = (int)((I + side - 1) / side);
+  g.tj = (J + side - 1) / side;
+  const int64_t tiles = (int64_t)g.ti * g.tj, room = g.kind == TILE_256 ? 256 : g.kind == TILE_128 ? 512 : 1024;
   // fewer tiles than the card has room for: k is split, down to 256 of it per block
-  int64_t s = tiles >= 512 || tiles == 0 ? 1 : 1024 / tiles;
+  int64_t s = tiles * 2 > room || tiles == 0 ? 1 : room / tiles;
   if (s > Kd / 256) s = Kd / 256;
   if (s > 32) s = 32;
   if (s < 1) s = 1;
-  const int64_t step = dtype == SEG_DT_F32 ? 16 : 32;
+  const int64_t step = g.kind != TILE_ANY ? 64 : dtype == SEG_DT_F32 ? 16 : 32;
   g.kper = ((Kd + s - 1) / s + step - 1) / step * step;
   g.splits = g.kper > 0 ? (int)((Kd + g.kper - 1) / g.kper) : 1;
   if (g.splits < 1) g.splits = 1;
@@ -226,19 +441,42 @@ inline int vec_of(const void* A, int64_t a_ld, const void* B, int64_t b_ld, int 
   return 1;
 }
 
+// whether the operands of a pass suit the LDS-DMA tile kernels: 16-bit, 16-byte rows, offsets inside a tile below 2 GiB
+inline bool dma_ok(const seg_linear_args& a, int pass) {
+  if (a.dtype == SEG_DT_F32) return false;
+  const Extents e = extents(a, pass);
+  const void *A = pass == SEG_LINEAR_BWD_WEIGHT ? a.dy : a.x, *B = pass == SEG_LINEAR_BWD_WEIGHT ? a.x : a.w;
+  const int64_t al = pass == SEG_LINEAR_BWD_WEIGHT ? a.dy_ld : a.x_ld, bl = pass == SEG_LINEAR_BWD_WEIGHT ? a.x_ld : a.w_ld;
+  if (!aligned16(A) || !aligned16(B) || al % 8 != 0 || bl % 8 != 0 || al > (1 << 21) || bl > (1 << 21) || al <= 0 || bl <= 0) return false;
+  if (e.J % 8 != 0 || (pass == SEG_LINEAR_BWD_WEIGHT ? e.I % 8 != 0 : e.Kd % 8 != 0) || (pass != SEG_LINEAR_BWD_WEIGHT && e.Kd >= (1 << 21))) return false;
+  // tiles far larger than the result waste the matrix cores
+  return e.I >= 64 && e.J >= 64;
+}
+inline GemmPlan plan_of(const seg_linear_args& a, int pass) {
+  const Extents e = extents(a, pass);
+  return gemm_plan(e.I, e.J, e.Kd, a.dtype, dma_ok(a, pass));
+}
+
 template <int PASS>
 int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
   const Extents e = extents(a, PASS);
-  const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a.dtype);
+  const GemmPlan g = plan_of(a, PASS);
   p.I = e.I; p.J = e.J; p.Kd = e.Kd;
   p.ti = g.ti; p.tj = g.tj; p.splits = g.splits; p.kper = g.kper;
   p.part = (float*)a.workspace;
   p.act = a.act; p.alpha = a.alpha;
+  p.vecio = PASS == SEG_LINEAR_BWD_WEIGHT ? vec_ok(p.out, p.out_ld, 0, SEG_DT_F32)
+                                          : vec_ok(p.out, p.out_ld, 0, a.dtype) && vec_ok(p.z, p.z_ld, 0, a.dtype) && vec_ok(p.res, p.res_ld, 0, a.dtype);
   const dim3 grid((unsigned)(g.ti * g.tj), (unsigned)g.splits);
   const int vec = vec_of(p.A, p.a_ld, p.B, p.b_ld, a.dtype);
   seq_dispatch_dtype(a.dtype, [&](auto* tp) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
-    if (vec == 4) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 4>), grid, dim3(TPB), 0, st, p);
+    if (g.kind != TILE_ANY) {
+      if constexpr (!std::is_same<T, float>::value) {
+        if (g.kind == TILE_256) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 256, 256, 2, 4>), grid, dim3(512), 0, st, p);
+        else hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 128, 2, 2>), grid, dim3(256), 0, st, p);
+      }
+    } else if (vec == 4) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 4>), grid, dim3(TPB), 0, st, p);
     else if (vec == 8) {
       if constexpr (!std::is_same<T, float>::value) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 8>), grid, dim3(TPB), 0, st, p);
     } else hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 1>), grid, dim3(TPB), 0, st, p);
@@ -258,7 +496,8 @@ int check_linear(const seg_linear_args* a, int pass, const char* name) {
                 "%s: activation %d", name, a->act);
   const Extents e = extents(*a, pass);
   SEG_CHECK_ARG(((e.I + 63) / 64) * ((int64_t)(e.J + 63) / 64) < (int64_t)1 << 24, "%s: result of %lld x %d is too large for one call", name, (long long)e.I, e.J);
-  const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a->dtype);
+  const GemmPlan g = plan_of(*a, pass);
+  SEG_CHECK_ARG(aligned16(a->workspace), "%s: workspace needs 16-byte alignment", name);
   SEG_CHECK_ARG(a->M == 0 || g.splits <= 1 || a->workspace != nullptr, "%s: workspace is NULL (%lld bytes are needed)", name, (long long)seg_linear_workspace_bytes(a, pass));
   return SEG_OK;
 }
@@ -268,7 +507,7 @@ int check_linear(const seg_linear_args* a, int pass, const char* name) {
 extern "C" int64_t seg_linear_workspace_bytes(const seg_linear_args* a, int32_t pass) {
   if (a == nullptr || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
   const Extents e = extents(*a, pass);
-  const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a->dtype);
+  const GemmPlan g = plan_of(*a, pass);
   int64_t b = g.splits > 1 ? (int64_t)g.splits * e.I * e.J * 4 : 0;
   if (pass == SEG_LINEAR_BWD_WEIGHT) {
     const int64_t c = colsum_plan(a->M, a->N).parts * a->N * 4;
@@ -322,7 +561,7 @@ extern "C" int seg_linear_bwd_weight(const seg_linear_args* a, seg_stream_t stre
   }
   if (a->db != nullptr) {
     const Extents e = extents(*a, SEG_LINEAR_BWD_WEIGHT);
-    const GemmPlan g = gemm_plan(e.I, e.J, e.Kd, a->dtype);
+    const GemmPlan g = plan_of(*a, SEG_LINEAR_BWD_WEIGHT);
     const int64_t off = g.splits > 1 ? ((int64_t)g.splits * e.I * e.J * 4 + 15) / 16 * 16 : 0;
     float* part = (float*)((char*)a->workspace + off);
     const ColsumPlan c = a->M > 0 ? colsum_plan(a->M, a->N) : ColsumPlan{0, 0};
