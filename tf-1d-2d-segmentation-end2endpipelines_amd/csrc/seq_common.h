@@ -62,10 +62,10 @@ template <typename T, bool VEC> __device__ __forceinline__ void row_store8(T* p,
 }
 
 __device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
-// Phi(v) = erfc(-v / sqrt 2) / 2 and e = exp(-v^2 / 2).  erfc(x) exp(x^2) = t P(t) with t = 1 / (1 + 0.3 x), P of degree 8 fitted to a
+// h = Phi(-|v|) = erfc(|v| / sqrt 2) / 2 and e = exp(-v^2 / 2).  erfc(x) exp(x^2) = t P(t) with t = 1 / (1 + 0.3 x), P of degree 8 fitted to a
 // relative error of 2e-8 on 0 <= x <= 9.5 (behind it both factors are 0 in 32 bits): the left tail keeps its relative precision, which
 // 1 + erf loses, at about 20 instructions - half of the library's erff, and the derivative's Gaussian comes with it.
-__device__ __forceinline__ float phi_f(float v, float& e) {
+__device__ __forceinline__ float phi_neg(float v, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.21213203435596426f, fabsf(v), 1.f));
   e = __builtin_amdgcn_exp2f(-0.72134752044448170f * v * v);
   float P = -0.12943415125844135f;
@@ -77,8 +77,7 @@ __device__ __forceinline__ float phi_f(float v, float& e) {
   P = fmaf(P, t, 0.1484823543501283f);
   P = fmaf(P, t, 0.17069194623730768f);
   P = fmaf(P, t, 0.16918961408577482f);
-  const float h = 0.5f * t * P * e;
-  return v < 0.f ? h : 1.f - h;
+  return 0.5f * t * P * e;
 }
 
 __device__ __forceinline__ float seq_act(float v, int act, float alpha) {
@@ -87,7 +86,7 @@ __device__ __forceinline__ float seq_act(float v, int act, float alpha) {
     case SEG_ACT_LEAKY: return v > 0.f ? v : v * alpha;
     case SEG_ACT_SIGMOID: return sigmoid_f(v);
     case SEG_ACT_SILU: return v * sigmoid_f(v);
-    case SEG_ACT_GELU: { float e; return v * phi_f(v, e); }
+    case SEG_ACT_GELU: { float e; const float h = phi_neg(v, e); return fmaf(-fabsf(v), h, fmaxf(v, 0.f)); }      // v Phi(v)
     default: return v;
   }
 }
@@ -98,10 +97,32 @@ __device__ __forceinline__ float seq_act_slope(float v, int act, float alpha) {
     case SEG_ACT_LEAKY: return v > 0.f ? 1.f : alpha;
     case SEG_ACT_SIGMOID: { const float s = sigmoid_f(v); return s * (1.f - s); }
     case SEG_ACT_SILU: { const float s = sigmoid_f(v); return s * (1.f + v * (1.f - s)); }
-    case SEG_ACT_GELU: { float e; const float h = phi_f(v, e); return fmaf(v * 0.39894228040143268f, e, h); }
+    case SEG_ACT_GELU: { float e; const float h = phi_neg(v, e); return fmaf(v * 0.39894228040143268f, e, v < 0.f ? h : 1.f - h); }
     default: return 1.f;
   }
 }
+
+// eight at a time, the (launch-uniform) choice taken once
+#define SEQ_ACT8_CASES(F)                                                                        \
+  switch (act) {                                                                                 \
+    case SEG_ACT_RELU: F(SEG_ACT_RELU) break;                                                    \
+    case SEG_ACT_LEAKY: F(SEG_ACT_LEAKY) break;                                                  \
+    case SEG_ACT_SIGMOID: F(SEG_ACT_SIGMOID) break;                                              \
+    case SEG_ACT_SILU: F(SEG_ACT_SILU) break;                                                    \
+    case SEG_ACT_GELU: F(SEG_ACT_GELU) break;                                                    \
+    default: break;                                                                              \
+  }
+__device__ __forceinline__ void act8(float* v, int act, float alpha) {
+#define SEQ_F(A) { _Pragma("unroll") for (int t = 0; t < 8; ++t) v[t] = seq_act(v[t], A, alpha); }
+  SEQ_ACT8_CASES(SEQ_F)
+#undef SEQ_F
+}
+__device__ __forceinline__ void slope8(float* v, const float* z, int act, float alpha) {
+#define SEQ_F(A) { _Pragma("unroll") for (int t = 0; t < 8; ++t) v[t] *= seq_act_slope(z[t], A, alpha); }
+  SEQ_ACT8_CASES(SEQ_F)
+#undef SEQ_F
+}
+#undef SEQ_ACT8_CASES
 
 // out[c] = sum over parts of part[p][c], fixed order: 16 columns x 16 parts per 256 threads, each thread its parts in turn
 constexpr int CR_COLS = 16;
