@@ -151,7 +151,7 @@ def test_linear_arguments(lib):
         refused(lib, lib.seg_linear_fwd(linear_args(**k), None), text)
     refused(lib, lib.seg_linear_bwd_data(linear_args(bias=FAKE), None), "bias")
     refused(lib, lib.seg_linear_bwd_data(linear_args(w_ld=31), None), "strides")
-    long = linear_args(M=64, N=8, K=1 << 16, x_ld=1 << 16, w_ld=1 << 16)
+    long = linear_args(M=128, N=8, K=1 << 16, x_ld=1 << 16, w_ld=1 << 16)
     assert lib.seg_linear_workspace_bytes(long, ffi.LINEAR_FWD) > 0
     refused(lib, lib.seg_linear_fwd(long, None), "workspace")
     refused(lib, lib.seg_linear_bwd_weight(linear_args(dy=None), None), "NULL")

@@ -422,6 +422,64 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
   }
 }
 
+// ---- a few rows against all the weights (forward, up to 64 rows): the weights' bytes and one memory latency bound it, so they go straight
+// into the matrix instructions' registers, once, with no LDS in between.  A block owns 16 units; its waves share k in steps of 64 bytes per
+// row (lane l: row l % 16, 16 bytes at chunk l / 16), keep four steps' loads in flight and add their sums in the LDS.  MT x 16 rows of x.
+template <typename T, int MT, int WK>
+__global__ __launch_bounds__(64 * WK) void gemm_rows_kernel(const GemmArgs p) {
+  constexpr int EPC = 16 / (int)sizeof(T), STEP = 4 * EPC, UN = MT <= 2 ? 4 : 2;
+  __shared__ float red[WK][MT * 16][17];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, ch = lane >> 4, j0 = blockIdx.x * 16, M = (int)p.I;
+  const T* w = (const T*)p.B + (int64_t)(j0 + r < p.J ? j0 + r : p.J - 1) * p.b_ld + ch * EPC;     // (rows that are not there: results dropped)
+  const T* x[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) x[m] = (const T*)p.A + (int64_t)(m * 16 + r < M ? m * 16 + r : M - 1) * p.a_ld + ch * EPC;
+  f4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f4{0.f, 0.f, 0.f, 0.f};
+  const u4 zero = {0u, 0u, 0u, 0u};
+  const int K = (int)p.Kd, steps = (K + STEP - 1) / STEP;
+  for (int s0 = wave; s0 < steps; s0 += WK * UN) {
+    u4 wv[UN], xv[MT][UN];
+#pragma unroll
+    for (int q = 0; q < UN; ++q) {
+      const int k = (s0 + q * WK) * STEP;
+      const bool in = k + ch * EPC < K;
+      wv[q] = in ? ld16(w + k) : zero;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xv[m][q] = in ? ld16(x[m] + k) : zero;
+    }
+#pragma unroll
+    for (int q = 0; q < UN; ++q)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if constexpr (std::is_same<T, float>::value) {
+          const f4 a = __builtin_bit_cast(f4, wv[q]), b = __builtin_bit_cast(f4, xv[m][q]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], acc[m], 0, 0, 0);
+        } else if constexpr (std::is_same<T, half_t>::value) {
+          acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, wv[q]), __builtin_bit_cast(h8, xv[m][q]), acc[m], 0, 0, 0);
+        } else {
+          acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, wv[q]), __builtin_bit_cast(b8, xv[m][q]), acc[m], 0, 0, 0);
+        }
+      }
+  }
+  // lane: row of x l % 16, units 4 (l / 16) + 0 .. 3
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[wave][m * 16 + r][ch * 4 + e] = acc[m][e];
+  __syncthreads();
+  for (int o = tid; o < MT * 256; o += 64 * WK) {
+    const int i = o >> 4, j = o & 15;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < WK; ++k) v += red[k][i][j];
+    if (i < M && j0 + j < p.J) epilogue1<SEG_LINEAR_FWD, T>(p, i, j0 + j, v);
+  }
+}
+
 // the split ranges of k added in order, then the epilogue
 template <int PASS, typename T>
 __global__ __launch_bounds__(TPB) void gemm_join_kernel(const GemmArgs p) {
@@ -470,7 +528,7 @@ inline ColsumPlan colsum_plan(int64_t rows, int cols) {
 }
 
 // ---- plans
-enum { TILE_ANY = 0, TILE_128 = 1, TILE_256 = 2 };
+enum { TILE_ANY = 0, TILE_128 = 1, TILE_256 = 2, FEW_ROWS = 3 };
 struct GemmPlan { int kind; int ti, tj, splits; int64_t kper; };
 inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   GemmPlan g;
@@ -520,8 +578,15 @@ inline bool dma_ok(const seg_linear_args& a, int pass) {
   // tiles far larger than the result waste the matrix cores
   return e.I >= 64 && e.J >= 64;
 }
+// up to 64 rows forward, every row of both operands in 16-byte pieces
+inline bool rows_ok(const seg_linear_args& a, int pass) {
+  if (pass != SEG_LINEAR_FWD || a.M > 64) return false;
+  const int64_t u = a.dtype == SEG_DT_F32 ? 4 : 8;
+  return aligned16(a.x) && aligned16(a.w) && a.x_ld % u == 0 && a.w_ld % u == 0 && a.K % u == 0;
+}
 inline GemmPlan plan_of(const seg_linear_args& a, int pass) {
   const Extents e = extents(a, pass);
+  if (rows_ok(a, pass)) return {FEW_ROWS, 1, (e.J + 15) / 16, 1, e.Kd};
   return gemm_plan(e.I, e.J, e.Kd, a.dtype, dma_ok(a, pass));
 }
 
@@ -539,7 +604,17 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
   const int vec = vec_of(p.A, p.a_ld, p.B, p.b_ld, a.dtype);
   seq_dispatch_dtype(a.dtype, [&](auto* tp) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
-    if (g.kind != TILE_ANY) {
+    if (g.kind == FEW_ROWS) {
+      if constexpr (PASS == SEG_LINEAR_FWD) {
+        // 16 waves per block where the blocks alone do not fill the card
+        const bool deep = g.tj < 256;
+#define ROWS_CASE(m, wk) hipLaunchKernelGGL((gemm_rows_kernel<T, m, wk>), dim3((unsigned)g.tj), dim3(64 * wk), 0, st, p)
+        if (p.I <= 16) { if (deep) ROWS_CASE(1, 16); else ROWS_CASE(1, 8); }
+        else if (p.I <= 32) { if (deep) ROWS_CASE(2, 16); else ROWS_CASE(2, 8); }
+        else ROWS_CASE(4, 8);
+#undef ROWS_CASE
+      }
+    } else if (g.kind != TILE_ANY) {
       if constexpr (!std::is_same<T, float>::value) {
         if (g.kind == TILE_256) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 256, 256, 2, 4, 64, 2, 2>), grid, dim3(512), 0, st, p);
         else hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 128, 2, 2, 64, 2, 2>), grid, dim3(256), 0, st, p);

@@ -19,7 +19,7 @@
 namespace {
 
 constexpr int TT = 32;            // rows per tile = distance of the saved states
-constexpr int SUB = 16;           // rows whose a and h the backward pass holds in registers
+constexpr int SUB = 8;            // rows whose a and h the backward pass holds in registers
 constexpr int MAXS = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -29,7 +29,9 @@ template <int G> struct Lay {
   static constexpr int NW = NT / 64;
   static constexpr int SP = 4 * G;                             // states, padded
   static constexpr int CHUNKS = CB / 8;                        // 8-channel pieces of a row
-  static constexpr int TASKS = TT * CHUNKS;
+  static constexpr int TASKS = TT * CHUNKS;                    // pieces of a tile
+  static constexpr int PIECES = TASKS > NT ? TASKS / NT : 1;   // of these per thread (G > 4: the first TASKS threads, one each)
+  static constexpr int ROWS = NT / CHUNKS;                     // rows between a thread's pieces
 };
 
 __device__ __forceinline__ float exp2_f(float v) { return __builtin_amdgcn_exp2f(v); }
@@ -79,39 +81,59 @@ __device__ __forceinline__ void store_states(float* row, int s0, int S, f4 h) {
       if (s0 + i < S) row[s0 + i] = h[i];
   }
 }
-// rows t0 .. t0 + TT of Bm / Cm as fp32 [TT][SP]; zero behind the length and behind S
-template <typename T, int G>
-__device__ __forceinline__ void stage_states(const T* m, int64_t bs, int64_t ld, int b, int t0, int len, int S, float* dst) {
-  for (int e = threadIdx.x; e < TT * Lay<G>::SP; e += Lay<G>::NT) {
-    const int t = t0 + e / Lay<G>::SP, s = e % Lay<G>::SP;
-    dst[e] = (t < len && s < S) ? (float)m[b * bs + t * ld + s] : 0.f;
-  }
-}
 template <bool VEC> __device__ __forceinline__ void load_chan(const float* p, int c, int n, float* f) {
   row_load8<float, VEC>(p + c, p != nullptr ? n : 0, f);
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void stage_delta(const seg_scan_args& p, int b, int t, int len, int c, int n, const float* bias, float* delta) {
-  row_load8<T, VEC>((const T*)p.dt + b * p.dt_bs + t * p.dt_ld + c, t < len ? n : 0, delta);
+// A tile's rows on their way: every thread fetches its 8-channel pieces (PIECES of them: one row each) and its share of the tile's
+// Bm / Cm elements a tile ahead, in their memory format, so that no wave waits for memory between two tiles.
+template <typename T, bool VEC> struct Raw {
+  typedef T tv __attribute__((ext_vector_type(8)));
+  tv v;
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if constexpr (VEC) {
+      if (n > 0) v = *reinterpret_cast<const tv*>(p);
+      else v = tv{};
+    } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float v = delta[j] + bias[j];
-    delta[j] = t < len ? (p.softplus ? softplus_f(v) : v) : 0.f;
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (T)0.f;
+    }
   }
+  __device__ __forceinline__ float operator[](int j) const { return (float)v[j]; }
+};
+template <typename T, int G> struct RawStates {
+  static constexpr int N = TT * Lay<G>::SP / Lay<G>::NT;
+  T v[N];
+  __device__ __forceinline__ void load(const T* m, int64_t bs, int64_t ld, int b, int t0, int len, int S) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = threadIdx.x + i * Lay<G>::NT, t = t0 + e / Lay<G>::SP, s = e % Lay<G>::SP;
+      v[i] = (t < len && s < S) ? m[b * bs + t * ld + s] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ void put(float* dst) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) dst[threadIdx.x + i * Lay<G>::NT] = (float)v[i];
+  }
+};
+// delta of eight channels from the raw step; 0 behind the length
+__device__ __forceinline__ float delta_of(const seg_scan_args& p, float dt, float bias, bool on) {
+  const float v = dt + bias;
+  return on ? (p.softplus ? softplus_f(v) : v) : 0.f;
 }
 
 // MAIN: y, saved states and the last state from the chunk's true start; else the chunk's last state from zero and its sum of delta
 template <typename T, bool VEC, int G, bool MAIN>
-__global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_args p, int clen, float* start, float* sumd) {
+__global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_args p, int clen, int nch, float* start, float* sumd) {
   typedef Lay<G> Y;
   __shared__ float2 sdu[TT][Y::CB];
   __shared__ __align__(16) float sB[TT * Y::SP], sC[MAIN ? TT * Y::SP : 1];
   __shared__ __align__(16) float sy[MAIN ? TT : 1][Y::CB];
-  const int tid = threadIdx.x, g = tid % G, c = tid / G, b = blockIdx.z, chunk = blockIdx.y, nch = gridDim.y;
+  const int tid = threadIdx.x, g = tid % G, c = tid / G, b = blockIdx.z, chunk = blockIdx.y;
   const int c0 = blockIdx.x * Y::CB, d = c0 + c, len = scan_len(p, b);
   const bool live = d < p.D;
   const int tbeg = chunk * clen, tend = tbeg + clen < p.L ? tbeg + clen : p.L;
-  const int q0c = (tid % Y::CHUNKS) * 8, tc = c0 + q0c, tn = tc < p.D ? p.D - tc : 0;      // this thread's channels when staging rows
+  const int row0 = tid / Y::CHUNKS, q0c = (tid % Y::CHUNKS) * 8, tc = c0 + q0c, tn = tc < p.D ? p.D - tc : 0;      // this thread's piece of the rows
+  const bool worker = tid < Y::TASKS;
   float bias[8], skip[8];
   load_chan<VEC>(p.dt_bias, tc, tn, bias);
   if constexpr (MAIN) load_chan<VEC>(p.Dskip, tc, tn, skip);
@@ -125,50 +147,77 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_arg
   }
   float dsum = 0.f;
   const int64_t nck = (p.L + TT - 1) / TT;
+  Raw<T, VEC> ru[Y::PIECES], rt[Y::PIECES], rz[MAIN ? Y::PIECES : 1], cu[Y::PIECES], cz[MAIN ? Y::PIECES : 1];
+  RawStates<T, G> rB, rC;
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < Y::PIECES; ++i) {
+      const int t = t0 + row0 + i * Y::ROWS, n = worker && t < len ? tn : 0;
+      ru[i].load((const T*)p.u + b * p.u_bs + t * p.u_ld + tc, n);
+      rt[i].load((const T*)p.dt + b * p.dt_bs + t * p.dt_ld + tc, n);
+      if constexpr (MAIN) rz[i].load((const T*)p.z + b * p.z_bs + t * p.z_ld + tc, p.z != nullptr ? n : 0);
+    }
+    rB.load((const T*)p.Bm, p.Bm_bs, p.Bm_ld, b, t0, len, p.S);
+    if constexpr (MAIN) rC.load((const T*)p.Cm, p.Cm_bs, p.Cm_ld, b, t0, len, p.S);
+  };
+  const int tlive = tend < len ? tend : len;                   // rows from here on leave the state as it is: their y is 0
+  if (tbeg < tlive) fetch(tbeg);
   for (int t0 = tbeg; t0 < tend; t0 += TT) {
     if constexpr (MAIN) {
       if (p.saved != nullptr && live) store_states(p.saved + (((int64_t)b * nck + t0 / TT) * p.D + d) * p.S, 4 * g, p.S, h);
     }
-    for (int q = tid; q < Y::TASKS; q += Y::NT) {
-      const int r = q / Y::CHUNKS, t = t0 + r;
-      float delta[8], u[8];
-      stage_delta<T, VEC>(p, b, t, len, tc, tn, bias, delta);
-      row_load8<T, VEC>((const T*)p.u + b * p.u_bs + t * p.u_ld + tc, t < len ? tn : 0, u);
+    if (t0 < tlive) {                                          // (block-uniform)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sdu[r][q0c + j] = float2{delta[j], delta[j] * u[j]};
-    }
-    stage_states<T, G>((const T*)p.Bm, p.Bm_bs, p.Bm_ld, b, t0, len, p.S, sB);
-    if constexpr (MAIN) stage_states<T, G>((const T*)p.Cm, p.Cm_bs, p.Cm_ld, b, t0, len, p.S, sC);
-    __syncthreads();
-#pragma unroll 4
-    for (int r = 0; r < TT; ++r) {
-      const float2 dd = sdu[r][c];
-      const f4 B4 = *reinterpret_cast<const f4*>(sB + r * Y::SP + 4 * g);
+      for (int i = 0; i < Y::PIECES; ++i) {
+        const int r = row0 + i * Y::ROWS;
+        cu[i] = ru[i];
+        if constexpr (MAIN) cz[i] = rz[i];
+        if (worker) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_f(dd.x * A2[i]), h[i], dd.y * B4[i]);
-      if constexpr (MAIN) {
-        const f4 C4 = *reinterpret_cast<const f4*>(sC + r * Y::SP + 4 * g);
-        const float y = group_sum<G>(fmaf(C4[3], h[3], fmaf(C4[2], h[2], fmaf(C4[1], h[1], C4[0] * h[0]))));
-        if (g == 0) sy[r][c] = y;
-      } else {
-        dsum += dd.x;
-      }
-    }
-    __syncthreads();
-    if constexpr (MAIN) {
-      for (int q = tid; q < Y::TASKS; q += Y::NT) {
-        const int r = q / Y::CHUNKS, t = t0 + r;
-        if (t < tend && tn > 0) {
-          float u[8], z[8], y[8];
-          row_load8<T, VEC>((const T*)p.u + b * p.u_bs + t * p.u_ld + tc, t < len ? tn : 0, u);
-          if (p.z != nullptr) row_load8<T, VEC>((const T*)p.z + b * p.z_bs + t * p.z_ld + tc, t < len ? tn : 0, z);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            y[j] = fmaf(skip[j], u[j], sy[r][q0c + j]);
-            if (p.z != nullptr) y[j] *= z[j] * sigmoid_f(z[j]);
-            if (t >= len) y[j] = 0.f;
+          for (int j = 0; j < 8; j += 2) {
+            const float d0 = delta_of(p, rt[i][j], bias[j], t0 + r < len), d1 = delta_of(p, rt[i][j + 1], bias[j + 1], t0 + r < len);
+            *reinterpret_cast<f4*>(&sdu[r][q0c + j]) = f4{d0, d0 * ru[i][j], d1, d1 * ru[i][j + 1]};
           }
-          row_store8<T, VEC>((T*)p.y + b * p.y_bs + t * p.y_ld + tc, tn, y);
+        }
+      }
+      rB.put(sB);
+      if constexpr (MAIN) rC.put(sC);
+      if (t0 + TT < tlive) fetch(t0 + TT);
+      __syncthreads();
+#pragma unroll 4
+      for (int r = 0; r < TT; ++r) {
+        const float2 dd = sdu[r][c];
+        const f4 B4 = *reinterpret_cast<const f4*>(sB + r * Y::SP + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_f(dd.x * A2[i]), h[i], dd.y * B4[i]);
+        if constexpr (MAIN) {
+          const f4 C4 = *reinterpret_cast<const f4*>(sC + r * Y::SP + 4 * g);
+          const float y = group_sum<G>(fmaf(C4[3], h[3], fmaf(C4[2], h[2], fmaf(C4[1], h[1], C4[0] * h[0]))));
+          if (g == 0) sy[r][c] = y;
+        } else {
+          dsum += dd.x;
+        }
+      }
+      __syncthreads();
+    }
+    if constexpr (MAIN) {
+      if (worker && tn > 0) {
+#pragma unroll
+        for (int i = 0; i < Y::PIECES; ++i) {
+          const int r = row0 + i * Y::ROWS, t = t0 + r;
+          if (t < tend) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = 0.f;
+            if (t < len) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                y[j] = fmaf(skip[j], cu[i][j], sy[r][q0c + j]);
+                if (p.z != nullptr) y[j] *= cz[i][j] * sigmoid_f(cz[i][j]);
+              }
+            }
+            row_store8<T, VEC>((T*)p.y + b * p.y_bs + t * p.y_ld + tc, tn, y);
+          }
         }
       }
       // (the next tile's staging writes sdu / sB / sC, whose readers are past the barrier above; sy is written behind its own next barrier)
@@ -194,6 +243,10 @@ __global__ __launch_bounds__(256) void scan_join_kernel(const seg_scan_args p, i
   float h = p.state != nullptr ? p.state[b * n + e] : 0.f;
   for (int k = 0; k < nch; ++k) {
     const int64_t o = (int64_t)b * nch + k;
+    if (k == nch - 1) {                                        // (its own last state was not computed: nothing starts behind it)
+      start[o * n + e] = h;
+      return;
+    }
     const float own = start[o * n + e];
     start[o * n + e] = h;
     h = fmaf(exp2_f(A2 * sumd[o * p.D + d]), h, own);
@@ -209,48 +262,65 @@ __global__ __launch_bounds__(256) void scan_join_bwd_kernel(const seg_scan_args 
   float q = p.dstate_out != nullptr ? p.dstate_out[b * n + e] : 0.f;
   for (int k = nch - 1; k >= 0; --k) {
     const int64_t o = (int64_t)b * nch + k;
+    if (k == 0) {                                              // (its own part was not computed: nothing lies in front of it)
+      adj[o * n + e] = q;
+      return;
+    }
     const float own = adj[o * n + e];
     adj[o * n + e] = q;
     q = fmaf(exp2_f(A2 * sumd[o * p.D + d]), q, own);
   }
 }
 
+// dp = dy silu(z) of a piece
 template <typename T, bool VEC>
-__device__ __forceinline__ void stage_dp(const seg_scan_args& p, int b, int t, int len, int c, int n, float* dp, float* z) {
-  row_load8<T, VEC>((const T*)p.dy + b * p.dy_bs + t * p.dy_ld + c, t < len ? n : 0, dp);
-  if (p.z != nullptr) {
-    row_load8<T, VEC>((const T*)p.z + b * p.z_bs + t * p.z_ld + c, t < len ? n : 0, z);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dp[j] *= z[j] * sigmoid_f(z[j]);
-  }
+__device__ __forceinline__ float dp_of(const seg_scan_args& p, const Raw<T, VEC>& dy, const Raw<T, VEC>& z, int j) {
+  return p.z != nullptr ? dy[j] * z[j] * sigmoid_f(z[j]) : dy[j];
 }
 
-// a chunk's own part of the adjoint in front of it, and its sum of delta
+// a chunk's own part of the adjoint in front of it, and its sum of delta (chunks 1 ..: blockIdx.y + 1)
 template <typename T, bool VEC, int G>
-__global__ __launch_bounds__(Lay<G>::NT) void scan_bwd_local_kernel(const seg_scan_args p, int clen, float* adj, float* sumd) {
+__global__ __launch_bounds__(Lay<G>::NT) void scan_bwd_local_kernel(const seg_scan_args p, int clen, int nch, float* adj, float* sumd) {
   typedef Lay<G> Y;
   __shared__ float2 sdp[TT][Y::CB];
   __shared__ __align__(16) float sC[TT * Y::SP];
-  const int tid = threadIdx.x, g = tid % G, c = tid / G, b = blockIdx.z, chunk = blockIdx.y, nch = gridDim.y;
+  const int tid = threadIdx.x, g = tid % G, c = tid / G, b = blockIdx.z, chunk = blockIdx.y + 1;
   const int c0 = blockIdx.x * Y::CB, d = c0 + c, len = scan_len(p, b);
   const bool live = d < p.D;
-  const int tbeg = chunk * clen, tend = tbeg + clen < p.L ? tbeg + clen : p.L;
-  const int q0c = (tid % Y::CHUNKS) * 8, tc = c0 + q0c, tn = tc < p.D ? p.D - tc : 0;
+  const int tbeg = chunk * clen, tend = tbeg + clen < p.L ? tbeg + clen : p.L, tlive = tend < len ? tend : len;
+  const int row0 = tid / Y::CHUNKS, q0c = (tid % Y::CHUNKS) * 8, tc = c0 + q0c, tn = tc < p.D ? p.D - tc : 0;
+  const bool worker = tid < Y::TASKS;
   float bias[8];
   load_chan<VEC>(p.dt_bias, tc, tn, bias);
   f4 A2 = {0.f, 0.f, 0.f, 0.f}, P = {1.f, 1.f, 1.f, 1.f}, q = A2;
   if (live) A2 = load_states(p.A + (int64_t)d * p.S, 4 * g, p.S) * LOG2E;
   float dsum = 0.f;
-  for (int t0 = tbeg; t0 < tend; t0 += TT) {
-    for (int k = tid; k < Y::TASKS; k += Y::NT) {
-      const int r = k / Y::CHUNKS, t = t0 + r;
-      float delta[8], dp[8], z[8];
-      stage_delta<T, VEC>(p, b, t, len, tc, tn, bias, delta);
-      stage_dp<T, VEC>(p, b, t, len, tc, tn, dp, z);
+  Raw<T, VEC> rt[Y::PIECES], ry[Y::PIECES], rz[Y::PIECES];
+  RawStates<T, G> rC;
+  auto fetch = [&](int t0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sdp[r][q0c + j] = float2{delta[j], dp[j]};
+    for (int i = 0; i < Y::PIECES; ++i) {
+      const int t = t0 + row0 + i * Y::ROWS, n = worker && t < len ? tn : 0;
+      rt[i].load((const T*)p.dt + b * p.dt_bs + t * p.dt_ld + tc, n);
+      ry[i].load((const T*)p.dy + b * p.dy_bs + t * p.dy_ld + tc, n);
+      rz[i].load((const T*)p.z + b * p.z_bs + t * p.z_ld + tc, p.z != nullptr ? n : 0);
     }
-    stage_states<T, G>((const T*)p.Cm, p.Cm_bs, p.Cm_ld, b, t0, len, p.S, sC);
+    rC.load((const T*)p.Cm, p.Cm_bs, p.Cm_ld, b, t0, len, p.S);
+  };
+  if (tbeg < tlive) fetch(tbeg);
+  for (int t0 = tbeg; t0 < tlive; t0 += TT) {
+    if (worker) {
+#pragma unroll
+      for (int i = 0; i < Y::PIECES; ++i) {
+        const int r = row0 + i * Y::ROWS;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+          *reinterpret_cast<f4*>(&sdp[r][q0c + j]) = f4{delta_of(p, rt[i][j], bias[j], t0 + r < len), dp_of<T, VEC>(p, ry[i], rz[i], j),
+                                                       delta_of(p, rt[i][j + 1], bias[j + 1], t0 + r < len), dp_of<T, VEC>(p, ry[i], rz[i], j + 1)};
+      }
+    }
+    rC.put(sC);
+    if (t0 + TT < tlive) fetch(t0 + TT);
     __syncthreads();
 #pragma unroll 4
     for (int r = 0; r < TT; ++r) {
@@ -294,17 +364,19 @@ template <int G> __device__ __forceinline__ void lane_sums(const float* v, float
 // the gradients of a chunk.  adj: the adjoint that enters each chunk from behind (NULL: one chunk, dstate_out).  Partial sums:
 // pbc[channel block][B][L][2][S] (dB, dC), pA[B nch][D][S], pD[B nch][2][D] (dD, ddt_bias)
 template <typename T, bool VEC, int G>
-__global__ __launch_bounds__(Lay<G>::NT) void scan_bwd_kernel(const seg_scan_args p, int clen, const float* adj, float* pbc, float* pA, float* pD) {
+__global__ __launch_bounds__(Lay<G>::NT, 2) void scan_bwd_kernel(const seg_scan_args p, int clen, const float* adj, float* pbc, float* pA, float* pD) {
   typedef Lay<G> Y;
   __shared__ f4 sx[TT][Y::CB];                               // delta, u -> sum g B, dp -> sum g a h A, -> C . h
   __shared__ __align__(16) float sB[TT * Y::SP], sC[TT * Y::SP];
   __shared__ __align__(16) float sbc[Y::NW][SUB][2][Y::SP];
+  __shared__ f4 shs[TT / SUB - 1][Y::NT];                    // the states in front of every SUB rows of the tile but the first
   const int tid = threadIdx.x, g = tid % G, c = tid / G, b = blockIdx.z, chunk = blockIdx.y, nch = gridDim.y;
   const int lane = tid & 63, wave = tid >> 6;
   const int c0 = blockIdx.x * Y::CB, d = c0 + c, len = scan_len(p, b);
   const bool live = d < p.D;
-  const int tbeg = chunk * clen, tend = tbeg + clen < p.L ? tbeg + clen : p.L;
-  const int q0c = (tid % Y::CHUNKS) * 8, tc = c0 + q0c, tn = tc < p.D ? p.D - tc : 0;
+  const int tbeg = chunk * clen, tend = tbeg + clen < p.L ? tbeg + clen : p.L, tlive = tend < len ? tend : len;
+  const int row0 = tid / Y::CHUNKS, q0c = (tid % Y::CHUNKS) * 8, tc = c0 + q0c, tn = tc < p.D ? p.D - tc : 0;
+  const bool worker = tid < Y::TASKS;
   float bias[8], skip[8], accD[8], accB[8];
   load_chan<VEC>(p.dt_bias, tc, tn, bias);
   load_chan<VEC>(p.Dskip, tc, tn, skip);
@@ -318,125 +390,181 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_bwd_kernel(const seg_scan_arg
     else if (p.dstate_out != nullptr) q = load_states(p.dstate_out + ((int64_t)b * p.D + d) * p.S, 4 * g, p.S);
   }
   const int64_t nck = (p.L + TT - 1) / TT;
-  const int ntile = tend > tbeg ? (tend - tbeg + TT - 1) / TT : 0;
+  // rows behind the length: gradients are 0, the adjoint passes
+  for (int t = (tlive > tbeg ? tlive : tbeg) + row0; worker && tn > 0 && t < tend; t += (Y::ROWS < TT ? Y::ROWS : TT)) {
+    float o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = 0.f;
+    if (p.du != nullptr) row_store8<T, VEC>((T*)p.du + b * p.du_bs + t * p.du_ld + tc, tn, o);
+    if (p.ddt != nullptr) row_store8<T, VEC>((T*)p.ddt + b * p.ddt_bs + t * p.ddt_ld + tc, tn, o);
+    if (p.dz != nullptr) row_store8<T, VEC>((T*)p.dz + b * p.dz_bs + t * p.dz_ld + tc, tn, o);
+  }
+  if (pbc != nullptr) {
+    const int t1 = tlive > tbeg ? tlive : tbeg;
+    for (int64_t e = tid; e < (int64_t)(tend - t1) * 2 * p.S; e += Y::NT) pbc[(((int64_t)blockIdx.x * p.B + b) * p.L + t1) * 2 * p.S + e] = 0.f;
+  }
+  Raw<T, VEC> ru[Y::PIECES], rt[Y::PIECES], rz[Y::PIECES], ry[Y::PIECES];
+  RawStates<T, G> rB, rC;
+  f4 rh = {0.f, 0.f, 0.f, 0.f};
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < Y::PIECES; ++i) {
+      const int t = t0 + row0 + i * Y::ROWS, n = worker && t < len ? tn : 0;
+      ru[i].load((const T*)p.u + b * p.u_bs + t * p.u_ld + tc, n);
+      rt[i].load((const T*)p.dt + b * p.dt_bs + t * p.dt_ld + tc, n);
+      rz[i].load((const T*)p.z + b * p.z_bs + t * p.z_ld + tc, p.z != nullptr ? n : 0);
+      ry[i].load((const T*)p.dy + b * p.dy_bs + t * p.dy_ld + tc, n);
+    }
+    rB.load((const T*)p.Bm, p.Bm_bs, p.Bm_ld, b, t0, len, p.S);
+    rC.load((const T*)p.Cm, p.Cm_bs, p.Cm_ld, b, t0, len, p.S);
+    if (live) rh = load_states(p.saved + (((int64_t)b * nck + t0 / TT) * p.D + d) * p.S, 4 * g, p.S);
+  };
+  const int ntile = tlive > tbeg ? (tlive - tbeg + TT - 1) / TT : 0;
+  if (ntile > 0) fetch(tbeg + (ntile - 1) * TT);
   for (int tile = ntile - 1; tile >= 0; --tile) {
     const int t0 = tbeg + tile * TT;
-    f4 hs = {0.f, 0.f, 0.f, 0.f};
-    if (live) hs = load_states(p.saved + (((int64_t)b * nck + t0 / TT) * p.D + d) * p.S, 4 * g, p.S);
-    for (int k = tid; k < Y::TASKS; k += Y::NT) {
-      const int r = k / Y::CHUNKS, t = t0 + r;
-      float delta[8], u[8], dp[8], z[8];
-      stage_delta<T, VEC>(p, b, t, len, tc, tn, bias, delta);
-      row_load8<T, VEC>((const T*)p.u + b * p.u_bs + t * p.u_ld + tc, t < len ? tn : 0, u);
-      stage_dp<T, VEC>(p, b, t, len, tc, tn, dp, z);
+    Raw<T, VEC> cu[Y::PIECES], ct[Y::PIECES], cz[Y::PIECES], cy[Y::PIECES];
+    f4 h = rh;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sx[r][q0c + j] = f4{delta[j], u[j], dp[j], 0.f};
+    for (int i = 0; i < Y::PIECES; ++i) {
+      const int r = row0 + i * Y::ROWS;
+      cu[i] = ru[i]; ct[i] = rt[i]; cz[i] = rz[i]; cy[i] = ry[i];
+      if (worker) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sx[r][q0c + j] = f4{delta_of(p, rt[i][j], bias[j], t0 + r < len), ru[i][j], dp_of<T, VEC>(p, ry[i], rz[i], j), 0.f};
+      }
     }
-    stage_states<T, G>((const T*)p.Bm, p.Bm_bs, p.Bm_ld, b, t0, len, p.S, sB);
-    stage_states<T, G>((const T*)p.Cm, p.Cm_bs, p.Cm_ld, b, t0, len, p.S, sC);
+    rB.put(sB);
+    rC.put(sC);
     __syncthreads();
-    f4 hmid = hs;                                            // the state in front of the tile's second half
-#pragma unroll 4
-    for (int r = 0; r < SUB; ++r) {
-      const f4 x = sx[r][c];
-      const f4 B4 = *reinterpret_cast<const f4*>(sB + r * Y::SP + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) hmid[i] = fmaf(exp2_f(x[0] * A2[i]), hmid[i], x[0] * x[1] * B4[i]);
-    }
+    // (a row's LDS reads are issued one row ahead, no further: left alone the compiler moves all of a sub-tile's reads to its front, and
+    // their registers leave one wave per SIMD)
+    const f4 h0 = h;
 #pragma unroll 1
-    for (int half = TT / SUB - 1; half >= 0; --half) {
-      f4 a[SUB], hp[SUB], h = half ? hmid : hs;
+    for (int s = 1; s < TT / SUB; ++s) {
+      const int r0 = (s - 1) * SUB;
+      float2 x = *reinterpret_cast<const float2*>(&sx[r0][c]);
+      f4 B4 = *reinterpret_cast<const f4*>(sB + r0 * Y::SP + 4 * g);
 #pragma unroll
       for (int k = 0; k < SUB; ++k) {
-        const int r = half * SUB + k;
-        const f4 x = sx[r][c];
-        const f4 B4 = *reinterpret_cast<const f4*>(sB + r * Y::SP + 4 * g), C4 = *reinterpret_cast<const f4*>(sC + r * Y::SP + 4 * g);
-        const float du = x[0] * x[1];
-        hp[k] = h;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[k][i] = exp2_f(x[0] * A2[i]);
-          h[i] = fmaf(a[k][i], h[i], du * B4[i]);
+        const float2 xc = x;
+        const f4 Bc = B4;
+        if (k + 1 < SUB) {
+          x = *reinterpret_cast<const float2*>(&sx[r0 + k + 1][c]);
+          B4 = *reinterpret_cast<const f4*>(sB + (r0 + k + 1) * Y::SP + 4 * g);
         }
-        const float y = group_sum<G>(fmaf(C4[3], h[3], fmaf(C4[2], h[2], fmaf(C4[1], h[1], C4[0] * h[0]))));
-        if (g == 0) sx[r][c][3] = y;
+        const float du = xc.x * xc.y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_f(xc.x * A2[i]), h[i], du * Bc[i]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      shs[s - 1][tid] = h;
+    }
+#pragma unroll 1
+    for (int s = TT / SUB - 1; s >= 0; --s) {
+      f4 a[SUB], hp[SUB];
+      const int r0 = s * SUB;
+      h = s > 0 ? shs[s - 1][tid] : h0;
+      {
+        float2 x = *reinterpret_cast<const float2*>(&sx[r0][c]);
+        f4 B4 = *reinterpret_cast<const f4*>(sB + r0 * Y::SP + 4 * g), C4 = *reinterpret_cast<const f4*>(sC + r0 * Y::SP + 4 * g);
+#pragma unroll
+        for (int k = 0; k < SUB; ++k) {
+          const float2 xc = x;
+          const f4 Bc = B4, Cc = C4;
+          if (k + 1 < SUB) {
+            x = *reinterpret_cast<const float2*>(&sx[r0 + k + 1][c]);
+            B4 = *reinterpret_cast<const f4*>(sB + (r0 + k + 1) * Y::SP + 4 * g);
+            C4 = *reinterpret_cast<const f4*>(sC + (r0 + k + 1) * Y::SP + 4 * g);
+          }
+          const float du = xc.x * xc.y;
+          hp[k] = h;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            a[k][i] = exp2_f(xc.x * A2[i]);
+            h[i] = fmaf(a[k][i], h[i], du * Bc[i]);
+          }
+          const float y = group_sum<G>(fmaf(Cc[3], h[3], fmaf(Cc[2], h[2], fmaf(Cc[1], h[1], Cc[0] * h[0]))));
+          if (g == 0) sx[r0 + k][c][3] = y;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      f4 x = sx[r0 + SUB - 1][c];
+      f4 B4 = *reinterpret_cast<const f4*>(sB + (r0 + SUB - 1) * Y::SP + 4 * g), C4 = *reinterpret_cast<const f4*>(sC + (r0 + SUB - 1) * Y::SP + 4 * g);
 #pragma unroll
       for (int k = SUB - 1; k >= 0; --k) {
-        const int r = half * SUB + k;
-        const f4 x = sx[r][c];
-        const f4 B4 = *reinterpret_cast<const f4*>(sB + r * Y::SP + 4 * g), C4 = *reinterpret_cast<const f4*>(sC + r * Y::SP + 4 * g);
-        const float du = x[0] * x[1];
+        const f4 xc = x, Bc = B4, Cc = C4;
+        if (k > 0) {
+          x = sx[r0 + k - 1][c];
+          B4 = *reinterpret_cast<const f4*>(sB + (r0 + k - 1) * Y::SP + 4 * g);
+          C4 = *reinterpret_cast<const f4*>(sC + (r0 + k - 1) * Y::SP + 4 * g);
+        }
+        const float du = xc[0] * xc[1];
         float v[8], w[2], sgB = 0.f, sA = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float gi = fmaf(C4[i], x[2], q[i]);
+          const float gi = fmaf(Cc[i], xc[2], q[i]);
           const float ga = gi * a[k][i], gh = ga * hp[k][i];
-          sgB = fmaf(gi, B4[i], sgB);
+          sgB = fmaf(gi, Bc[i], sgB);
           sA = fmaf(gh, A[i], sA);
-          dA[i] = fmaf(gh, x[0], dA[i]);
+          dA[i] = fmaf(gh, xc[0], dA[i]);
           v[i] = gi * du;
-          v[4 + i] = x[2] * h[i];
+          v[4 + i] = xc[2] * h[i];
           q[i] = ga;
         }
         h = hp[k];
         sgB = group_sum<G>(sgB);
         sA = group_sum<G>(sA);
-        if (g == 0) { sx[r][c][1] = sgB; sx[r][c][2] = sA; }
+        if (g == 0) { sx[r0 + k][c][1] = sgB; sx[r0 + k][c][2] = sA; }
         lane_sums<G>(v, w);
-        if ((lane & 15) < G) {
-          float* o = &sbc[wave][k][lane >> 5][4 * g + 2 * ((lane >> 4) & 1)];
-          o[0] = w[0];
-          o[1] = w[1];
-        }
+        if ((lane & 15) < G) *reinterpret_cast<float2*>(&sbc[wave][k][lane >> 5][4 * g + 2 * ((lane >> 4) & 1)]) = float2{w[0], w[1]};
+        __builtin_amdgcn_sched_barrier(0);
       }
       __syncthreads();
       if (pbc != nullptr) {
         for (int e = tid; e < SUB * 2 * Y::SP; e += Y::NT) {
-          const int k = e / (2 * Y::SP), wh = (e / Y::SP) & 1, s = e % Y::SP, t = t0 + half * SUB + k;
-          if (t < tend && s < p.S) {
+          const int k = e / (2 * Y::SP), wh = (e / Y::SP) & 1, st = e % Y::SP, t = t0 + s * SUB + k;
+          if (t < tlive && st < p.S) {
             float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < Y::NW; ++w) v += sbc[w][k][wh][s];
-            pbc[((((int64_t)blockIdx.x * p.B + b) * p.L + t) * 2 + wh) * p.S + s] = v;
+            for (int w = 0; w < Y::NW; ++w) v += sbc[w][k][wh][st];
+            pbc[((((int64_t)blockIdx.x * p.B + b) * p.L + t) * 2 + wh) * p.S + st] = v;
           }
         }
       }
       __syncthreads();
     }
-    for (int k = tid; k < Y::TASKS; k += Y::NT) {
-      const int r = k / Y::CHUNKS, t = t0 + r;
-      if (t < tend && tn > 0) {
-        float u[8], dp[8], z[8], dtv[8], dout[8], o[8];
-        const int n = t < len ? tn : 0;
-        row_load8<T, VEC>((const T*)p.u + b * p.u_bs + t * p.u_ld + tc, n, u);
-        row_load8<T, VEC>((const T*)p.dt + b * p.dt_bs + t * p.dt_ld + tc, n, dtv);
-        row_load8<T, VEC>((const T*)p.dy + b * p.dy_bs + t * p.dy_ld + tc, n, dout);
-        stage_dp<T, VEC>(p, b, t, len, tc, tn, dp, z);
-        f4 x[8];
+    if (tile > 0) fetch(t0 - TT);
+    if (worker && tn > 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = sx[r][q0c + j];
-        if (p.du != nullptr) {
+      for (int i = 0; i < Y::PIECES; ++i) {
+        const int r = row0 + i * Y::ROWS, t = t0 + r;
+        if (t < tlive) {
+          float o[8];
+          f4 x[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = t < len ? fmaf(skip[j], dp[j], x[j][0] * x[j][1]) : 0.f;
-          row_store8<T, VEC>((T*)p.du + b * p.du_bs + t * p.du_ld + tc, tn, o);
-        }
+          for (int j = 0; j < 8; ++j) x[j] = sx[r][q0c + j];
+          if (p.du != nullptr) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          o[j] = fmaf(x[j][1], u[j], x[j][2]);
-          if (p.softplus) o[j] *= sigmoid_f(dtv[j] + bias[j]);
-          if (t >= len) o[j] = 0.f;
-          accB[j] += o[j];
-          accD[j] = fmaf(dp[j], u[j], accD[j]);
-        }
-        if (p.ddt != nullptr) row_store8<T, VEC>((T*)p.ddt + b * p.ddt_bs + t * p.ddt_ld + tc, tn, o);
-        if (p.dz != nullptr) {
+            for (int j = 0; j < 8; ++j) o[j] = fmaf(skip[j], dp_of<T, VEC>(p, cy[i], cz[i], j), x[j][0] * x[j][1]);
+            row_store8<T, VEC>((T*)p.du + b * p.du_bs + t * p.du_ld + tc, tn, o);
+          }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float s = sigmoid_f(z[j]);
-            o[j] = t < len ? dout[j] * fmaf(skip[j], u[j], x[j][3]) * s * (1.f + z[j] * (1.f - s)) : 0.f;
+            o[j] = fmaf(x[j][1], cu[i][j], x[j][2]);
+            if (p.softplus) o[j] *= sigmoid_f(ct[i][j] + bias[j]);
+            accB[j] += o[j];
+            accD[j] = fmaf(dp_of<T, VEC>(p, cy[i], cz[i], j), cu[i][j], accD[j]);
           }
-          row_store8<T, VEC>((T*)p.dz + b * p.dz_bs + t * p.dz_ld + tc, tn, o);
+          if (p.ddt != nullptr) row_store8<T, VEC>((T*)p.ddt + b * p.ddt_bs + t * p.ddt_ld + tc, tn, o);
+          if (p.dz != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float z = cz[i][j], sg = sigmoid_f(z);
+              o[j] = cy[i][j] * fmaf(skip[j], cu[i][j], x[j][3]) * sg * (1.f + z * (1.f - sg));
+            }
+            row_store8<T, VEC>((T*)p.dz + b * p.dz_bs + t * p.dz_ld + tc, tn, o);
+          }
         }
       }
     }
@@ -446,9 +574,9 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_bwd_kernel(const seg_scan_arg
   if (live && pA != nullptr) store_states(pA + (o * p.D + d) * p.S, 4 * g, p.S, dA);
   if (live && p.dstate != nullptr && chunk == 0) store_states(p.dstate + ((int64_t)b * p.D + d) * p.S, 4 * g, p.S, q);
   if (pD != nullptr) {
-    // the threads of a channel piece: NT / CHUNKS rows of CB values, added by the block's first CB threads, dD and then ddt_bias
+    // the threads of a channel piece: ROWS rows of CB values, added by the block's first CB threads, dD and then ddt_bias
     float* sh = reinterpret_cast<float*>(&sx[0][0]);
-    constexpr int R = Y::NT / Y::CHUNKS;
+    constexpr int R = Y::ROWS;
     static_assert(R * Y::CB * 4 <= (int)sizeof(sx), "the rows fit the tile's LDS");
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -521,12 +649,16 @@ inline int scan_group(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 16 ? 4 : S 
 inline int scan_cb(int S) { const int G = scan_group(S); return G <= 4 ? 64 : 256 / G; }
 
 struct ScanPlan { int nblk, nch, clen; };
-inline ScanPlan scan_plan(const seg_scan_args& a) {
+inline ScanPlan scan_plan(const seg_scan_args& a, bool bwd) {
   ScanPlan s;
   const int cb = scan_cb(a.S);
   s.nblk = (a.D + cb - 1) / cb;
   const int64_t blocks = (int64_t)s.nblk * a.B;
-  int64_t nch = blocks >= 512 ? 1 : (1024 + blocks - 1) / (blocks < 1 ? 1 : blocks);
+  // chunks until this many blocks are there.  Forward: 256 / 512 / 1024 / 2048 blocks took 353 / 313 / 273 / 255 us (8 prompts of up to
+  // 2048 rows, 2048 channels, 16 states, bf16: short sequences leave early, many blocks level that); backward: a block keeps two waves
+  // per SIMD busy at most, and every chunk adds partial rows of dA - 256 / 512 / 1024: 423 / 326 / 325 us (8 x 1024 x 1024 x 16, f16)
+  const int64_t want = bwd ? 512 : 2048;
+  int64_t nch = (want + blocks - 1) / (blocks < 1 ? 1 : blocks);
   const int64_t most = (a.L + 63) / 64;
   if (nch > most) nch = most;
   if (nch < 1) nch = 1;
@@ -599,13 +731,13 @@ extern "C" int64_t seg_selective_scan_saved_bytes(const seg_scan_args* a) {
 }
 extern "C" int64_t seg_selective_scan_fwd_workspace_bytes(const seg_scan_args* a) {
   if (a == nullptr || a->B <= 0 || a->L <= 0 || a->D <= 0 || a->S <= 0) return 0;
-  const ScanPlan s = scan_plan(*a);
+  const ScanPlan s = scan_plan(*a, false);
   if (s.nch <= 1) return 0;
   return ((int64_t)a->B * s.nch * a->D * a->S + 3) / 4 * 16 + (int64_t)a->B * s.nch * a->D * 4;
 }
 extern "C" int64_t seg_selective_scan_bwd_workspace_bytes(const seg_scan_args* a) {
   if (a == nullptr || a->B <= 0 || a->L <= 0 || a->D <= 0 || a->S <= 0) return 0;
-  return scan_bwd_space(*a, scan_plan(*a)).total * 4;
+  return scan_bwd_space(*a, scan_plan(*a, true)).total * 4;
 }
 
 extern "C" int seg_selective_scan_fwd(const seg_scan_args* a, seg_stream_t stream) {
@@ -614,7 +746,7 @@ extern "C" int seg_selective_scan_fwd(const seg_scan_args* a, seg_stream_t strea
   SEG_CHECK_ARG(scan_rows_ok(*a) && (a->L <= 1 || a->y_ld >= a->D), "selective_scan_fwd: row strides below the channels / states");
   SEG_CHECK_ARG(a->state_out == nullptr || a->state_out != a->state, "selective_scan_fwd: state_out may not be state");
   if (a->B == 0 || (a->L == 0 && a->state_out == nullptr)) return SEG_OK;
-  const ScanPlan s = scan_plan(*a);
+  const ScanPlan s = scan_plan(*a, false);
   SEG_CHECK_ARG(s.nch <= 1 || a->workspace != nullptr, "selective_scan_fwd: workspace is NULL (%lld bytes are needed)", (long long)seg_selective_scan_fwd_workspace_bytes(a));
   hipStream_t st = (hipStream_t)stream;
   float* start = s.nch > 1 ? (float*)a->workspace : nullptr;
@@ -625,13 +757,14 @@ extern "C" int seg_selective_scan_fwd(const seg_scan_args* a, seg_stream_t strea
     typedef typename std::remove_pointer<decltype(tp)>::type T;
     constexpr int G = Gc(), NT = Lay<G>::NT;
     if (s.nch > 1) {
-      if (vec) hipLaunchKernelGGL((scan_fwd_kernel<T, true, G, false>), grid, dim3(NT), 0, st, *a, s.clen, start, sumd);
-      else hipLaunchKernelGGL((scan_fwd_kernel<T, false, G, false>), grid, dim3(NT), 0, st, *a, s.clen, start, sumd);
+      const dim3 front((unsigned)s.nblk, (unsigned)s.nch - 1, (unsigned)a->B);           // (the last chunk's own last state starts nothing)
+      if (vec) hipLaunchKernelGGL((scan_fwd_kernel<T, true, G, false>), front, dim3(NT), 0, st, *a, s.clen, s.nch, start, sumd);
+      else hipLaunchKernelGGL((scan_fwd_kernel<T, false, G, false>), front, dim3(NT), 0, st, *a, s.clen, s.nch, start, sumd);
       const int64_t n = (int64_t)a->D * a->S;
       hipLaunchKernelGGL(scan_join_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)a->B), dim3(256), 0, st, *a, s.nch, start, sumd);
     }
-    if (vec) hipLaunchKernelGGL((scan_fwd_kernel<T, true, G, true>), grid, dim3(NT), 0, st, *a, s.clen, start, sumd);
-    else hipLaunchKernelGGL((scan_fwd_kernel<T, false, G, true>), grid, dim3(NT), 0, st, *a, s.clen, start, sumd);
+    if (vec) hipLaunchKernelGGL((scan_fwd_kernel<T, true, G, true>), grid, dim3(NT), 0, st, *a, s.clen, s.nch, start, sumd);
+    else hipLaunchKernelGGL((scan_fwd_kernel<T, false, G, true>), grid, dim3(NT), 0, st, *a, s.clen, s.nch, start, sumd);
   });
   SEG_CHECK_LAUNCH("selective_scan_fwd");
   return SEG_OK;
@@ -648,7 +781,7 @@ extern "C" int seg_selective_scan_bwd(const seg_scan_args* a, seg_stream_t strea
   SEG_CHECK_ARG(a->dz == nullptr || a->z != nullptr, "selective_scan_bwd: dz without z");
   SEG_CHECK_ARG(none || a->workspace != nullptr, "selective_scan_bwd: workspace is NULL (%lld bytes are needed)", (long long)seg_selective_scan_bwd_workspace_bytes(a));
   hipStream_t st = (hipStream_t)stream;
-  const ScanPlan s = scan_plan(*a);
+  const ScanPlan s = scan_plan(*a, true);
   const ScanBwdSpace w = scan_bwd_space(*a, s);
   float* ws = (float*)a->workspace;
   const int64_t n = (int64_t)a->D * a->S;
@@ -661,8 +794,9 @@ extern "C" int seg_selective_scan_bwd(const seg_scan_args* a, seg_stream_t strea
       typedef typename std::remove_pointer<decltype(tp)>::type T;
       constexpr int G = Gc(), NT = Lay<G>::NT;
       if (s.nch > 1) {
-        if (vec) hipLaunchKernelGGL((scan_bwd_local_kernel<T, true, G>), grid, dim3(NT), 0, st, *a, s.clen, adj, sumd);
-        else hipLaunchKernelGGL((scan_bwd_local_kernel<T, false, G>), grid, dim3(NT), 0, st, *a, s.clen, adj, sumd);
+        const dim3 back((unsigned)s.nblk, (unsigned)s.nch - 1, (unsigned)a->B);          // (nothing lies in front of the first chunk)
+        if (vec) hipLaunchKernelGGL((scan_bwd_local_kernel<T, true, G>), back, dim3(NT), 0, st, *a, s.clen, s.nch, adj, sumd);
+        else hipLaunchKernelGGL((scan_bwd_local_kernel<T, false, G>), back, dim3(NT), 0, st, *a, s.clen, s.nch, adj, sumd);
         hipLaunchKernelGGL(scan_join_bwd_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)a->B), dim3(256), 0, st, *a, s.nch, adj, sumd);
       }
       float *pbc = bc && !none ? ws + w.pbc : nullptr, *pA = a->dA != nullptr && !none ? ws + w.pA : nullptr, *pD = pd && !none ? ws + w.pD : nullptr;

@@ -20,7 +20,7 @@ import torch
 
 from . import _ffi
 from ._ffi import SEQ_ACT, CausalConvArgs, LinearArgs, ScanArgs
-from .ops import call
+from .ops import KernelProfile, _DryRun, call
 
 __all__ = ["layer_norm", "layer_norm_backward", "linear", "linear_backward", "activation_backward", "causal_conv", "causal_conv_backward",
            "causal_conv_step", "selective_scan", "selective_scan_backward", "selective_scan_step", "ScanGrads"]
@@ -30,69 +30,81 @@ MAX_TAPS, MAX_STATES = 8, 64
 
 
 # ----------------------------------------------------------------------------------------------------------------- checks
+# Small calls are bound by the host: the checks look at what is right first (a few attribute reads) and find out what is wrong after.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_fns = {}
+
+
 def _fail(what, msg):
     raise ValueError(f"{what}: {msg}")
 
 
 def _dtype(what, x):
+    try:
+        return _DT[x.dtype]
+    except (AttributeError, KeyError):
+        pass
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: a torch tensor is needed, got {type(x).__name__}")
-    dt = _DT.get(x.dtype)
-    if dt is None:
-        _fail(what, f"elements must be float16, bfloat16 or float32, got {x.dtype}")
-    return dt
+    _fail(what, f"elements must be float16, bfloat16 or float32, got {x.dtype}")
+
+
+def _wrong(what, name, t, ref, dtype, shape):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: {name} must be a torch tensor, got {type(t).__name__}")
+    if t.dtype != dtype or t.device != ref.device:
+        _fail(what, f"{name} is {t.dtype} on {t.device}, expected {dtype} on {ref.device}")
+    if t.shape != shape:
+        _fail(what, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _like(what, name, t, ref, shape):
     """t: elements like ref's, of this shape, channels contiguous."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{what}: {name} must be a torch tensor, got {type(t).__name__}")
-    if t.dtype != ref.dtype or t.device != ref.device:
-        _fail(what, f"{name} is {t.dtype} on {t.device}, expected {ref.dtype} on {ref.device}")
-    if tuple(t.shape) != tuple(shape):
-        _fail(what, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        _fail(what, f"{name}: the channel axis must be contiguous (strides {t.stride()})")
-    return t
+    try:
+        if t.dtype is ref.dtype and t.shape == shape and t.get_device() == ref.get_device() and (t.stride(-1) == 1 or shape[-1] == 1):
+            return t
+    except AttributeError:
+        pass
+    _wrong(what, name, t, ref, ref.dtype, shape)
+    _fail(what, f"{name}: the channel axis must be contiguous (strides {t.stride()})")
 
 
 def _param(what, name, t, ref, shape, dtype=torch.float32):
     """t: a dense tensor of parameters or states (None passes)."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{what}: {name} must be a torch tensor, got {type(t).__name__}")
-    if t.dtype != dtype or t.device != ref.device:
-        _fail(what, f"{name} is {t.dtype} on {t.device}, expected {dtype} on {ref.device}")
-    if tuple(t.shape) != tuple(shape):
-        _fail(what, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if not t.is_contiguous():
-        _fail(what, f"{name} must be contiguous (strides {t.stride()})")
-    return t
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == ref.get_device() and t.is_contiguous():
+            return t
+    except AttributeError:
+        pass
+    _wrong(what, name, t, ref, dtype, shape)
+    _fail(what, f"{name} must be contiguous (strides {t.stride()})")
 
 
 def _rows(what, name, t):
     """(rows, row stride) of [..., C] whose leading axes collapse into one."""
-    C_ = t.shape[-1]
-    if C_ > 1 and t.stride(-1) != 1:
-        _fail(what, f"{name}: the channel axis must be contiguous (strides {t.stride()})")
-    rows, ld = 1, C_
-    first = True
-    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        if size != 1:
-            if first:
-                ld, first = stride, False
-            elif stride != ld * rows:
-                _fail(what, f"{name}: leading axes of strides {t.stride()} and sizes {tuple(t.shape)} are not evenly spaced rows; call .contiguous()")
-            rows *= size
-    if rows > 1 and ld < C_:
-        _fail(what, f"{name}: rows overlap (strides {t.stride()}); call .contiguous()")
+    shape, strides = t.shape, t.stride()
+    c = shape[-1]
+    if c > 1 and strides[-1] != 1:
+        _fail(what, f"{name}: the channel axis must be contiguous (strides {strides})")
+    if len(shape) == 2:
+        rows, ld = shape[0], strides[0]
+    else:
+        rows, ld, first = 1, c, True
+        for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+            if size != 1:
+                if first:
+                    ld, first = stride, False
+                elif stride != ld * rows:
+                    _fail(what, f"{name}: leading axes of strides {strides} and sizes {tuple(shape)} are not evenly spaced rows; call .contiguous()")
+                rows *= size
+    if rows > 1:
+        if ld < c:
+            _fail(what, f"{name}: rows overlap (strides {strides}); call .contiguous()")
+    else:
+        ld = c
     return rows, ld
-
-
-def _bl(t, L):
-    """(batch stride, row stride) of [B, L, C]."""
-    return t.stride(0), t.stride(1)
 
 
 def _spaced(what, name, t):
@@ -112,16 +124,25 @@ def _ptr(t):
 
 
 def _gpu(what, t):
-    if not t.is_cuda:
+    """The index of t's device."""
+    i = t.get_device()
+    if i < 0:
         raise RuntimeError(f"{what}: the tensors are on {t.device}; the operators run on an MI355X only - there is no CPU fallback")
+    return i
 
 
-def _launch(dev, name, *args):
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+def _launch(i, name, *args):
+    """Enqueue on device i's current stream."""
+    if _DryRun.on or KernelProfile.on or _raw_stream is None or i != torch.cuda.current_device():
+        with torch.cuda.device(i):
             call(name, *args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
-    else:
-        call(name, *args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        return
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_ffi.lib(), name)
+    rc = fn(*args, _raw_stream(i))
+    if rc != 0:
+        _ffi.check(rc, name)
 
 
 def _bytes(n, dev):
@@ -150,12 +171,12 @@ def layer_norm(x, gamma=None, beta=None, eps: float = 1e-3, stats: bool = False)
     _param(what, "beta", beta, x, (c,))
     rows, ld = _rows(what, "x", x)
     _no_grad(what, x, gamma, beta)
-    _gpu(what, x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    di = _gpu(what, x)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
     if stats:
         mean, rstd = torch.empty((2,) + tuple(x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
-    _launch(x.device, "seg_layernorm_fwd", _ptr(x), ld, _ptr(y), c, rows, c, dt, _ptr(gamma), _ptr(beta), eps, _ptr(mean), _ptr(rstd))
+    _launch(di, "seg_layernorm_fwd", _ptr(x), ld, _ptr(y), c, rows, c, dt, _ptr(gamma), _ptr(beta), eps, _ptr(mean), _ptr(rstd))
     return (y, mean, rstd) if stats else y
 
 
@@ -175,12 +196,12 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None) -> Tuple[torch.Tensor, to
     rows, ld = _rows(what, "x", x)
     _r, dy_ld = _rows(what, "dy", dy)
     _no_grad(what, dy, x, mean, rstd, gamma)
-    _gpu(what, x)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    di = _gpu(what, x)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     par = torch.empty((2, c), dtype=torch.float32, device=x.device)
     ws = _bytes(_ffi.lib().seg_layernorm_bwd_workspace_bytes(rows, c, dt), x.device)
     p = par.data_ptr()
-    _launch(x.device, "seg_layernorm_bwd", _ptr(dy), dy_ld, _ptr(x), ld, _ptr(dx), c, rows, c, dt, _ptr(mean), _ptr(rstd), _ptr(gamma), p, p + 4 * c, _ptr(ws))
+    _launch(di, "seg_layernorm_bwd", _ptr(dy), dy_ld, _ptr(x), ld, _ptr(dx), c, rows, c, dt, _ptr(mean), _ptr(rstd), _ptr(gamma), p, p + 4 * c, _ptr(ws))
     return dx, par[0], par[1]
 
 
@@ -208,19 +229,19 @@ def linear(x, w, bias=None, activation: Optional[str] = None, alpha: float = 0.3
         _fail(what, f"x has {x.shape[-1]} inputs, w {k}")
     _param(what, "bias", bias, x, (n,))
     m, x_ld = _rows(what, "x", x)
-    shape = tuple(x.shape[:-1]) + (n,)
+    shape = x.shape[:-1] + (n,)
     r_ld = 0
     if residual is not None:
         _like(what, "residual", residual, x, shape)
         _r, r_ld = _rows(what, "residual", residual)
     _no_grad(what, x, w, bias, residual)
-    _gpu(what, x)
+    di = _gpu(what, x)
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     z = torch.empty(shape, dtype=x.dtype, device=x.device) if preactivation else None
     a = LinearArgs(m, n, k, dt, act, alpha, _ptr(x), x_ld, _ptr(w), w_ld, _ptr(bias), _ptr(residual), r_ld, _ptr(z), n, _ptr(y), n)
     ws = _bytes(_ffi.lib().seg_linear_workspace_bytes(a, _ffi.LINEAR_FWD), x.device)
     a.workspace = _ptr(ws)
-    _launch(x.device, "seg_linear_fwd", a)
+    _launch(di, "seg_linear_fwd", a)
     return (y, z) if preactivation else y
 
 
@@ -236,7 +257,7 @@ def linear_backward(dy, x, w, z=None, activation: Optional[str] = None, alpha: f
     n, k = w.shape
     if x.shape[-1] != k:
         _fail(what, f"x has {x.shape[-1]} inputs, w {k}")
-    _like(what, "dy", dy, x, tuple(x.shape[:-1]) + (n,))
+    _like(what, "dy", dy, x, x.shape[:-1] + (n,))
     m, x_ld = _rows(what, "x", x)
     _m, dy_ld = _rows(what, "dy", dy)
     if act != 0 and z is None and need_dx:
@@ -249,22 +270,22 @@ def linear_backward(dy, x, w, z=None, activation: Optional[str] = None, alpha: f
         _like(what, "residual", residual, x, x.shape)
         _m, r_ld = _rows(what, "residual", residual)
     _no_grad(what, dy, x, w, z, residual)
-    _gpu(what, x)
+    di = _gpu(what, x)
     dev, lib = x.device, _ffi.lib()
     dx = dw = db = None
     if need_dx:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
         a = LinearArgs(m, k, n, dt, act, alpha, _ptr(dy), dy_ld, _ptr(w), w_ld, None, _ptr(residual), r_ld, _ptr(z) if act != 0 else None, z_ld, _ptr(dx), k)
         ws = _bytes(lib.seg_linear_workspace_bytes(a, _ffi.LINEAR_BWD_DATA), dev)
         a.workspace = _ptr(ws)
-        _launch(dev, "seg_linear_bwd_data", a)
+        _launch(di, "seg_linear_bwd_data", a)
     if need_dw or need_db:
         dw = torch.empty((n, k), dtype=torch.float32, device=dev) if need_dw else None
         db = torch.empty((n,), dtype=torch.float32, device=dev) if need_db else None
         a = LinearArgs(m, n, k, dt, 0, 0.0, _ptr(x), x_ld, None, 0, None, None, 0, None, 0, None, 0, _ptr(dy), dy_ld, _ptr(dw), k, _ptr(db))
         ws = _bytes(lib.seg_linear_workspace_bytes(a, _ffi.LINEAR_BWD_WEIGHT), dev)
         a.workspace = _ptr(ws)
-        _launch(dev, "seg_linear_bwd_weight", a)
+        _launch(di, "seg_linear_bwd_weight", a)
     return dx, dw, db
 
 
@@ -278,10 +299,10 @@ def activation_backward(dy, z, activation: str, alpha: float = 0.3):
     rows, z_ld = _rows(what, "z", z)
     _r, dy_ld = _rows(what, "dy", dy)
     _no_grad(what, dy, z)
-    _gpu(what, z)
+    di = _gpu(what, z)
     c = z.shape[-1]
-    dx = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    _launch(z.device, "seg_linear_act_bwd", _ptr(dy), dy_ld, _ptr(z), z_ld, _ptr(dx), c, rows, c, dt, act, alpha)
+    dx = torch.empty_like(z, memory_format=torch.contiguous_format)
+    _launch(di, "seg_linear_act_bwd", _ptr(dy), dy_ld, _ptr(z), z_ld, _ptr(dx), c, rows, c, dt, act, alpha)
     return dx
 
 
@@ -319,11 +340,11 @@ def causal_conv(x, w, bias=None, activation: Optional[str] = None, state=None, l
     _spaced(what, "x", x)
     _lengths(what, lengths, x, B)
     _no_grad(what, x, w, bias, state)
-    _gpu(what, x)
+    di = _gpu(what, x)
     y = torch.empty((B, L, d), dtype=x.dtype, device=x.device)
     new = torch.empty((B, K - 1, d), dtype=x.dtype, device=x.device)
-    a = CausalConvArgs(B, L, d, K, dt, act, _ptr(x), *_bl(x, L), _ptr(w), _ptr(bias), _ptr(state), _ptr(lengths), _ptr(y), L * d, d, _ptr(new))
-    _launch(x.device, "seg_causal_conv_fwd", a)
+    a = CausalConvArgs(B, L, d, K, dt, act, _ptr(x), x.stride(0), x.stride(1), _ptr(w), _ptr(bias), _ptr(state), _ptr(lengths), _ptr(y), L * d, d, _ptr(new))
+    _launch(di, "seg_causal_conv_fwd", a)
     return y, new
 
 
@@ -339,17 +360,17 @@ def causal_conv_backward(dy, x, w, bias=None, activation: Optional[str] = None, 
     _lengths(what, lengths, x, B)
     _param(what, "dstate", dstate, x, (B, K - 1, d), x.dtype)
     _no_grad(what, dy, x, w, bias, state, dstate)
-    _gpu(what, x)
+    di = _gpu(what, x)
     dev = x.device
     dx = torch.empty((B, L, d), dtype=x.dtype, device=dev)
     dw = torch.empty((K, d), dtype=torch.float32, device=dev)
     db = torch.empty((d,), dtype=torch.float32, device=dev) if bias is not None else None
     dst = torch.empty((B, K - 1, d), dtype=x.dtype, device=dev) if state is not None else None
-    a = CausalConvArgs(B, L, d, K, dt, act, _ptr(x), *_bl(x, L), _ptr(w), _ptr(bias), _ptr(state), _ptr(lengths), None, 0, 0, None,
-                       _ptr(dy), *_bl(dy, L), _ptr(dstate), _ptr(dx), L * d, d, _ptr(dw), _ptr(db), _ptr(dst))
+    a = CausalConvArgs(B, L, d, K, dt, act, _ptr(x), x.stride(0), x.stride(1), _ptr(w), _ptr(bias), _ptr(state), _ptr(lengths), None, 0, 0, None,
+                       _ptr(dy), dy.stride(0), dy.stride(1), _ptr(dstate), _ptr(dx), L * d, d, _ptr(dw), _ptr(db), _ptr(dst))
     ws = _bytes(_ffi.lib().seg_causal_conv_bwd_workspace_bytes(a), dev)
     a.workspace = _ptr(ws)
-    _launch(dev, "seg_causal_conv_bwd", a)
+    _launch(di, "seg_causal_conv_bwd", a)
     return dx, dw, db, dst
 
 
@@ -357,10 +378,9 @@ def _new_state(what, state, new_state):
     if new_state is None:
         return state
     _param(what, "new_state", new_state, state, state.shape, state.dtype)
-    if new_state.data_ptr() != state.data_ptr():
-        lo, hi = sorted((state, new_state), key=lambda t: t.data_ptr())
-        if lo.data_ptr() + lo.numel() * lo.element_size() > hi.data_ptr() and lo.numel():
-            _fail(what, "new_state overlaps state: give the same tensor or another one")
+    a, b = state.data_ptr(), new_state.data_ptr()
+    if a != b and abs(a - b) < state.numel() * state.element_size():
+        _fail(what, "new_state overlaps state: give the same tensor or another one")
     return new_state
 
 
@@ -374,10 +394,10 @@ def causal_conv_step(x, state, w, bias=None, activation: Optional[str] = None, n
     if B > 1 and x.stride(0) < d:
         _fail(what, f"x: rows overlap (strides {x.stride()}); call .contiguous()")
     _no_grad(what, x, w, bias, state)
-    _gpu(what, x)
-    y = torch.empty((B, d), dtype=x.dtype, device=x.device)
+    di = _gpu(what, x)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     a = CausalConvArgs(B, 1, d, K, dt, act, _ptr(x), x.stride(0), d, _ptr(w), _ptr(bias), _ptr(state), None, _ptr(y), d, d, _ptr(new))
-    _launch(x.device, "seg_causal_conv_step", a)
+    _launch(di, "seg_causal_conv_step", a)
     return y
 
 
@@ -396,36 +416,36 @@ class ScanGrads(NamedTuple):
 
 
 def _scan_common(what, u, dt, A, B, C_, D, z, dt_bias, rank):
+    """Checks what every scan call has; (type code, batch, channels, states, [strides of u, dt, z, B, C])."""
     dtc = _dtype(what, u)
-    if u.dim() != rank or u.shape[-1] < 1:
-        _fail(what, f"u has shape {tuple(u.shape)}, expected " + ("[B, L, D]" if rank == 3 else "[B, D]"))
+    shape = u.shape
+    if len(shape) != rank or shape[-1] < 1:
+        _fail(what, f"u has shape {tuple(shape)}, expected " + ("[B, L, D]" if rank == 3 else "[B, D]"))
     if not isinstance(A, torch.Tensor) or A.dim() != 2:
         _fail(what, "A must be [D, S]")
-    d, S = u.shape[-1], A.shape[1]
+    d, S, nb = shape[-1], A.shape[1], shape[0]
     if not 1 <= S <= MAX_STATES:
         _fail(what, f"{S} states per channel (1 .. {MAX_STATES})")
-    if d > 1 and u.stride(-1) != 1:
-        _fail(what, f"u: the channel axis must be contiguous (strides {u.stride()})")
     _param(what, "A", A, u, (d, S))
-    _like(what, "dt", dt, u, u.shape)
-    _like(what, "B", B, u, tuple(u.shape[:-1]) + (S,))
-    _like(what, "C", C_, u, tuple(u.shape[:-1]) + (S,))
-    if z is not None:
-        _like(what, "z", z, u, u.shape)
+    bc = (nb, shape[1], S) if rank == 3 else (nb, S)
+    strides = []
+    for n, t, sh in (("u", u, shape), ("dt", dt, shape), ("z", z, shape), ("B", B, bc), ("C", C_, bc)):
+        if t is None and n == "z":
+            strides.append((0,) * rank)
+            continue
+        if t is not u:
+            _like(what, n, t, u, sh)
+        st = t.stride()
+        if t is u and st[-1] != 1 and d > 1:
+            _fail(what, f"u: the channel axis must be contiguous (strides {st})")
+        if sh[-2] > 1 and st[-2] < sh[-1]:
+            _fail(what, f"{n}: rows overlap (strides {st}); call .contiguous()")
+        strides.append(st)
     _param(what, "D", D, u, (d,))
     _param(what, "dt_bias", dt_bias, u, (d,))
-    if rank == 3:
-        for n, t in (("u", u), ("dt", dt), ("B", B), ("C", C_), ("z", z)):
-            if t is not None:
-                _spaced(what, n, t)
-    else:
-        for n, t in (("u", u), ("dt", dt), ("B", B), ("C", C_), ("z", z)):
-            if t is not None and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-                _fail(what, f"{n}: rows overlap (strides {t.stride()}); call .contiguous()")
-    for n, t in (("A", A),):
-        if t.data_ptr() % 16:
-            _fail(what, f"{n} must be 16-byte aligned")
-    return dtc, u.shape[0], d, S
+    if A.data_ptr() % 16:
+        _fail(what, "A must be 16-byte aligned")
+    return dtc, nb, d, S, strides
 
 
 def _aligned(what, **ts):
@@ -434,13 +454,10 @@ def _aligned(what, **ts):
             _fail(what, f"{n} must be 16-byte aligned")
 
 
-def _st(t):
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
-
-
-def _scan_args(B, L, d, S, dtc, softplus, u, dt, z, Bm, Cm, A, D, dt_bias, state, lengths):
-    return ScanArgs(B, L, d, S, dtc, 1 if softplus else 0, *_st(u), *_st(dt), *_st(z), *_st(Bm), *_st(Cm), _ptr(A), _ptr(D), _ptr(dt_bias), _ptr(state),
-                    _ptr(lengths))
+def _scan_args(B, L, d, S, dtc, softplus, u, dt, z, Bm, Cm, A, D, dt_bias, state, lengths, st):
+    (ub, ul, _), (tb, tl, _), (zb, zl, _), (bb, bl, _), (cb, cl, _) = st
+    return ScanArgs(B, L, d, S, dtc, 1 if softplus else 0, u.data_ptr(), ub, ul, dt.data_ptr(), tb, tl, _ptr(z), zb, zl, Bm.data_ptr(), bb, bl,
+                    Cm.data_ptr(), cb, cl, A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(state), _ptr(lengths))
 
 
 def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus: bool = True, state=None, lengths=None, training: bool = False):
@@ -450,17 +467,17 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus: bool 
     the first row (None: zeros); lengths int32 [B]: rows behind a length are not read, their y is 0 and the state stays what it was.
     Returns (y, last state), with training=True (y, last state, saved) - `saved` is what selective_scan_backward needs."""
     what = "selective_scan"
-    dtc, nb, d, S = _scan_common(what, u, dt, A, B, C, D, z, dt_bias, 3)
+    dtc, nb, d, S, st = _scan_common(what, u, dt, A, B, C, D, z, dt_bias, 3)
     L = u.shape[1]
     _param(what, "state", state, u, (nb, d, S))
     _aligned(what, state=state)
     _lengths(what, lengths, u, nb)
     _no_grad(what, u, dt, A, B, C, D, z, dt_bias, state)
-    _gpu(what, u)
+    di = _gpu(what, u)
     dev, lib = u.device, _ffi.lib()
     y = torch.empty((nb, L, d), dtype=u.dtype, device=dev)
     last = torch.empty((nb, d, S), dtype=torch.float32, device=dev)
-    a = _scan_args(nb, L, d, S, dtc, softplus, u, dt, z, B, C, A, D, dt_bias, state, lengths)
+    a = _scan_args(nb, L, d, S, dtc, softplus, u, dt, z, B, C, A, D, dt_bias, state, lengths, st)
     a.y, a.y_bs, a.y_ld, a.state_out = _ptr(y), L * d, d, _ptr(last)
     saved = None
     if training:
@@ -468,7 +485,7 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus: bool 
         a.saved = _ptr(saved)
     ws = _bytes(lib.seg_selective_scan_fwd_workspace_bytes(a), dev)
     a.workspace = _ptr(ws)
-    _launch(dev, "seg_selective_scan_fwd", a)
+    _launch(di, "seg_selective_scan_fwd", a)
     return (y, last, saved) if training else (y, last)
 
 
@@ -476,7 +493,7 @@ def selective_scan_backward(dy, u, dt, A, B, C, saved, D=None, z=None, dt_bias=N
     """All gradients of selective_scan(..., training=True) from dy and dstate, the gradient of the last state (None: zeros); the other
     operands as in the forward call.  Rows behind a length: dy is not read, their gradients are 0."""
     what = "selective_scan_backward"
-    dtc, nb, d, S = _scan_common(what, u, dt, A, B, C, D, z, dt_bias, 3)
+    dtc, nb, d, S, st = _scan_common(what, u, dt, A, B, C, D, z, dt_bias, 3)
     L = u.shape[1]
     _like(what, "dy", dy, u, u.shape)
     _spaced(what, "dy", dy)
@@ -486,10 +503,10 @@ def selective_scan_backward(dy, u, dt, A, B, C, saved, D=None, z=None, dt_bias=N
     if saved is None:
         _fail(what, "saved is needed (selective_scan(..., training=True) returns it)")
     lib = _ffi.lib()
-    a = _scan_args(nb, L, d, S, dtc, softplus, u, dt, z, B, C, A, D, dt_bias, None, lengths)
+    a = _scan_args(nb, L, d, S, dtc, softplus, u, dt, z, B, C, A, D, dt_bias, None, lengths, st)
     _param(what, "saved", saved, u, (lib.seg_selective_scan_saved_bytes(a) // 4,))
     _no_grad(what, dy, u, dt, A, B, C, D, z, dt_bias, dstate)
-    _gpu(what, u)
+    di = _gpu(what, u)
     dev = u.device
 
     def rows(c):
@@ -509,7 +526,7 @@ def selective_scan_backward(dy, u, dt, A, B, C, saved, D=None, z=None, dt_bias=N
     a.dA, a.dD, a.ddt_bias, a.dstate = _ptr(g.dA), _ptr(g.dD), _ptr(g.ddt_bias), _ptr(g.dstate)
     ws = _bytes(lib.seg_selective_scan_bwd_workspace_bytes(a), dev)
     a.workspace = _ptr(ws)
-    _launch(dev, "seg_selective_scan_bwd", a)
+    _launch(di, "seg_selective_scan_bwd", a)
     return g
 
 
@@ -517,17 +534,17 @@ def selective_scan_step(u, dt, A, B, C, state, D=None, z=None, dt_bias=None, sof
     """One more row per sequence: u, dt, z [B, D], B, C [B, S] -> y [B, D].  state fp32 [B, D, S] is updated in place, or written to
     new_state."""
     what = "selective_scan_step"
-    dtc, nb, d, S = _scan_common(what, u, dt, A, B, C, D, z, dt_bias, 2)
+    dtc, nb, d, S, st = _scan_common(what, u, dt, A, B, C, D, z, dt_bias, 2)
     if state is None:
         _fail(what, "state is needed")
     _param(what, "state", state, u, (nb, d, S))
     new = _new_state(what, state, new_state)
-    _aligned(what, state=state, new_state=new)
+    if state.data_ptr() % 16 or new.data_ptr() % 16:
+        _fail(what, "state must be 16-byte aligned")
     _no_grad(what, u, dt, A, B, C, D, z, dt_bias, state)
-    _gpu(what, u)
-    y = torch.empty((nb, d), dtype=u.dtype, device=u.device)
-    st = [(None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), 0) for t in (u, dt, z, B, C)]
-    a = ScanArgs(nb, 1, d, S, dtc, 1 if softplus else 0, *st[0], *st[1], *st[2], *st[3], *st[4], _ptr(A), _ptr(D), _ptr(dt_bias), _ptr(state), None,
-                 _ptr(y), d, d, _ptr(new))
-    _launch(u.device, "seg_selective_scan_step", a)
+    di = _gpu(what, u)
+    y = torch.empty_like(u, memory_format=torch.contiguous_format)
+    a = ScanArgs(nb, 1, d, S, dtc, 1 if softplus else 0, u.data_ptr(), st[0][0], 0, dt.data_ptr(), st[1][0], 0, _ptr(z), st[2][0], 0, B.data_ptr(), st[3][0], 0,
+                 C.data_ptr(), st[4][0], 0, A.data_ptr(), _ptr(D), _ptr(dt_bias), state.data_ptr(), None, y.data_ptr(), d, d, new.data_ptr())
+    _launch(di, "seg_selective_scan_step", a)
     return y
