@@ -9,19 +9,31 @@
 
 namespace {
 
-constexpr int RUN = 16;          // rows per thread
+constexpr int RUN = 16, RUN_SMALL = 8;          // rows per thread, forward / backward and small grids
 constexpr int MAXK = 8;
 
 struct ConvDims { int B, L, D, act; };
 
+// eight channels of a row in their memory format; n <= 0: zeros
+template <typename T, bool VEC> struct Raw {
+  typedef T tv __attribute__((ext_vector_type(8)));
+  tv v;
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if constexpr (VEC) {
+      v = tv{};
+      if (n > 0) v = *reinterpret_cast<const tv*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ float operator[](int j) const { return (float)v[j]; }
+};
 // rows of xx = [state; x]: r < 0 is state row K - 1 + r.  x rows at or behind the length are not read
 template <typename T, bool VEC, int K>
-__device__ __forceinline__ void load_xx(const seg_causal_conv_args& p, int b, int r, int len, int c, float* f) {
-  if (r >= 0) {
-    row_load8<T, VEC>((const T*)p.x + b * p.x_bs + r * p.x_ld + c, r < len ? p.D - c : 0, f);
-  } else {
-    row_load8<T, VEC>((const T*)p.state + ((int64_t)b * (K - 1) + K - 1 + r) * p.D + c, p.state != nullptr ? p.D - c : 0, f);
-  }
+__device__ __forceinline__ void load_xx(const seg_causal_conv_args& p, int b, int r, int len, int c, Raw<T, VEC>& f) {
+  if (r >= 0) f.load((const T*)p.x + b * p.x_bs + r * p.x_ld + c, r < len ? p.D - c : 0);
+  else f.load((const T*)p.state + ((int64_t)b * (K - 1) + K - 1 + r) * p.D + c, p.state != nullptr ? p.D - c : 0);
 }
 template <bool VEC> __device__ __forceinline__ void load_par(const float* p, int n, float* f) {
   if (p == nullptr) n = 0;
@@ -34,46 +46,46 @@ __device__ __forceinline__ int conv_len(const seg_causal_conv_args& p, int b) {
 }
 __device__ __forceinline__ float conv_act(float v, int act) { return act == SEG_ACT_SILU ? v * sigmoid_f(v) : v; }
 
-// threads: 32 channel groups of 8 x 8 runs of RUN rows; grid (channels / 256, runs / 8, B)
-template <typename T, bool VEC, int K>
+// threads: 32 channel groups of 8 x 8 runs of RUNS rows; grid (channels / 256, runs / 8, B).  A run's rows are all on their way before the
+// first is used: one memory latency per run
+template <typename T, bool VEC, int K, int RUNS>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(const seg_causal_conv_args p) {
   const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8, b = blockIdx.z;
   const int64_t run = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5);
   if (c >= p.D) return;
   const int len = conv_len(p, b), n = p.D - c;
-  const int64_t t0l = run * RUN;
+  const int64_t t0l = run * RUNS;
   if (run == 0 && p.state_out != nullptr && K > 1) {          // one thread per channel group carries the state on
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
-      float f[8];
+      Raw<T, VEC> f;
       load_xx<T, VEC, K>(p, b, len - (K - 1) + k, len, c, f);
-      row_store8<T, VEC>((T*)p.state_out + ((int64_t)b * (K - 1) + k) * p.D + c, n, f);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = f[j];
+      row_store8<T, VEC>((T*)p.state_out + ((int64_t)b * (K - 1) + k) * p.D + c, n, v);
     }
   }
   if (t0l >= p.L) return;
-  const int t0 = (int)t0l, t1 = t0 + RUN < p.L ? t0 + RUN : p.L;
-  float w[K][8], bias[8], win[K][8];
+  const int t0 = (int)t0l, t1 = t0 + RUNS < p.L ? t0 + RUNS : p.L;
+  Raw<T, VEC> x[RUNS + K - 1];                                 // x[i]: row t0 - (K - 1) + i of xx
+#pragma unroll
+  for (int i = 0; i < RUNS + K - 1; ++i) load_xx<T, VEC, K>(p, b, t0 - (K - 1) + i, len, c, x[i]);
+  float w[K][8], bias[8];
 #pragma unroll
   for (int k = 0; k < K; ++k) load_par<VEC>(p.w + (int64_t)k * p.D + c, n, w[k]);
   load_par<VEC>(p.bias == nullptr ? nullptr : p.bias + c, n, bias);
-#pragma unroll
-  for (int k = 1; k < K; ++k) load_xx<T, VEC, K>(p, b, t0 - K + k, len, c, win[k]);
   T* y = (T*)p.y + b * p.y_bs + c;
 #pragma unroll
-  for (int i = 0; i < RUN; ++i) {
+  for (int i = 0; i < RUNS; ++i) {
     const int t = t0 + i;
     if (t < t1) {
-#pragma unroll
-      for (int k = 0; k + 1 < K; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) win[k][j] = win[k + 1][j];
-      load_xx<T, VEC, K>(p, b, t, len, c, win[K - 1]);
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = bias[j];
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[j] = fmaf(w[k][j], win[k][j], v[j]);
+        for (int k = 0; k < K; ++k) v[j] = fmaf(w[k][j], x[i + k][j], v[j]);
         v[j] = t < len ? conv_act(v[j], p.act) : 0.f;
       }
       row_store8<T, VEC>(y + t * p.y_ld, n, v);
@@ -81,49 +93,49 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(const seg_causal_conv_arg
   }
 }
 
-// The same run of rows backward: dv of rows t0 .. t0 + RUN + K - 2 (each from its own window), dx[t] from the K dv behind it; dw / db
+// The same run of rows backward: dv of rows t0 .. t0 + RUNS + K - 2 (each from its own window), dx[t] from the K dv behind it; dw / db
 // from the run's own rows only, summed over the block's eight runs in LDS: part[block along rows and B][K + 1][D].
 template <typename T, bool VEC, int K>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(const seg_causal_conv_args p, float* part) {
+  constexpr int RUNS = RUN_SMALL;
   const int cg = threadIdx.x & 31, c = (blockIdx.x * 32 + cg) * 8, b = blockIdx.z;
-  const int64_t run = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5), t0l = run * RUN;
+  const int64_t run = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5), t0l = run * RUNS;
   const int len = conv_len(p, b), n = c < p.D ? p.D - c : 0;
   float dw[K + 1][8];
 #pragma unroll
   for (int k = 0; k <= K; ++k)
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[k][j] = 0.f;
-  // rows of dx this thread writes: [lo, t1); the first run also owns the carried state's rows -(K - 1) .. -1
+  // rows of dx this thread writes: [t0, t1); the first run also owns the carried state's rows -(K - 1) .. -1
   if (n > 0 && (t0l < p.L || run == 0)) {
-    const int t0 = (int)t0l, t1 = t0 + RUN < p.L ? t0 + RUN : p.L;
-    float w[K][8], bias[8], win[K][8], dv[K][8];               // dv[k] = dv of row r - (K - 1) + k
+    const int t0 = (int)t0l, t1 = t0 + RUNS < p.L ? t0 + RUNS : p.L;
+    Raw<T, VEC> x[RUNS + 2 * K - 2], dy[RUNS + K - 1];         // x[i]: row t0 - (K - 1) + i of xx;  dy[i]: row t0 + i
+#pragma unroll
+    for (int i = 0; i < RUNS + 2 * K - 2; ++i) load_xx<T, VEC, K>(p, b, t0 - (K - 1) + i, len, c, x[i]);
+#pragma unroll
+    for (int i = 0; i < RUNS + K - 1; ++i) dy[i].load((const T*)p.dy + b * p.dy_bs + (t0 + i) * p.dy_ld + c, t0 + i < len ? n : 0);
+    float w[K][8], bias[8], dv[K][8];                          // dv[k] = dv of row r - (K - 1) + k
 #pragma unroll
     for (int k = 0; k < K; ++k) load_par<VEC>(p.w + (int64_t)k * p.D + c, n, w[k]);
     load_par<VEC>(p.bias == nullptr ? nullptr : p.bias + c, n, bias);
 #pragma unroll
-    for (int k = 1; k < K; ++k) load_xx<T, VEC, K>(p, b, t0 - K + k, len, c, win[k]);
-#pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) dv[k][j] = 0.f;
-    const T* dy = (const T*)p.dy + b * p.dy_bs + c;
 #pragma unroll
-    for (int i = 0; i < RUN + K - 1; ++i) {
+    for (int i = 0; i < RUNS + K - 1; ++i) {
       const int r = t0 + i;                                    // the row whose dv is computed; dx of row r - (K - 1) is complete then
       if (r < t1 + K - 1) {
-#pragma unroll
-        for (int k = 0; k + 1 < K; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) { win[k][j] = win[k + 1][j]; dv[k][j] = dv[k + 1][j]; }
-        load_xx<T, VEC, K>(p, b, r, len, c, win[K - 1]);
         float d[8];
-        row_load8<T, VEC>(dy + r * p.dy_ld, r < len ? n : 0, d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int k = 0; k + 1 < K; ++k) dv[k][j] = dv[k + 1][j];
+          d[j] = dy[i][j];
           if (p.act == SEG_ACT_SILU) {
             float v = bias[j];
 #pragma unroll
-            for (int k = 0; k < K; ++k) v = fmaf(w[k][j], win[k][j], v);
+            for (int k = 0; k < K; ++k) v = fmaf(w[k][j], x[i + k][j], v);
             const float s = sigmoid_f(v);
             d[j] *= s * (1.f + v * (1.f - s));
           }
@@ -135,7 +147,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const seg_causal_conv_arg
           for (int j = 0; j < 8; ++j) {
             dw[K][j] += d[j];
 #pragma unroll
-            for (int k = 0; k < K; ++k) dw[k][j] = fmaf(d[j], win[k][j], dw[k][j]);
+            for (int k = 0; k < K; ++k) dw[k][j] = fmaf(d[j], x[i + k][j], dw[k][j]);
           }
         }
         const int t = r - (K - 1);                             // dxx row t + K - 1: sum_k w[k] dv[t + K - 1 - k]
@@ -226,8 +238,8 @@ inline bool conv_vec(const seg_causal_conv_args& a, bool bwd) {
   if (bwd) return ok && vec_ok(a.dy, a.dy_ld, a.dy_bs, a.dtype) && vec_ok(a.dx, a.dx_ld, a.dx_bs, a.dtype) && vec_ok(a.dstate, 0, 0, a.dtype) && vec_ok(a.dstate_out, 0, 0, a.dtype);
   return ok && vec_ok(a.y, a.y_ld, a.y_bs, a.dtype) && vec_ok(a.state_out, 0, 0, a.dtype);
 }
-inline dim3 conv_grid(const seg_causal_conv_args& a) {
-  const int64_t runs = ((int64_t)a.L + RUN - 1) / RUN, yb = (runs + 7) / 8;
+inline dim3 conv_grid(const seg_causal_conv_args& a, int run) {
+  const int64_t runs = ((int64_t)a.L + run - 1) / run, yb = (runs + 7) / 8;
   return dim3((unsigned)((a.D + 255) / 256), (unsigned)(yb < 1 ? 1 : yb), (unsigned)a.B);
 }
 
@@ -238,7 +250,7 @@ int check_conv(const seg_causal_conv_args* a, const char* name) {
   SEG_CHECK_ARG(a->K >= 1 && a->K <= MAXK, "%s: K = %d (1 .. %d)", name, a->K, MAXK);
   SEG_CHECK_ARG(a->act == SEG_ACT_NONE || a->act == SEG_ACT_SILU, "%s: activation %d (none or silu)", name, a->act);
   SEG_CHECK_ARG(a->B <= 65535, "%s: %d sequences in one call (65535 at most)", name, a->B);
-  SEG_CHECK_ARG(a->L <= 65535 * 8 * RUN, "%s: %d rows in one call (%d at most)", name, a->L, 65535 * 8 * RUN);
+  SEG_CHECK_ARG(a->L <= 65535 * 8 * RUN_SMALL, "%s: %d rows in one call (%d at most)", name, a->L, 65535 * 8 * RUN_SMALL);
   SEG_CHECK_ARG(a->w != nullptr, "%s: w is NULL", name);
   return SEG_OK;
 }
@@ -253,7 +265,10 @@ extern "C" int seg_causal_conv_fwd(const seg_causal_conv_args* a, seg_stream_t s
   if (a->B == 0 || (a->L == 0 && a->state_out == nullptr)) return SEG_OK;
   conv_dispatch(*a, conv_vec(*a, false), [&](auto* tp, auto V, auto Kc) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
-    hipLaunchKernelGGL((conv_fwd_kernel<T, V(), Kc()>), conv_grid(*a), dim3(256), 0, (hipStream_t)stream, *a);
+    // runs of 16 rows read the window's edges half as often as runs of 8; too few of them to fill the card are halved
+    const dim3 grid = conv_grid(*a, RUN);
+    if ((int64_t)grid.x * grid.y * grid.z >= 1024) hipLaunchKernelGGL((conv_fwd_kernel<T, V(), Kc(), RUN>), grid, dim3(256), 0, (hipStream_t)stream, *a);
+    else hipLaunchKernelGGL((conv_fwd_kernel<T, V(), Kc(), RUN_SMALL>), conv_grid(*a, RUN_SMALL), dim3(256), 0, (hipStream_t)stream, *a);
   });
   SEG_CHECK_LAUNCH("causal_conv_fwd");
   return SEG_OK;
@@ -261,7 +276,7 @@ extern "C" int seg_causal_conv_fwd(const seg_causal_conv_args* a, seg_stream_t s
 
 extern "C" int64_t seg_causal_conv_bwd_workspace_bytes(const seg_causal_conv_args* a) {
   if (a == nullptr || a->B <= 0 || a->L < 0 || a->D <= 0 || a->K < 1) return 0;
-  return (int64_t)a->B * conv_grid(*a).y * (a->K + 1) * a->D * 4;
+  return (int64_t)a->B * conv_grid(*a, RUN_SMALL).y * (a->K + 1) * a->D * 4;
 }
 
 extern "C" int seg_causal_conv_bwd(const seg_causal_conv_args* a, seg_stream_t stream) {
@@ -273,15 +288,14 @@ extern "C" int seg_causal_conv_bwd(const seg_causal_conv_args* a, seg_stream_t s
   SEG_CHECK_ARG(a->dx == nullptr || (a->dx != a->dy && a->dx != a->x), "causal_conv_bwd: dx may not be dy or x");
   hipStream_t st = (hipStream_t)stream;
   float* part = params ? (float*)a->workspace : nullptr;
-  const dim3 grid = conv_grid(*a);
+  const dim3 grid = conv_grid(*a, RUN_SMALL);
   if (a->B > 0)
     conv_dispatch(*a, conv_vec(*a, true), [&](auto* tp, auto V, auto Kc) {
       typedef typename std::remove_pointer<decltype(tp)>::type T;
       hipLaunchKernelGGL((conv_bwd_kernel<T, V(), Kc()>), grid, dim3(256), 0, st, *a, part);
     });
   const int64_t parts = (int64_t)a->B * grid.y, ld = (int64_t)(a->K + 1) * a->D;
-  if (a->dw != nullptr) launch_colsum_parts(part, parts, ld, (int64_t)a->K * a->D, a->dw, st);
-  if (a->db != nullptr) launch_colsum_parts(part == nullptr ? nullptr : part + (int64_t)a->K * a->D, parts, ld, a->D, a->db, st);
+  launch_colsum_pair(part, parts, ld, (int64_t)a->K * a->D, a->dw, a->D, a->db, st);
   SEG_CHECK_LAUNCH("causal_conv_bwd");
   return SEG_OK;
 }

@@ -717,7 +717,7 @@ extern "C" int seg_linear_bwd_weight(const seg_linear_args* a, seg_stream_t stre
         else
           hipLaunchKernelGGL((colsum_rows_kernel<T, false>), grid, dim3(TPB), 0, st, (const T*)a->dy, a->dy_ld, a->M, a->N, c.per, part);
       });
-    launch_colsum_parts(part, c.parts, a->N, a->N, a->db, st);
+    launch_colsum_pair(part, c.parts, a->N, a->N, a->db, 0, nullptr, st);
   }
   SEG_CHECK_LAUNCH("linear_bwd_weight");
   return SEG_OK;

@@ -301,21 +301,26 @@ inline LnShape ln_shape(int C) {
   if (chunks <= 1024) return {256, 4};
   return {256, 8};
 }
+// backward: five row-sized arrays per lane instead of one - rows of more than 512 channels take the whole block
+inline LnShape ln_bwd_shape(int C) {
+  const int chunks = (C + 7) / 8;
+  return chunks <= 64 ? ln_shape(C) : chunks <= 256 ? LnShape{256, 1} : ln_shape(C);
+}
 template <typename F>
 inline void ln_dispatch(const LnShape& s, F&& f) {
   using std::integral_constant;
 #define LN_CASE(L, N) \
   if (s.lpr == L && s.nch == N) return f(integral_constant<int, L>{}, integral_constant<int, N>{});
-  LN_CASE(8, 1) LN_CASE(16, 1) LN_CASE(32, 1) LN_CASE(64, 1) LN_CASE(64, 2) LN_CASE(64, 4) LN_CASE(256, 2) LN_CASE(256, 4) LN_CASE(256, 8)
+  LN_CASE(8, 1) LN_CASE(16, 1) LN_CASE(32, 1) LN_CASE(64, 1) LN_CASE(64, 2) LN_CASE(64, 4) LN_CASE(256, 1) LN_CASE(256, 2) LN_CASE(256, 4) LN_CASE(256, 8)
 #undef LN_CASE
 }
 // the kernels walk rows with the grid as stride: more blocks than this gain nothing
 inline unsigned ln_grid(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20); }
 inline int64_t ln_bwd_blocks(int64_t rows, int C) {
   if (C > LN_REG_MAX) return rows < 64 ? rows : 64;
-  const int64_t rpb = TPB / ln_shape(C).lpr, groups = (rows + rpb - 1) / rpb;
-  // at least four row groups per block: the partial rows are then at most a tenth of the traffic
-  const int64_t most = 1024, want = (groups + 3) / 4;
+  const int64_t rpb = TPB / ln_bwd_shape(C).lpr, groups = (rows + rpb - 1) / rpb;
+  // every block leaves a partial row pair in 32 bits: at least eight rows per block keep that below a tenth of the traffic
+  const int64_t most = 1024, share = rpb >= 4 ? 2 : 8 / rpb, want = (groups + share - 1) / share;
   return want < most ? want : most;
 }
 
@@ -385,19 +390,14 @@ extern "C" int seg_layernorm_bwd(const void* dy, int64_t dy_ld, const void* x, i
           hipLaunchKernelGGL((ln_bwd_long_dx_kernel<T>), dim3(ln_grid(rows)), dim3(TPB), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (T*)dx, dx_ld, rows, C, mean, rstd, gamma);
         return;
       }
-      ln_dispatch(ln_shape(C), [&](auto L, auto N) {
+      ln_dispatch(ln_bwd_shape(C), [&](auto L, auto N) {
         if (ln_vec({x, dy, dx, gamma}, {x_ld, dy_ld, dx == nullptr ? 0 : dx_ld}, C, dtype))
           hipLaunchKernelGGL((ln_bwd_kernel<T, true, L(), N()>), dim3((unsigned)nblk), dim3(TPB), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (T*)dx, dx_ld, rows, C, mean, rstd, gamma, part);
         else
           hipLaunchKernelGGL((ln_bwd_kernel<T, false, L(), N()>), dim3((unsigned)nblk), dim3(TPB), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (T*)dx, dx_ld, rows, C, mean, rstd, gamma, part);
       });
     });
-  if (dgamma != nullptr && dbeta == dgamma + C) {            // one buffer for both: one launch
-    launch_colsum_parts(part, nblk, 2 * (int64_t)C, 2 * (int64_t)C, dgamma, st);
-    dgamma = dbeta = nullptr;
-  }
-  if (dgamma != nullptr) launch_colsum_parts(part, nblk, 2 * (int64_t)C, C, dgamma, st);
-  if (dbeta != nullptr) launch_colsum_parts(part == nullptr ? nullptr : part + C, nblk, 2 * (int64_t)C, C, dbeta, st);
+  launch_colsum_pair(part, nblk, 2 * (int64_t)C, C, dgamma, C, dbeta, st);
   SEG_CHECK_LAUNCH("layernorm_bwd");
   return SEG_OK;
 }

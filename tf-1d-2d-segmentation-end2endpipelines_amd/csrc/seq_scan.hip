@@ -35,12 +35,20 @@ template <int G> struct Lay {
 };
 
 __device__ __forceinline__ float exp2_f(float v) { return __builtin_amdgcn_exp2f(v); }
-// max(v, 0) + log(1 + e), e = exp(-|v|), with a small RELATIVE error: 1 + e loses low bits of e, which the logarithm gets back to first
-// order (log(1 + e) = log(w) + (e - (w - 1)) / w, w the rounded sum); where e is small the series is used
+// max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1], with a small RELATIVE error for every v: log(1 + e) = e P(e), P of degree 8 fitted to
+// 3e-8 on [0, 1] - half the instructions of a logarithm whose argument's lost bits are corrected
 __device__ __forceinline__ float softplus_f(float v) {
-  const float e = __expf(-fabsf(v)), w = 1.f + e;
-  const float l = e < 0.03125f ? e * (1.f - e * (0.5f - e * (0.33333333f - e * (0.25f - e * 0.2f)))) : __logf(w) + (e - (w - 1.f)) * __frcp_rn(w);
-  return fmaxf(v, 0.f) + l;
+  const float e = __expf(-fabsf(v));
+  float P = 0.0052326812f;
+  P = fmaf(P, e, -0.0295051865f);
+  P = fmaf(P, e, 0.0782258667f);
+  P = fmaf(P, e, -0.136632386f);
+  P = fmaf(P, e, 0.191060034f);
+  P = fmaf(P, e, -0.248429813f);
+  P = fmaf(P, e, 0.333190967f);
+  P = fmaf(P, e, -0.499994931f);
+  P = fmaf(P, e, 0.99999997f);
+  return fmaf(P, e, fmaxf(v, 0.f));
 }
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -53,6 +61,29 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
   if constexpr (G >= 8) v += dpp<DPP_HALF_MIRROR>(v);
   if constexpr (G >= 16) v += dpp<DPP_MIRROR>(v);
   return v;
+}
+
+// y[0..3]: a channel's parts of four rows in each of its G lanes.  Stores the rows' sums at o[row * ld]: lane g & 3 the row of that number,
+// no lane waits for another's branch (in two halvings for G = 4: a lane keeps what it will store and sends the rest)
+template <int G> __device__ __forceinline__ void store_rows4(const float* y, int g, float* o, int ld) {
+  if constexpr (G == 4) {
+    const bool odd = g & 1, up = g & 2;
+    const float a = (odd ? y[1] : y[0]) + dpp<DPP_XOR1>(odd ? y[0] : y[1]), b = (odd ? y[3] : y[2]) + dpp<DPP_XOR1>(odd ? y[2] : y[3]);
+    o[g * ld] = (up ? b : a) + dpp<DPP_XOR2>(up ? a : b);
+  } else if constexpr (G > 4) {
+    float s[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = group_sum<G>(y[k]);
+    o[(g & 3) * ld] = (g & 2) ? ((g & 1) ? s[3] : s[2]) : ((g & 1) ? s[1] : s[0]);       // (lanes of one number store the same value)
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; k += G) {
+      float s[G];
+#pragma unroll
+      for (int j = 0; j < G; ++j) s[j] = group_sum<G>(y[k + j]);
+      o[(k + g) * ld] = G == 1 ? s[0] : g ? s[G - 1] : s[0];
+    }
+  }
 }
 
 __device__ __forceinline__ int scan_len(const seg_scan_args& p, int b) {
@@ -184,19 +215,34 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_arg
       if constexpr (MAIN) rC.put(sC);
       if (t0 + TT < tlive) fetch(t0 + TT);
       __syncthreads();
-#pragma unroll 4
-      for (int r = 0; r < TT; ++r) {
-        const float2 dd = sdu[r][c];
-        const f4 B4 = *reinterpret_cast<const f4*>(sB + r * Y::SP + 4 * g);
+      // four rows at a time, the next four rows' operands on their way from the LDS meanwhile
+      float2 dn[4];
+      f4 Bn[4], Cn[4];
+      auto ahead = [&](int r) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_f(dd.x * A2[i]), h[i], dd.y * B4[i]);
-        if constexpr (MAIN) {
-          const f4 C4 = *reinterpret_cast<const f4*>(sC + r * Y::SP + 4 * g);
-          const float y = group_sum<G>(fmaf(C4[3], h[3], fmaf(C4[2], h[2], fmaf(C4[1], h[1], C4[0] * h[0]))));
-          if (g == 0) sy[r][c] = y;
-        } else {
-          dsum += dd.x;
+        for (int k = 0; k < 4; ++k) {
+          dn[k] = sdu[r + k][c];
+          Bn[k] = *reinterpret_cast<const f4*>(sB + (r + k) * Y::SP + 4 * g);
+          if constexpr (MAIN) Cn[k] = *reinterpret_cast<const f4*>(sC + (r + k) * Y::SP + 4 * g);
         }
+      };
+      ahead(0);
+#pragma unroll 2
+      for (int r = 0; r < TT; r += 4) {
+        float2 dd[4];
+        f4 B4[4], C4[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { dd[k] = dn[k]; B4[k] = Bn[k]; C4[k] = Cn[k]; }
+        if (r + 4 < TT) ahead(r + 4);
+        float y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_f(dd[k].x * A2[i]), h[i], dd[k].y * B4[k][i]);
+          if constexpr (MAIN) y[k] = fmaf(C4[k][3], h[3], fmaf(C4[k][2], h[2], fmaf(C4[k][1], h[1], C4[k][0] * h[0])));
+          else dsum += dd[k].x;
+        }
+        if constexpr (MAIN) store_rows4<G>(y, g, &sy[r][c], Y::CB);
       }
       __syncthreads();
     }
@@ -485,7 +531,7 @@ __global__ __launch_bounds__(Lay<G>::NT, 2) void scan_bwd_kernel(const seg_scan_
             h[i] = fmaf(a[k][i], h[i], du * Bc[i]);
           }
           const float y = group_sum<G>(fmaf(Cc[3], h[3], fmaf(Cc[2], h[2], fmaf(Cc[1], h[1], Cc[0] * h[0]))));
-          if (g == 0) sx[r0 + k][c][3] = y;
+          sx[r0 + k][c][3] = y;                                // (every lane of the channel holds and stores the same sum: no branch)
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -515,9 +561,10 @@ __global__ __launch_bounds__(Lay<G>::NT, 2) void scan_bwd_kernel(const seg_scan_
         h = hp[k];
         sgB = group_sum<G>(sgB);
         sA = group_sum<G>(sA);
-        if (g == 0) { sx[r0 + k][c][1] = sgB; sx[r0 + k][c][2] = sA; }
+        sx[r0 + k][c][1] = sgB;
+        sx[r0 + k][c][2] = sA;
         lane_sums<G>(v, w);
-        if ((lane & 15) < G) *reinterpret_cast<float2*>(&sbc[wave][k][lane >> 5][4 * g + 2 * ((lane >> 4) & 1)]) = float2{w[0], w[1]};
+        *reinterpret_cast<float2*>(&sbc[wave][k][lane >> 5][4 * g + 2 * ((lane >> 4) & 1)]) = float2{w[0], w[1]};
         __builtin_amdgcn_sched_barrier(0);
       }
       __syncthreads();
@@ -809,9 +856,17 @@ extern "C" int seg_selective_scan_bwd(const seg_scan_args* a, seg_stream_t strea
     });
   }
   const int64_t parts = none ? 0 : (int64_t)a->B * s.nch;
-  if (a->dA != nullptr) launch_colsum_parts(ws + (none ? 0 : w.pA), parts, n, n, a->dA, st);
-  if (a->dD != nullptr) launch_colsum_parts(ws + (none ? 0 : w.pD), parts, 2 * (int64_t)a->D, a->D, a->dD, st);
-  if (a->ddt_bias != nullptr) launch_colsum_parts(none ? ws : ws + w.pD + a->D, parts, 2 * (int64_t)a->D, a->D, a->ddt_bias, st);
+  // dA and, their columns being neighbours, dD / ddt_bias in one launch; outputs that are not neighbours take another
+  const float *pAs = none ? nullptr : ws + w.pA, *pDs = none ? nullptr : ws + w.pD;
+  const int64_t D2 = 2 * (int64_t)a->D;
+  ColsumSet sa{pAs, parts, n, a->dA != nullptr ? n : 0, a->dA}, sd{pDs, parts, D2, 0, a->dD};
+  if (a->dD != nullptr && a->ddt_bias == a->dD + a->D) {
+    sd.cols = D2;
+    launch_colsum_sets(sa, sd, st);
+  } else {
+    launch_colsum_sets(sa, sd, st);
+    launch_colsum_pair(pDs, parts, D2, a->D, a->dD, a->D, a->ddt_bias, st);
+  }
   SEG_CHECK_LAUNCH("selective_scan_bwd");
   return SEG_OK;
 }

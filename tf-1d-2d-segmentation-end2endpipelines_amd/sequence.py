@@ -363,8 +363,8 @@ def causal_conv_backward(dy, x, w, bias=None, activation: Optional[str] = None, 
     di = _gpu(what, x)
     dev = x.device
     dx = torch.empty((B, L, d), dtype=x.dtype, device=dev)
-    dw = torch.empty((K, d), dtype=torch.float32, device=dev)
-    db = torch.empty((d,), dtype=torch.float32, device=dev) if bias is not None else None
+    par = torch.empty((K + 1, d), dtype=torch.float32, device=dev)          # (one buffer: the sums over the blocks take one launch)
+    dw, db = par[:K], par[K] if bias is not None else None
     dst = torch.empty((B, K - 1, d), dtype=x.dtype, device=dev) if state is not None else None
     a = CausalConvArgs(B, L, d, K, dt, act, _ptr(x), x.stride(0), x.stride(1), _ptr(w), _ptr(bias), _ptr(state), _ptr(lengths), None, 0, 0, None,
                        _ptr(dy), dy.stride(0), dy.stride(1), _ptr(dstate), _ptr(dx), L * d, d, _ptr(dw), _ptr(db), _ptr(dst))
@@ -515,8 +515,9 @@ def selective_scan_backward(dy, u, dt, A, B, C, saved, D=None, z=None, dt_bias=N
     def flat(*shape):
         return torch.empty(shape, dtype=torch.float32, device=dev)
 
-    g = ScanGrads(rows(d), rows(d), flat(d, S), rows(S), rows(S), None if D is None else flat(d), None if z is None else rows(d),
-                  None if dt_bias is None else flat(d), flat(nb, d, S))
+    par = flat(2, d)
+    g = ScanGrads(rows(d), rows(d), flat(d, S), rows(S), rows(S), None if D is None else par[0], None if z is None else rows(d),
+                  None if dt_bias is None else par[1], flat(nb, d, S))
     a.saved, a.dy, a.dy_bs, a.dy_ld, a.dstate_out = _ptr(saved), _ptr(dy), dy.stride(0), dy.stride(1), _ptr(dstate)
     for n, t, c in (("du", g.du, d), ("ddt", g.ddt, d), ("dz", g.dz, d), ("dBm", g.dB, S), ("dCm", g.dC, S)):
         if t is not None:
