@@ -168,7 +168,8 @@ def test_linear_backward(M, N, K, dtype):
     R.assert_close(dw, d64.t() @ x64, d64.abs().t() @ x64.abs(), M + 4, "dw")
     R.assert_close(db, d64.sum(0), d64.abs().sum(0), M + 4, "db")
     dx, none, db2 = seq.linear_backward(dy.cuda(), x.cuda(), w.cuda(), need_dw=False)
-    assert none is None and torch.equal(db, db2)
+    assert none is None
+    R.assert_close(db2, d64.sum(0), d64.abs().sum(0), M + 4, "db alone (another order of the same sum)")
     R.assert_close(dx, d64 @ w64, s, N + 4, "dx plain")
 
 

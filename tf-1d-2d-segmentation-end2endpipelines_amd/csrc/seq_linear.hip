@@ -27,6 +27,8 @@ struct GemmArgs {
   const void* res; int64_t res_ld;
   void* z; int64_t z_ld;
   void* out; int64_t out_ld;
+  float* db;                     // bwd_weight: column sums of dy (NULL: not wanted)
+  float* part_db;                // [splits][I]
   int vecio;                     // rows of z, residual and out take 16-byte accesses
 };
 
@@ -44,6 +46,27 @@ template <int PASS, typename T> __device__ __forceinline__ void epilogue1(const 
     }
     if (p.res != nullptr) v += (float)((const T*)p.res)[i * p.res_ld + j];
     ((T*)p.out)[i * p.out_ld + j] = (T)v;
+  }
+}
+
+template <typename T> __device__ __forceinline__ f16v mfma16(u4 a, u4 b, f16v c) {
+  if constexpr (std::is_same<T, half_t>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+template <typename T> __device__ __forceinline__ u4 ones16() {
+  const uint32_t one = std::is_same<T, half_t>::value ? 0x3c003c00u : 0x3f803f80u;
+  return u4{one, one, one, one};
+}
+// a product with ones: every column of the 32 x 32 tile holds the rows' sums
+__device__ __forceinline__ void store_sums(const GemmArgs& p, const f16v& acc, int64_t ib, int lane) {
+  if ((lane & 31) != 0) return;
+  float* o = p.splits > 1 ? p.part_db + blockIdx.y * p.I : p.db;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const int64_t i = ib + (q & 3) + 8 * (q >> 2) + 4 * (lane >> 5);
+    if (i < p.I) o[i] = acc[q];
   }
 }
 
@@ -102,10 +125,12 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
       for (int e = 0; e < S::EPT; ++e) d[e * S::LD] = r[e];
     }
   };
-  f16v acc;
+  f16v acc, accb;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) acc[q] = 0.f;
+  for (int q = 0; q < 16; ++q) acc[q] = accb[q] = 0.f;
   const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+  // the sums of dy's columns ride on the first tile column's waves as one more product, with ones
+  const bool sums = PASS == SEG_LINEAR_BWD_WEIGHT && p.db != nullptr && j0 == 0 && wj == 0;
   fetch(A, p.a_ld, AKC, i0, p.I, kbeg, ra);
   fetch(B, p.b_ld, BKC, j0, p.J, kbeg, rb);
   int buf = 0;
@@ -121,17 +146,21 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
       for (int ks = 0; ks < S::BK / 2; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(sa[2 * ks + fh], sb[2 * ks + fh], acc, 0, 0, 0);
-    } else if constexpr (std::is_same<T, half_t>::value) {
+      if (sums) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8*>(sa + ks * 16 + fh * 8), *reinterpret_cast<const h8*>(sb + ks * 16 + fh * 8), acc, 0, 0, 0);
+        for (int ks = 0; ks < S::BK / 2; ++ks) accb = __builtin_amdgcn_mfma_f32_32x32x2f32(sa[2 * ks + fh], 1.f, accb, 0, 0, 0);
+      }
     } else {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const b8*>(sa + ks * 16 + fh * 8), *reinterpret_cast<const b8*>(sb + ks * 16 + fh * 8), acc, 0, 0, 0);
+      for (int ks = 0; ks < 2; ++ks) acc = mfma16<T>(ld16(sa + ks * 16 + fh * 8), ld16(sb + ks * 16 + fh * 8), acc);
+      if (sums) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) accb = mfma16<T>(ld16(sa + ks * 16 + fh * 8), ones16<T>(), accb);
+      }
     }
     // the buffer written next is the one whose readers passed the barrier above
   }
+  if (sums) store_sums(p, accb, i0 + wi, lane);
   const int j = j0 + wj + fr;
   if (j < p.J) {
 #pragma unroll
@@ -231,13 +260,6 @@ template <bool KC, int ROWS, int BK> __device__ __forceinline__ u4 tile_frag(con
     return u4{l[0], l[1], h[0], h[1]};
   }
 }
-template <typename T> __device__ __forceinline__ f16v mfma16(u4 a, u4 b, f16v c) {
-  if constexpr (std::is_same<T, half_t>::value)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-}
-
 // eight neighbouring elements of the result through the pass's epilogue; f: the row of z (bwd_data), r: of the residual, fetched before
 template <int PASS, typename T> __device__ __forceinline__ void epilogue8(const GemmArgs& p, int64_t i, int j, const float* bias, float* v, const float* f,
                                                                           const float* r, bool vec) {
@@ -483,16 +505,22 @@ __global__ __launch_bounds__(64 * WK) void gemm_rows_kernel(const GemmArgs p) {
 // the split ranges of k added in order, then the epilogue
 template <int PASS, typename T>
 __global__ __launch_bounds__(TPB) void gemm_join_kernel(const GemmArgs p) {
-  const int64_t n = p.I * p.J;
-  for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < n; e += (int64_t)gridDim.x * TPB) {
+  const int64_t n = p.I * p.J, all = n + (p.db != nullptr ? p.I : 0);
+  for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < all; e += (int64_t)gridDim.x * TPB) {
     float v = 0.f;
+    if (PASS == SEG_LINEAR_BWD_WEIGHT && e >= n) {
+      for (int s = 0; s < p.splits; ++s) v += p.part_db[s * p.I + e - n];
+      p.db[e - n] = v;
+      continue;
+    }
     for (int s = 0; s < p.splits; ++s) v += p.part[s * n + e];
     const int64_t i = e / p.J;
     epilogue1<PASS, T>(p, i, (int)(e - i * p.J), v);
   }
 }
 
-// ---- bias gradient: column sums of dy, rows in ranges of blocks (part[range][N], added up in order by colsum_parts_kernel)
+// ---- the bias gradient where gemm_any_kernel does not carry it (no weight gradient wanted; the tile kernels, whose registers the extra
+// product overflows: 133 -> 213 us): column sums of dy, rows in ranges of blocks (part[range][N], added up in order by colsum_parts_kernel)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(TPB) void colsum_rows_kernel(const T* dy, int64_t ld, int64_t rows, int cols, int64_t per, float* part) {
   const int l = threadIdx.x & 31, r = threadIdx.x >> 5, c = (blockIdx.x * 32 + l) * 8;
@@ -590,6 +618,14 @@ inline GemmPlan plan_of(const seg_linear_args& a, int pass) {
   return gemm_plan(e.I, e.J, e.Kd, a.dtype, dma_ok(a, pass));
 }
 
+// bwd_weight: whether db is part of the product's launch, and the floats of the product's split sums (whole 16 bytes)
+inline bool sums_ride(const seg_linear_args& a) { return a.dw != nullptr && plan_of(a, SEG_LINEAR_BWD_WEIGHT).kind == TILE_ANY; }
+inline int64_t weight_parts(const seg_linear_args& a) {
+  const GemmPlan g = plan_of(a, SEG_LINEAR_BWD_WEIGHT);
+  if (a.dw == nullptr || g.splits <= 1) return 0;
+  return ((int64_t)g.splits * a.N * (a.K + (a.db != nullptr && g.kind == TILE_ANY ? 1 : 0)) + 3) / 4 * 4;
+}
+
 template <int PASS>
 int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
   const Extents e = extents(a, PASS);
@@ -597,6 +633,7 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
   p.I = e.I; p.J = e.J; p.Kd = e.Kd;
   p.ti = g.ti; p.tj = g.tj; p.splits = g.splits; p.kper = g.kper;
   p.part = (float*)a.workspace;
+  p.part_db = p.part + (int64_t)g.splits * e.I * e.J;
   p.act = a.act; p.alpha = a.alpha;
   p.vecio = PASS == SEG_LINEAR_BWD_WEIGHT ? vec_ok(p.out, p.out_ld, 0, SEG_DT_F32)
                                           : vec_ok(p.out, p.out_ld, 0, a.dtype) && vec_ok(p.z, p.z_ld, 0, a.dtype) && vec_ok(p.res, p.res_ld, 0, a.dtype);
@@ -624,7 +661,7 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
       if constexpr (!std::is_same<T, float>::value) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 8>), grid, dim3(TPB), 0, st, p);
     } else hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 1>), grid, dim3(TPB), 0, st, p);
     if (g.splits > 1) {
-      const int64_t blocks = (p.I * p.J + TPB - 1) / TPB;
+      const int64_t blocks = (p.I * (p.J + (p.db != nullptr ? 1 : 0)) + TPB - 1) / TPB;
       hipLaunchKernelGGL((gemm_join_kernel<PASS, T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(TPB), 0, st, p);
     }
   });
@@ -641,7 +678,8 @@ int check_linear(const seg_linear_args* a, int pass, const char* name) {
   SEG_CHECK_ARG(((e.I + 63) / 64) * ((int64_t)(e.J + 63) / 64) < (int64_t)1 << 24, "%s: result of %lld x %d is too large for one call", name, (long long)e.I, e.J);
   const GemmPlan g = plan_of(*a, pass);
   SEG_CHECK_ARG(aligned16(a->workspace), "%s: workspace needs 16-byte alignment", name);
-  SEG_CHECK_ARG(a->M == 0 || g.splits <= 1 || a->workspace != nullptr, "%s: workspace is NULL (%lld bytes are needed)", name, (long long)seg_linear_workspace_bytes(a, pass));
+  const bool joins = g.splits > 1 && !(pass == SEG_LINEAR_BWD_WEIGHT && a->dw == nullptr);
+  SEG_CHECK_ARG(a->M == 0 || !joins || a->workspace != nullptr, "%s: workspace is NULL (%lld bytes are needed)", name, (long long)seg_linear_workspace_bytes(a, pass));
   return SEG_OK;
 }
 
@@ -651,11 +689,8 @@ extern "C" int64_t seg_linear_workspace_bytes(const seg_linear_args* a, int32_t 
   if (a == nullptr || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
   const Extents e = extents(*a, pass);
   const GemmPlan g = plan_of(*a, pass);
-  int64_t b = g.splits > 1 ? (int64_t)g.splits * e.I * e.J * 4 : 0;
-  if (pass == SEG_LINEAR_BWD_WEIGHT) {
-    const int64_t c = colsum_plan(a->M, a->N).parts * a->N * 4;
-    b = (b + 15) / 16 * 16 + c;
-  }
+  if (pass == SEG_LINEAR_BWD_WEIGHT) return (weight_parts(*a) + (a->db != nullptr && !sums_ride(*a) ? colsum_plan(a->M, a->N).parts * a->N : 0)) * 4;
+  const int64_t b = g.splits > 1 ? (int64_t)g.splits * e.I * e.J * 4 : 0;
   return b;
 }
 
@@ -695,18 +730,15 @@ extern "C" int seg_linear_bwd_weight(const seg_linear_args* a, seg_stream_t stre
   SEG_CHECK_ARG(a->M == 0 || (a->dy != nullptr && (a->dw == nullptr || a->x != nullptr)), "linear_bwd_weight: dy / x is NULL");
   SEG_CHECK_ARG(a->M <= 1 || (a->dy_ld >= a->N && (a->dw == nullptr || a->x_ld >= a->K)), "linear_bwd_weight: row strides below N = %d / K = %d", a->N, a->K);
   SEG_CHECK_ARG(a->dw == nullptr || a->N == 1 || a->dw_ld >= a->K, "linear_bwd_weight: dw_ld below K = %d", a->K);
-  SEG_CHECK_ARG(a->db == nullptr || a->M == 0 || a->workspace != nullptr, "linear_bwd_weight: db needs the workspace");
+  SEG_CHECK_ARG(a->db == nullptr || sums_ride(*a) || a->M == 0 || a->workspace != nullptr, "linear_bwd_weight: db needs the workspace");
   hipStream_t st = (hipStream_t)stream;
   if (a->dw != nullptr) {
     GemmArgs p = {};
-    p.A = a->dy; p.a_ld = a->dy_ld; p.B = a->x; p.b_ld = a->x_ld; p.out = a->dw; p.out_ld = a->dw_ld;
+    p.A = a->dy; p.a_ld = a->dy_ld; p.B = a->x; p.b_ld = a->x_ld; p.out = a->dw; p.out_ld = a->dw_ld; p.db = sums_ride(*a) ? a->db : nullptr;
     run_gemm<SEG_LINEAR_BWD_WEIGHT>(*a, p, st);       // (M = 0: an empty sum, zeros are stored)
   }
-  if (a->db != nullptr) {
-    const Extents e = extents(*a, SEG_LINEAR_BWD_WEIGHT);
-    const GemmPlan g = plan_of(*a, SEG_LINEAR_BWD_WEIGHT);
-    const int64_t off = g.splits > 1 ? ((int64_t)g.splits * e.I * e.J * 4 + 15) / 16 * 16 : 0;
-    float* part = (float*)((char*)a->workspace + off);
+  if (a->db != nullptr && !sums_ride(*a)) {
+    float* part = (float*)a->workspace + weight_parts(*a);
     const ColsumPlan c = a->M > 0 ? colsum_plan(a->M, a->N) : ColsumPlan{0, 0};
     if (a->M > 0)
       seq_dispatch_dtype(a->dtype, [&](auto* tp) {
