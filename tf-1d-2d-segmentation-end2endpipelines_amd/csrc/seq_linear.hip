@@ -398,49 +398,56 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
   float* slab = reinterpret_cast<float*>(smem + wave * SLAB);
   const int fr = lane & 31, fh = lane >> 5;
   const bool vec = p.vecio != 0;
+  // what the epilogue reads (z of bwd_data, the residual) is fetched a 32 x 64 piece ahead of its use
+  constexpr int PIECES = TN / 2 * TM;
+  constexpr bool READS = PASS != SEG_LINEAR_BWD_WEIGHT;
+  Row8<T> zr[2][4], rr[2][4];
+  auto fetch = [&](int u) {
+    const int j = j0 + wc + (u / TM) * 64 + (lane & 7) * 8;
 #pragma unroll
-  for (int bp = 0; bp < TN / 2; ++bp) {
+    for (int r = 0; r < 4; ++r) {
+      const int64_t i = i0 + wr + (u % TM) * 32 + (lane >> 3) + r * 8;
+      if (j < p.J && i < p.I && p.splits == 1) {
+        if (PASS == SEG_LINEAR_BWD_DATA && p.z != nullptr) zr[u & 1][r].load((const T*)p.z + i * p.z_ld + j, vec);
+        if (p.res != nullptr) rr[u & 1][r].load((const T*)p.res + i * p.res_ld + j, vec);
+      }
+    }
+  };
+  if constexpr (READS) fetch(0);
+  float bias[8];
+#pragma unroll
+  for (int u = 0; u < PIECES; ++u) {
+    const int bp = u / TM, a = u % TM;
     const int j = j0 + wc + bp * 64 + (lane & 7) * 8;
     const bool jn = j < p.J;
-    float bias[8];
+    if (a == 0) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) bias[q] = (PASS == SEG_LINEAR_FWD && p.bias != nullptr && jn) ? p.bias[j + q] : 0.f;
-#pragma unroll
-    for (int a = 0; a < TM; ++a) {
-      const int64_t ib = i0 + wr + a * 32 + (lane >> 3);
-      Row8<T> zr[4], rr[4];
-      if constexpr (PASS != SEG_LINEAR_BWD_WEIGHT) {           // what the epilogue reads is on its way while the slab is written
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int64_t i = ib + r * 8;
-          if (jn && i < p.I && p.splits == 1) {
-            if (PASS == SEG_LINEAR_BWD_DATA && p.z != nullptr) zr[r].load((const T*)p.z + i * p.z_ld + j, vec);
-            if (p.res != nullptr) rr[r].load((const T*)p.res + i * p.res_ld + j, vec);
-          }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) slab[((q & 3) + 8 * (q >> 2) + 4 * fh) * 68 + h * 32 + fr] = acc[a][2 * bp + h][q];
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t i = ib + r * 8;
-        float v[8], f[8], g[8];
-        load8<float>(slab + ((lane >> 3) + r * 8) * 68 + (lane & 7) * 8, v);
-        if (i < p.I && jn) {
-          if (p.splits > 1) {
-            store8<float>(p.part + ((int64_t)blockIdx.y * p.I + i) * p.J + j, v);
-          } else {
-            if (PASS == SEG_LINEAR_BWD_DATA && p.z != nullptr) zr[r].get(f);
-            if (PASS != SEG_LINEAR_BWD_WEIGHT && p.res != nullptr) rr[r].get(g);
-            epilogue8<PASS, T>(p, i, j, bias, v, f, g, vec);
-          }
-        }
-      }
-      __builtin_amdgcn_wave_barrier();
+      for (int q = 0; q < 8; ++q) bias[q] = (PASS == SEG_LINEAR_FWD && p.bias != nullptr && jn) ? p.bias[j + q] : 0.f;
     }
+    if constexpr (READS) {
+      if (u + 1 < PIECES) fetch(u + 1);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) slab[((q & 3) + 8 * (q >> 2) + 4 * fh) * 68 + h * 32 + fr] = acc[a][2 * bp + h][q];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t i = i0 + wr + a * 32 + (lane >> 3) + r * 8;
+      float v[8], f[8], g[8];
+      load8<float>(slab + ((lane >> 3) + r * 8) * 68 + (lane & 7) * 8, v);
+      if (i < p.I && jn) {
+        if (p.splits > 1) {
+          store8<float>(p.part + ((int64_t)blockIdx.y * p.I + i) * p.J + j, v);
+        } else {
+          if (PASS == SEG_LINEAR_BWD_DATA && p.z != nullptr) zr[u & 1][r].get(f);
+          if (READS && p.res != nullptr) rr[u & 1][r].get(g);
+          epilogue8<PASS, T>(p, i, j, bias, v, f, g, vec);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
