@@ -1,5 +1,7 @@
 """GPU: the sequence operators (sequence.py) against their definitions in 64 bits (tests/sequence_ref.py), with bounds that count
 roundings; strides, lengths, empty and single rows, graphs, streams, and a whole mixer block forward, backward and row by row."""
+import importlib
+
 import pytest
 import torch
 
@@ -608,3 +610,144 @@ def test_two_streams_at_once():
                 got[k].append(m.prompt(xs[k])[0])
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[k]) for k in range(2) for y in got[k])
+
+
+# ------------------------------------------------------------------------------------------------------- offsets past 32 bits
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last rows come out as they do from a call on those rows alone (products and sums of another
+    launch shape: equal to two steps of the stored type)."""
+    def near(a, b, what):
+        a, b = a.float(), b.float()
+        assert float((a - b).abs().max()) <= 2.0 ** -9 * float(b.abs().max()), what
+    D = 1032
+    rows = (1 << 31) // D + 77
+    x = torch.randn(rows, D, device="cuda", dtype=torch.float16, generator=torch.Generator("cuda").manual_seed(1))
+    tail = x[-100:].contiguous()
+    y, mean, rstd = seq.layer_norm(x, stats=True)
+    assert torch.equal(y[-100:], seq.layer_norm(tail))
+    dx, _dg, _db = seq.layer_norm_backward(y, x, mean, rstd)
+    assert torch.equal(dx[-100:], seq.layer_norm_backward(y[-100:].contiguous(), tail, mean[-100:].contiguous(), rstd[-100:].contiguous())[0])
+    del dx
+    for n in (64, 20):                                          # the tile kernels and the one for every size
+        w = torch.randn(n, D, device="cuda", dtype=torch.float16, generator=torch.Generator("cuda").manual_seed(2)) * D ** -0.5
+        z = seq.linear(x, w)
+        near(z[-100:], seq.linear(tail, w), "linear")
+        near(seq.linear_backward(z, x, w, need_dw=False, need_db=False)[0][-100:], seq.linear_backward(z[-100:].contiguous(), tail, w, need_dw=False, need_db=False)[0], "dx")
+        _none, dw, db = seq.linear_backward(z, x, w, need_dx=False)
+        head, rest = rows - 100, slice(rows - 100, rows)
+        a = seq.linear_backward(z[:head], x[:head], w, need_dx=False)
+        b = seq.linear_backward(z[rest].contiguous(), tail, w, need_dx=False)
+        near(dw, a[1] + b[1], "dw")
+        assert float((db - a[2] - b[2]).abs().max()) <= 2.0 ** -9 * float(z.float().abs().sum(0).max()) * 2.0 ** -8, "db"
+    del z, y
+    cw = torch.randn(4, D, device="cuda")
+    xs = x[None]
+    yc, st = seq.causal_conv(xs, cw, activation="silu")
+    yt, st2 = seq.causal_conv(xs[:, -50:].contiguous(), cw, activation="silu", state=xs[:, -53:-50].contiguous())
+    assert torch.equal(yc[:, -50:], yt) and torch.equal(st, st2)
+    dxc = seq.causal_conv_backward(yc, xs, cw, activation="silu")[0]
+    dxt = seq.causal_conv_backward(yt, xs[:, -50:].contiguous(), cw, activation="silu", state=xs[:, -53:-50].contiguous())[0]
+    assert torch.equal(dxc[:, -50:], dxt)
+    del dxc, dxt
+
+
+def test_scan_offsets_past_32_bits():
+    D, S = 1032, 4
+    L = (1 << 31) // D + 77
+    g = torch.Generator("cuda").manual_seed(3)
+    u = torch.randn(1, L, D, device="cuda", dtype=torch.float16, generator=g)
+    bc = torch.randn(1, L, 2 * S, device="cuda", dtype=torch.float16, generator=g)
+    A = -(torch.rand(D, S, device="cuda", generator=g) + 0.1)
+    args = (u, u, A, bc[..., :S], bc[..., S:])
+    n = 96
+    y, last, saved = seq.selective_scan(*args, training=True)
+    front = seq.selective_scan(*(t if t is A else t[:, :-n] for t in args))[1]
+    cut = [t if t is A else t[:, -n:] for t in args]
+    yt, lt, st = seq.selective_scan(*cut, state=front, training=True)
+    # the chunks' borders lie elsewhere: a state may differ by the roundings of the rows since one (a few hundred, 2^-24 each)
+    assert float((last - lt).abs().max()) <= 1e-4 * float(lt.abs().max())
+    assert float((y[:, -n:].float() - yt.float()).abs().max()) <= 2.0 ** -9 * float(yt.float().abs().max())
+    d, dt_ = seq.selective_scan_backward(u, *args, saved), seq.selective_scan_backward(u[:, -n:], *cut, st)
+    for a, b in ((d.du, dt_.du), (d.ddt, dt_.ddt), (d.dB, dt_.dB), (d.dC, dt_.dC)):
+        assert float((a[:, -n:].float() - b.float()).abs().max()) <= 2.0 ** -9 * float(b.float().abs().max())
+
+
+def test_a_stream_that_is_not_the_operands_own():
+    """Operands made on one stream, the call on another that waits for it: what every operator promises is its tensors' device's current
+    stream."""
+    g = gen(51)
+    x, w = rnd(g, 300, 256, dtype=torch.float16).cuda(), rnd(g, 320, 256, dtype=torch.float16).cuda()
+    want = seq.linear(x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = seq.linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_profiled_launches_are_the_same_launches():
+    KernelProfile = importlib.import_module("tf-1d-2d-segmentation-end2endpipelines_amd.ops").KernelProfile
+    x = torch.randn(40, 64, generator=gen(52)).cuda()
+    want = seq.layer_norm(x)
+    KernelProfile.on, KernelProfile.records = True, []
+    try:
+        got = seq.layer_norm(x)
+        assert [r[0] for r in KernelProfile.records] == ["seg_layernorm_fwd"]
+    finally:
+        KernelProfile.on, KernelProfile.records = False, []
+    assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------------------------------------- difference quotients
+def directional(loss, args, grads, g, names):
+    """Every gradient along a random direction against the central difference of the 64-bit loss: the quotient is off by step^2 of a third
+    derivative of order one (1e-8) and by the loss' rounding over the step (1e-16 / 1e-4); the gradient by its 32-bit sums - 1e-4 of the
+    sum of its terms' absolute values covers both."""
+    for n in names:
+        v = torch.randn(args[n].shape, generator=g).double()
+        up, down = dict(args), dict(args)
+        up[n], down[n] = args[n] + 1e-4 * v, args[n] - 1e-4 * v
+        quotient = (float(loss(up)) - float(loss(down))) / 2e-4
+        got = grads[n].double().cpu()
+        assert abs(float((got * v).sum()) - quotient) <= 1e-4 * float((got * v).abs().sum()), (n, float((got * v).sum()), quotient)
+
+
+def test_gradients_are_difference_quotients():
+    g = gen(61)
+    # layer normalisation
+    x, dy, gamma, beta = rnd(g, 9, 40), rnd(g, 9, 40), torch.rand(40, generator=g) + 0.5, rnd(g, 40)
+    _y, mean, rstd = seq.layer_norm(x.cuda(), gamma.cuda(), beta.cuda(), stats=True)
+    dx, dg, db = seq.layer_norm_backward(dy.cuda(), x.cuda(), mean, rstd, gamma.cuda())
+
+    def ln(a):
+        m = a["x"].mean(1, keepdim=True)
+        return (((a["x"] - m) * (((a["x"] - m) ** 2).mean(1, keepdim=True) + 1e-3) ** -0.5 * a["gamma"] + a["beta"]) * dy.double()).sum()
+    directional(ln, dict(x=x.double(), gamma=gamma.double(), beta=beta.double()), dict(x=dx, gamma=dg, beta=db), g, ("x", "gamma", "beta"))
+    # causal convolution, the state that goes on among the outputs
+    B, L, D, K = 2, 21, 12, 4
+    a = dict(x=rnd(g, B, L, D), w=rnd(g, K, D), bias=rnd(g, D), state=rnd(g, B, K - 1, D))
+    dy, dst, lengths = rnd(g, B, L, D), rnd(g, B, K - 1, D), torch.tensor([L, 13], dtype=torch.int32)
+    c = {k: t.cuda() for k, t in a.items()}
+    got = seq.causal_conv_backward(dy.cuda(), c["x"], c["w"], c["bias"], activation="silu", state=c["state"], lengths=lengths.cuda(), dstate=dst.cuda())
+
+    def conv(a):
+        y, st = R.conv(a["x"], a["w"], a["bias"], a["state"], lengths, True)
+        return (y * dy.double()).sum() + (st * dst.double()).sum()
+    directional(conv, {k: t.double() for k, t in a.items()}, dict(zip(("x", "w", "bias", "state"), got)), g, ("x", "w", "bias", "state"))
+    # scan, the last state among the outputs
+    B, L, D, S = 2, 70, 12, 8
+    i, dy, dst, g = scan_inputs(62, B, L, D, S, torch.float32)
+    lengths = torch.tensor([L, 41], dtype=torch.int32)
+    c = {k: t.cuda() for k, t in i.items()}
+    state = c.pop("state")
+    _y, _l, saved = seq.selective_scan(**c, state=state, lengths=lengths.cuda(), training=True)
+    d = seq.selective_scan_backward(dy.cuda(), c["u"], c["dt"], c["A"], c["B"], c["C"], saved, D=c["D"], z=c["z"], dt_bias=c["dt_bias"], lengths=lengths.cuda(),
+                                    dstate=dst.cuda())
+
+    def scan(a):
+        y, last = R.scan(**a, lengths=lengths)
+        return (y * dy.double()).sum() + (last * dst.double()).sum()
+    directional(scan, {k: t.double() for k, t in i.items()},
+                dict(u=d.du, dt=d.ddt, A=d.dA, B=d.dB, C=d.dC, D=d.dD, z=d.dz, dt_bias=d.ddt_bias, state=d.dstate), g,
+                ("u", "dt", "A", "B", "C", "D", "z", "dt_bias", "state"))

@@ -76,19 +76,19 @@ __device__ __forceinline__ void store_sums(const GemmArgs& p, const f16v& acc, i
 template <typename T> struct AnyStep { static constexpr int BK = 32, EPT = 8, LD = 40; };
 template <> struct AnyStep<float> { static constexpr int BK = 16, EPT = 4, LD = 20; };
 
-template <typename T, int VEC> __device__ __forceinline__ void load_elems(const T* p, int64_t n, T* r) {
+// 16 bytes of elements, kept in their memory format until they are put into the LDS (unpacked earlier they would be waited for earlier)
+template <typename T, int VEC> __device__ __forceinline__ u4 load_elems(const T* p) {
   constexpr int EPT = AnyStep<T>::EPT;
-  typedef T vec __attribute__((ext_vector_type(VEC)));
-  if (VEC > 1 && n >= EPT) {
-#pragma unroll
-    for (int q = 0; q < EPT / VEC; ++q) {
-      const vec v = *reinterpret_cast<const vec*>(p + q * VEC);
-#pragma unroll
-      for (int t = 0; t < VEC; ++t) r[q * VEC + t] = v[t];
-    }
+  if constexpr (VEC == EPT) return ld16(p);
+  else if constexpr (VEC * sizeof(T) == 8) {
+    const u2 a = *reinterpret_cast<const u2*>(p), b = *reinterpret_cast<const u2*>(p + VEC);
+    return u4{a[0], a[1], b[0], b[1]};
   } else {
+    typedef T tv __attribute__((ext_vector_type(EPT)));
+    tv v;
 #pragma unroll
-    for (int t = 0; t < EPT; ++t) r[t] = t < n ? p[t] : (T)0.f;
+    for (int t = 0; t < EPT; ++t) v[t] = p[t];
+    return __builtin_bit_cast(u4, v);
   }
 }
 
@@ -104,25 +104,34 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   const int64_t kbeg = blockIdx.y * p.kper, kend = kbeg + p.kper < p.Kd ? kbeg + p.kper : p.Kd;
   constexpr int KCH = S::BK / S::EPT, ICH = 64 / S::EPT;       // chunks per k-contiguous / i-contiguous row
   const T *A = (const T*)p.A, *B = (const T*)p.B;
-  T ra[S::EPT], rb[S::EPT];
-  auto fetch = [&](const T* base, int64_t ld, bool kc, int64_t r0, int64_t rend, int64_t k, T* r) {
-    if (kc) {
-      const int64_t row = r0 + tid / KCH, kk = k + (tid % KCH) * S::EPT;
-      load_elems<T, VEC>(base + row * ld + kk, row < rend ? kend - kk : 0, r);
-    } else {
-      const int64_t kk = k + tid / ICH, row = r0 + (tid % ICH) * S::EPT;
-      load_elems<T, VEC>(base + kk * ld + row, kk < kend ? rend - row : 0, r);
-    }
+  typedef T tv __attribute__((ext_vector_type(S::EPT)));
+  u4 ra[2], rb[2];                                             // two steps on their way
+  // A whole step's chunk without a branch: a row that is not there is read from the last one (its results are dropped), and a chunk along
+  // i / j lies inside the operand where the tile does.  (Guards here cost the prefetch: the compiler waits for the loads where the guarded
+  // and the unguarded path meet - 22 us instead of 10 for 1111 x 333 x 700, f16.)
+  auto fetch = [&](const T* base, int64_t ld, bool kc, int64_t r0, int64_t rend, int64_t k) -> u4 {
+    const int64_t row = r0 + tid / KCH;
+    return kc ? load_elems<T, VEC>(base + (row < rend ? row : rend - 1) * ld + k + (tid % KCH) * S::EPT)
+              : load_elems<T, VEC>(base + (k + tid / ICH) * ld + r0 + (tid % ICH) * S::EPT);
   };
-  auto put = [&](T* s, bool kc, const T* r) {
-    if (kc) {
-      T* d = s + (tid / KCH) * S::LD + (tid % KCH) * S::EPT;
+  // element by element, what is not there reads as zero: the end of k, and tiles that reach over the operand's columns
+  auto fetch_edge = [&](const T* base, int64_t ld, bool kc, int64_t r0, int64_t rend, int64_t k) -> u4 {
+    const int64_t row = kc ? r0 + tid / KCH : r0 + (tid % ICH) * S::EPT, kk = kc ? k + (tid % KCH) * S::EPT : k + tid / ICH;
+    const T* p0 = kc ? base + row * ld + kk : base + kk * ld + row;
+    const int64_t n = kc ? (row < rend ? kend - kk : 0) : (kk < kend ? rend - row : 0);
+    tv r;
 #pragma unroll
-      for (int e = 0; e < S::EPT; ++e) d[e] = r[e];
+    for (int t = 0; t < S::EPT; ++t) r[t] = t < n ? p0[t] : (T)0.f;
+    return __builtin_bit_cast(u4, r);
+  };
+  auto put = [&](T* s, bool kc, u4 r) {
+    if (kc) {
+      st16(s + (tid / KCH) * S::LD + (tid % KCH) * S::EPT, r);
     } else {
+      const tv v = __builtin_bit_cast(tv, r);
       T* d = s + (tid % ICH) * S::EPT * S::LD + tid / ICH;
 #pragma unroll
-      for (int e = 0; e < S::EPT; ++e) d[e * S::LD] = r[e];
+      for (int e = 0; e < S::EPT; ++e) d[e * S::LD] = v[e];
     }
   };
   f16v acc, accb;
@@ -131,17 +140,7 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
   // the sums of dy's columns ride on the first tile column's waves as one more product, with ones
   const bool sums = PASS == SEG_LINEAR_BWD_WEIGHT && p.db != nullptr && j0 == 0 && wj == 0;
-  fetch(A, p.a_ld, AKC, i0, p.I, kbeg, ra);
-  fetch(B, p.b_ld, BKC, j0, p.J, kbeg, rb);
-  int buf = 0;
-  for (int64_t k = kbeg; k < kend; k += S::BK, buf ^= 1) {
-    put(smem[buf][0], AKC, ra);
-    put(smem[buf][1], BKC, rb);
-    __syncthreads();
-    if (k + S::BK < kend) {
-      fetch(A, p.a_ld, AKC, i0, p.I, k + S::BK, ra);
-      fetch(B, p.b_ld, BKC, j0, p.J, k + S::BK, rb);
-    }
+  auto step = [&](int buf) {                                   // (buf is a literal at every call: the registers are named at compile time)
     const T *sa = smem[buf][0] + (wi + fr) * S::LD, *sb = smem[buf][1] + (wj + fr) * S::LD;
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
@@ -158,7 +157,44 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
         for (int ks = 0; ks < 2; ++ks) accb = mfma16<T>(ld16(sa + ks * 16 + fh * 8), ones16<T>(), accb);
       }
     }
-    // the buffer written next is the one whose readers passed the barrier above
+  };
+  auto stage = [&](int buf) {                                  // (the buffer written next is the one whose readers passed the barrier)
+    put(smem[buf][0], AKC, ra[buf]);
+    put(smem[buf][1], BKC, rb[buf]);
+    __syncthreads();
+  };
+  const bool inside = (AKC || i0 + 64 <= p.I) && (BKC || j0 + 64 <= p.J);
+  const int64_t kfull = inside ? kbeg + (kend - kbeg) / S::BK * S::BK : kbeg;
+  auto fetch2 = [&](int set, int64_t k) {
+    ra[set] = fetch(A, p.a_ld, AKC, i0, p.I, k);
+    rb[set] = fetch(B, p.b_ld, BKC, j0, p.J, k);
+  };
+  int64_t k = kbeg;
+  if (kbeg < kfull) {
+    const int64_t last = kfull - S::BK;                        // (steps behind the last one fetch it again: no branch)
+    fetch2(0, kbeg);
+    fetch2(1, kbeg + S::BK < last ? kbeg + S::BK : last);
+    for (; k + S::BK < kfull; k += 2 * S::BK) {
+      stage(0);
+      fetch2(0, k + 2 * S::BK < last ? k + 2 * S::BK : last);
+      step(0);
+      stage(1);
+      fetch2(1, k + 3 * S::BK < last ? k + 3 * S::BK : last);
+      step(1);
+    }
+  }
+  if (k < kfull) {
+    stage(0);
+    step(0);
+    k += S::BK;
+    __syncthreads();
+  }
+  for (; k < kend; k += S::BK) {
+    ra[0] = fetch_edge(A, p.a_ld, AKC, i0, p.I, k);
+    rb[0] = fetch_edge(B, p.b_ld, BKC, j0, p.J, k);
+    stage(0);
+    step(0);
+    __syncthreads();                                           // (one buffer here)
   }
   if (sums) store_sums(p, accb, i0 + wi, lane);
   const int j = j0 + wj + fr;
@@ -575,9 +611,10 @@ inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   g.ti = (int)((I + side - 1) / side);
   g.tj = (J + side - 1) / side;
   const int64_t tiles = (int64_t)g.ti * g.tj, room = g.kind == TILE_256 ? 256 : g.kind == TILE_128 ? 512 : 1024;
-  // fewer tiles than the card has room for: k is split, down to 256 of it per block
+  // fewer tiles than the card has room for: k is split, down to 512 of it per block (a second launch joins the parts: 1111 x 333 x 700,
+  // f16, in one launch took SPLITNOTE)
   int64_t s = tiles * 2 > room || tiles == 0 ? 1 : room / tiles;
-  if (s > Kd / 256) s = Kd / 256;
+  if (s > Kd / 512) s = Kd / 512;
   if (s > 32) s = 32;
   if (s < 1) s = 1;
   const int64_t step = g.kind != TILE_ANY ? 64 : dtype == SEG_DT_F32 ? 16 : 32;
