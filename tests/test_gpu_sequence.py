@@ -236,6 +236,25 @@ def test_linear_large_tiles(dtype):
     assert torch.equal(dw, seq.linear_backward(dy, x, torch.zeros(N, K, dtype=dtype, device="cuda"), need_dx=False, need_db=False)[1])
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+def test_linear_large_and_odd(dtype):
+    """Large products of operands that no 16-byte access fits - odd sizes, slices at odd columns with NaN beside them."""
+    g = gen(15)
+    M, N, K = 8200, 519, 523
+    x, w, b, r, z = (rnd(g, *s, dtype=t).cuda() for s, t in (((M, K), dtype), ((N, K), dtype), ((N,), torch.float32), ((M, N), dtype), ((M, K), dtype)))
+    dy = r
+    for X, W, DY in ((x, w, dy), (wide(x, 3, 2), wide(w, 1, 4), wide(dy, 5, 0))):
+        y, pre = seq.linear(X, W, b, activation="silu", residual=r, preactivation=True)
+        z64, s = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t() + b.double().abs()
+        R.assert_close(pre, z64.cpu(), s.cpu(), K + 4, "z")
+        R.assert_close(y, (R.act(z64, "silu") + r.double()).cpu(), (1.13 * s + r.double().abs() + z64.abs() + 1).cpu(), K + 24, "y")
+        dx, dw, db = seq.linear_backward(DY, X, W, z=z, activation="silu")
+        p, s = dy.double() @ w.double(), dy.double().abs() @ w.double().abs()
+        R.assert_close(dx, (p * R.act_slope(z.double(), "silu")).cpu(), (1.13 * s + p.abs() * (1 + z.double().abs())).cpu(), N + 24, "dx")
+        R.assert_close(dw, (dy.double().t() @ x.double()).cpu(), (dy.double().abs().t() @ x.double().abs()).cpu(), M, "dw")
+        R.assert_close(db, dy.double().sum(0).cpu(), dy.double().abs().sum(0).cpu(), M, "db")
+
+
 def test_linear_no_rows_and_leading_axes():
     w = torch.randn(6, 10, generator=gen(1)).cuda()
     y = seq.linear(torch.empty(0, 10, device="cuda"), w)

@@ -11,6 +11,9 @@
 namespace {
 
 constexpr int TPB = 256;
+typedef short s4v __attribute__((__vector_size__(4 * sizeof(short))));
+typedef __attribute__((address_space(3))) s4v* lds_s4v_ptr;
+typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
 
 struct GemmArgs {
   const void *A, *B;
@@ -20,7 +23,8 @@ struct GemmArgs {
   int ti, tj;                    // tiles along i and j
   int splits;                    // ranges of k contracted by different blocks
   int64_t kper;                  // their length (a multiple of the K step)
-  float* part;                   // [splits][I][J] when splits > 1
+  float* part;                   // [splits][I][jp] when splits > 1
+  int jp;                        // J in whole pieces of 8
   int act;
   float alpha;
   const float* bias;
@@ -70,11 +74,12 @@ __device__ __forceinline__ void store_sums(const GemmArgs& p, const f16v& acc, i
   }
 }
 
-// ---- the kernel for every size, stride and type: 64 x 64 tiles, operands through registers into k-contiguous LDS rows (an operand
-// whose memory is contiguous along i / j is transposed on its way), four waves of one 32 x 32 tile each.  VEC: elements per memory
-// access - what the addresses' alignment allows; the ends of rows and of k go element by element.
-template <typename T> struct AnyStep { static constexpr int BK = 32, EPT = 8, LD = 40; };
-template <> struct AnyStep<float> { static constexpr int BK = 16, EPT = 4, LD = 20; };
+// ---- the kernel for every size, stride and type: 64 x 64 tiles, four waves of one 32 x 32 tile each, operands through registers into the
+// LDS in the order they have in memory - rows of BK along k (LD elements apart), or BK rows of 64 along i / j (LDT apart: the four rows of
+// a transposing 16-bit read fall into four 64-byte quarters of the banks; 32-bit fragments are single elements either way).  VEC: elements
+// per memory access - what the addresses' alignment allows; the ends of rows and of k go element by element.
+template <typename T> struct AnyStep { static constexpr int BK = 32, EPT = 8, LD = 40, LDT = 96, SIZE = 32 * 96; };
+template <> struct AnyStep<float> { static constexpr int BK = 16, EPT = 4, LD = 20, LDT = 68, SIZE = 64 * 20; };
 
 // 16 bytes of elements, kept in their memory format until they are put into the LDS (unpacked earlier they would be waited for earlier)
 template <typename T, int VEC> __device__ __forceinline__ u4 load_elems(const T* p) {
@@ -96,7 +101,8 @@ template <int PASS, typename T, int VEC>
 __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   typedef AnyStep<T> S;
   constexpr bool AKC = PASS != SEG_LINEAR_BWD_WEIGHT, BKC = PASS == SEG_LINEAR_FWD;
-  __shared__ __align__(16) T smem[2][2][64 * S::LD];
+  static_assert(S::SIZE >= 64 * S::LD && S::SIZE >= S::BK * S::LDT, "either order fits");
+  __shared__ __align__(16) T smem[2][2][S::SIZE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 31, fh = lane >> 5;
   const int t = xcd_remap(blockIdx.x, p.ti * p.tj);
   const int64_t i0 = (int64_t)(t / p.tj) * 64;
@@ -106,13 +112,14 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   const T *A = (const T*)p.A, *B = (const T*)p.B;
   typedef T tv __attribute__((ext_vector_type(S::EPT)));
   u4 ra[2], rb[2];                                             // two steps on their way
-  // A whole step's chunk without a branch: a row that is not there is read from the last one (its results are dropped), and a chunk along
-  // i / j lies inside the operand where the tile does.  (Guards here cost the prefetch: the compiler waits for the loads where the guarded
+  // A whole step's chunk without a branch: a row that is not there is read from the last one (its results are dropped), and so
+  // is a chunk along i / j where chunks lie inside the operand or outside as a whole.  (Guards here cost the prefetch: the compiler waits for the loads where the guarded
   // and the unguarded path meet - 22 us instead of 10 for 1111 x 333 x 700, f16.)
   auto fetch = [&](const T* base, int64_t ld, bool kc, int64_t r0, int64_t rend, int64_t k) -> u4 {
     const int64_t row = r0 + tid / KCH;
+    const int64_t col = r0 + (tid % ICH) * S::EPT;
     return kc ? load_elems<T, VEC>(base + (row < rend ? row : rend - 1) * ld + k + (tid % KCH) * S::EPT)
-              : load_elems<T, VEC>(base + (k + tid / ICH) * ld + r0 + (tid % ICH) * S::EPT);
+              : load_elems<T, VEC>(base + (k + tid / ICH) * ld + (col < rend ? col : rend - S::EPT));
   };
   // element by element, what is not there reads as zero: the end of k, and tiles that reach over the operand's columns
   auto fetch_edge = [&](const T* base, int64_t ld, bool kc, int64_t r0, int64_t rend, int64_t k) -> u4 {
@@ -125,15 +132,18 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
     return __builtin_bit_cast(u4, r);
   };
   auto put = [&](T* s, bool kc, u4 r) {
-    if (kc) {
-      st16(s + (tid / KCH) * S::LD + (tid % KCH) * S::EPT, r);
-    } else {
-      const tv v = __builtin_bit_cast(tv, r);
-      T* d = s + (tid % ICH) * S::EPT * S::LD + tid / ICH;
-#pragma unroll
-      for (int e = 0; e < S::EPT; ++e) d[e * S::LD] = v[e];
-    }
+    st16(kc ? s + (tid / KCH) * S::LD + (tid % KCH) * S::EPT : s + (tid / ICH) * S::LDT + (tid % ICH) * S::EPT, r);
   };
+  // a wave's 32 rows from row0, k step ks
+  auto frag = [&](const T* s, bool kc, int row0, int ks) -> u4 {
+    if (kc) return ld16(s + (row0 + fr) * S::LD + ks * 16 + fh * 8);
+    const int tg = lane >> 4, tt = lane & 15;
+    const T* a = s + (ks * 16 + 8 * (tg >> 1) + (tt >> 2)) * S::LDT + row0 + 16 * (tg & 1) + 4 * (tt & 3);
+    const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_ptr)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_ptr)(a + 4 * S::LDT));
+    const u2 l = __builtin_bit_cast(u2, lo), h = __builtin_bit_cast(u2, hi);
+    return u4{l[0], l[1], h[0], h[1]};
+  };
+  auto elem = [&](const T* s, bool kc, int row0, int k) -> T { return kc ? s[(row0 + fr) * S::LD + k] : s[k * S::LDT + row0 + fr]; };
   f16v acc, accb;
 #pragma unroll
   for (int q = 0; q < 16; ++q) acc[q] = accb[q] = 0.f;
@@ -141,20 +151,20 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   // the sums of dy's columns ride on the first tile column's waves as one more product, with ones
   const bool sums = PASS == SEG_LINEAR_BWD_WEIGHT && p.db != nullptr && j0 == 0 && wj == 0;
   auto step = [&](int buf) {                                   // (buf is a literal at every call: the registers are named at compile time)
-    const T *sa = smem[buf][0] + (wi + fr) * S::LD, *sb = smem[buf][1] + (wj + fr) * S::LD;
+    const T *sa = smem[buf][0], *sb = smem[buf][1];
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-      for (int ks = 0; ks < S::BK / 2; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(sa[2 * ks + fh], sb[2 * ks + fh], acc, 0, 0, 0);
-      if (sums) {
-#pragma unroll
-        for (int ks = 0; ks < S::BK / 2; ++ks) accb = __builtin_amdgcn_mfma_f32_32x32x2f32(sa[2 * ks + fh], 1.f, accb, 0, 0, 0);
+      for (int ks = 0; ks < S::BK / 2; ++ks) {
+        const float a = elem(sa, AKC, wi, 2 * ks + fh);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, elem(sb, BKC, wj, 2 * ks + fh), acc, 0, 0, 0);
+        if (PASS == SEG_LINEAR_BWD_WEIGHT && sums) accb = __builtin_amdgcn_mfma_f32_32x32x2f32(a, 1.f, accb, 0, 0, 0);
       }
     } else {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) acc = mfma16<T>(ld16(sa + ks * 16 + fh * 8), ld16(sb + ks * 16 + fh * 8), acc);
-      if (sums) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) accb = mfma16<T>(ld16(sa + ks * 16 + fh * 8), ones16<T>(), accb);
+      for (int ks = 0; ks < 2; ++ks) {
+        const u4 a = frag(sa, AKC, wi, ks);
+        acc = mfma16<T>(a, frag(sb, BKC, wj, ks), acc);
+        if (PASS == SEG_LINEAR_BWD_WEIGHT && sums) accb = mfma16<T>(a, ones16<T>(), accb);
       }
     }
   };
@@ -163,7 +173,7 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
     put(smem[buf][1], BKC, rb[buf]);
     __syncthreads();
   };
-  const bool inside = (AKC || i0 + 64 <= p.I) && (BKC || j0 + 64 <= p.J);
+  const bool inside = (AKC || i0 + 64 <= p.I || p.I % S::EPT == 0) && (BKC || j0 + 64 <= p.J || p.J % S::EPT == 0);
   const int64_t kfull = inside ? kbeg + (kend - kbeg) / S::BK * S::BK : kbeg;
   auto fetch2 = [&](int set, int64_t k) {
     ra[set] = fetch(A, p.a_ld, AKC, i0, p.I, k);
@@ -203,7 +213,7 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
     for (int q = 0; q < 16; ++q) {
       const int64_t i = i0 + wi + (q & 3) + 8 * (q >> 2) + 4 * fh;
       if (i < p.I) {
-        if (p.splits > 1) p.part[((int64_t)blockIdx.y * p.I + i) * p.J + j] = acc[q];
+        if (p.splits > 1) p.part[((int64_t)blockIdx.y * p.I + i) * p.jp + j] = acc[q];
         else epilogue1<PASS, T>(p, i, j, acc[q]);
       }
     }
@@ -218,9 +228,6 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
 // bytes keep chunk c of row r at c ^ ((r >> 1) & 7) (c ^ ((r >> 2) & 3)), so that the 16 rows a ds_read_b128 group touches lie on 16
 // different 16-byte slots; rows of one k keep it at c ^ ((k & 3) << 2), so that the four k rows of a transposing read lie in four
 // different 64-byte quarters.
-typedef short s4v __attribute__((__vector_size__(4 * sizeof(short))));
-typedef __attribute__((address_space(3))) s4v* lds_s4v_ptr;
-typedef __attribute__((address_space(3))) unsigned char* lds_byte_ptr;
 
 template <int BK> __device__ __forceinline__ int row_swizzle(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
 
@@ -241,7 +248,7 @@ template <bool KC, int ROWS, int BK, int NWV> struct TileLoader {
       constexpr int CPR = BK / 8, RPI = 64 / CPR;              // 16-byte chunks per row, rows per instruction
       static_assert(BK == 32 || NI % 2 == 0, "the swizzle of an instruction depends on its parity only");
       base = (const unsigned char*)ptr + r0 * ld2;
-      rsrc = make_rsrc(base, (int)((rows - 1) * ld2 + Kd * 2));          // rows behind the operand's end start behind this
+      rsrc = make_rsrc(base, (int)((rows - 1) * ld2 + (Kd + 7) / 8 * 16));          // rows behind the operand's end start behind this
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = (wave * NI + i) * RPI + lane / CPR;
@@ -251,7 +258,7 @@ template <bool KC, int ROWS, int BK, int NWV> struct TileLoader {
       }
     } else {
       base = (const unsigned char*)ptr + r0 * 2;
-      cols2 = (int)left * 2;
+      cols2 = ((int)left * 2 + 3) / 4 * 4;                     // (bounds are checked by 4 bytes)
       constexpr int RPI = 512 / ROWS, LPR = 64 / RPI;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -296,15 +303,17 @@ template <bool KC, int ROWS, int BK> __device__ __forceinline__ u4 tile_frag(con
     return u4{l[0], l[1], h[0], h[1]};
   }
 }
-// eight neighbouring elements of the result through the pass's epilogue; f: the row of z (bwd_data), r: of the residual, fetched before
+// eight neighbouring elements of the result (n of them exist; vec: all, and 16-byte accesses fit) through the pass's epilogue; f: the row
+// of z (bwd_data), r: of the residual, fetched before
 template <int PASS, typename T> __device__ __forceinline__ void epilogue8(const GemmArgs& p, int64_t i, int j, const float* bias, float* v, const float* f,
-                                                                          const float* r, bool vec) {
+                                                                          const float* r, int n, bool vec) {
   if constexpr (PASS == SEG_LINEAR_BWD_WEIGHT) {
     float* o = (float*)p.out + i * p.out_ld + j;
     if (vec) store8<float>(o, v);
     else {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) o[t] = v[t];
+      for (int t = 0; t < 8; ++t)
+        if (t < n) o[t] = v[t];
     }
   } else {
     if constexpr (PASS == SEG_LINEAR_FWD) {
@@ -312,7 +321,7 @@ template <int PASS, typename T> __device__ __forceinline__ void epilogue8(const 
       for (int t = 0; t < 8; ++t) v[t] += bias[t];
       if (p.z != nullptr) {
         if (vec) row_store8<T, true>((T*)p.z + i * p.z_ld + j, 8, v);
-        else row_store8<T, false>((T*)p.z + i * p.z_ld + j, 8, v);
+        else row_store8<T, false>((T*)p.z + i * p.z_ld + j, n, v);
       }
       act8(v, p.act, p.alpha);
     } else if (p.z != nullptr) {
@@ -323,17 +332,17 @@ template <int PASS, typename T> __device__ __forceinline__ void epilogue8(const 
       for (int t = 0; t < 8; ++t) v[t] += r[t];
     }
     if (vec) row_store8<T, true>((T*)p.out + i * p.out_ld + j, 8, v);
-    else row_store8<T, false>((T*)p.out + i * p.out_ld + j, 8, v);
+    else row_store8<T, false>((T*)p.out + i * p.out_ld + j, n, v);
   }
 }
 template <typename T> struct Row8 {                            // eight elements of a row in their memory format
   typedef T tv __attribute__((ext_vector_type(8)));
   tv v;
-  __device__ __forceinline__ void load(const T* p, bool vec) {
+  __device__ __forceinline__ void load(const T* p, int n, bool vec) {
     if (vec) v = *reinterpret_cast<const tv*>(p);
     else {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) v[t] = p[t];
+      for (int t = 0; t < 8; ++t) v[t] = t < n ? p[t] : (T)0.f;
     }
   }
   __device__ __forceinline__ void get(float* f) const {
@@ -433,19 +442,20 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
   ring_release_barrier();
   float* slab = reinterpret_cast<float*>(smem + wave * SLAB);
   const int fr = lane & 31, fh = lane >> 5;
-  const bool vec = p.vecio != 0;
+  const bool vecio = p.vecio != 0;
   // what the epilogue reads (z of bwd_data, the residual) is fetched a 32 x 64 piece ahead of its use
   constexpr int PIECES = TN / 2 * TM;
   constexpr bool READS = PASS != SEG_LINEAR_BWD_WEIGHT;
   Row8<T> zr[2][4], rr[2][4];
   auto fetch = [&](int u) {
-    const int j = j0 + wc + (u / TM) * 64 + (lane & 7) * 8;
+    const int j = j0 + wc + (u / TM) * 64 + (lane & 7) * 8, n = p.J - j;
+    const bool vec = vecio && n >= 8;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int64_t i = i0 + wr + (u % TM) * 32 + (lane >> 3) + r * 8;
       if (j < p.J && i < p.I && p.splits == 1) {
-        if (PASS == SEG_LINEAR_BWD_DATA && p.z != nullptr) zr[u & 1][r].load((const T*)p.z + i * p.z_ld + j, vec);
-        if (p.res != nullptr) rr[u & 1][r].load((const T*)p.res + i * p.res_ld + j, vec);
+        if (PASS == SEG_LINEAR_BWD_DATA && p.z != nullptr) zr[u & 1][r].load((const T*)p.z + i * p.z_ld + j, n, vec);
+        if (p.res != nullptr) rr[u & 1][r].load((const T*)p.res + i * p.res_ld + j, n, vec);
       }
     }
   };
@@ -455,10 +465,11 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
   for (int u = 0; u < PIECES; ++u) {
     const int bp = u / TM, a = u % TM;
     const int j = j0 + wc + bp * 64 + (lane & 7) * 8;
-    const bool jn = j < p.J;
+    const int n = p.J - j;
+    const bool jn = n > 0, vec = vecio && n >= 8;
     if (a == 0) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) bias[q] = (PASS == SEG_LINEAR_FWD && p.bias != nullptr && jn) ? p.bias[j + q] : 0.f;
+      for (int q = 0; q < 8; ++q) bias[q] = (PASS == SEG_LINEAR_FWD && p.bias != nullptr && q < n) ? p.bias[j + q] : 0.f;
     }
     if constexpr (READS) {
       if (u + 1 < PIECES) fetch(u + 1);
@@ -475,15 +486,30 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
       load8<float>(slab + ((lane >> 3) + r * 8) * 68 + (lane & 7) * 8, v);
       if (i < p.I && jn) {
         if (p.splits > 1) {
-          store8<float>(p.part + ((int64_t)blockIdx.y * p.I + i) * p.J + j, v);
+          store8<float>(p.part + ((int64_t)blockIdx.y * p.I + i) * p.jp + j, v);         // (whole pieces: jp)
         } else {
           if (PASS == SEG_LINEAR_BWD_DATA && p.z != nullptr) zr[u & 1][r].get(f);
           if (READS && p.res != nullptr) rr[u & 1][r].get(g);
-          epilogue8<PASS, T>(p, i, j, bias, v, f, g, vec);
+          epilogue8<PASS, T>(p, i, j, bias, v, f, g, n, vec);
         }
       }
     }
     __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ---- a copy of an operand whose rows no 16-byte access fits, in rows of whole 16 bytes with zeros at their ends
+template <typename T>
+__global__ __launch_bounds__(TPB) void pack_rows_kernel(const T* x, int64_t ld, int64_t rows, int64_t cols, T* o, int64_t ld8) {
+  const int64_t n = rows * (ld8 / 8);
+  for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < n; e += (int64_t)gridDim.x * TPB) {
+    const int64_t r = e / (ld8 / 8), c = (e - r * (ld8 / 8)) * 8;
+    typedef T tv __attribute__((ext_vector_type(8)));
+    tv v;
+    const T* p = x + r * ld + c;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] = c + t < cols ? p[t] : (T)0.f;
+    *reinterpret_cast<tv*>(o + r * ld8 + c) = v;
   }
 }
 
@@ -556,9 +582,10 @@ __global__ __launch_bounds__(TPB) void gemm_join_kernel(const GemmArgs p) {
       p.db[e - n] = v;
       continue;
     }
-    for (int s = 0; s < p.splits; ++s) v += p.part[s * n + e];
     const int64_t i = e / p.J;
-    epilogue1<PASS, T>(p, i, (int)(e - i * p.J), v);
+    const int j = (int)(e - i * p.J);
+    for (int s = 0; s < p.splits; ++s) v += p.part[(s * p.I + i) * p.jp + j];
+    epilogue1<PASS, T>(p, i, j, v);
   }
 }
 
@@ -612,7 +639,7 @@ inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   g.tj = (J + side - 1) / side;
   const int64_t tiles = (int64_t)g.ti * g.tj, room = g.kind == TILE_256 ? 256 : g.kind == TILE_128 ? 512 : 1024;
   // fewer tiles than the card has room for: k is split, down to 512 of it per block (a second launch joins the parts: 1111 x 333 x 700,
-  // f16, in one launch took SPLITNOTE)
+  // f16: 14 us in one launch, 16 in two)
   int64_t s = tiles * 2 > room || tiles == 0 ? 1 : room / tiles;
   if (s > Kd / 512) s = Kd / 512;
   if (s > 32) s = 32;
@@ -639,16 +666,36 @@ inline int vec_of(const void* A, int64_t a_ld, const void* B, int64_t b_ld, int 
   return 1;
 }
 
-// whether the operands of a pass suit the LDS-DMA tile kernels: 16-bit, 16-byte rows, offsets inside a tile below 2 GiB
-inline bool dma_ok(const seg_linear_args& a, int pass) {
-  if (a.dtype == SEG_DT_F32) return false;
+// What the LDS-DMA tile kernels take of a pass: 16-bit operands in 16-byte rows (k-contiguous ones also a whole number of 8 inputs),
+// offsets inside a tile below 2 GiB.  A product of 2^32 operations or more whose operands do not fit is worth a packed copy of them
+// (16384 x 4095 x 4095 f16: 2118 us without, 780 with copies; its backward pass 7473 and 1412).  dma: 0 no, 1 as they are, 2 with copies (a, b: which)
+struct Operand { const void* p; int64_t ld, rows, cols; bool kc; };
+struct DmaPlan { int dma; bool a, b; int64_t a_elems, b_elems; };
+inline Operand operand_a(const seg_linear_args& a, int pass) {
+  if (pass == SEG_LINEAR_BWD_WEIGHT) return {a.dy, a.dy_ld, a.M, a.N, false};
+  return {a.x, a.x_ld, a.M, a.K, true};
+}
+inline Operand operand_b(const seg_linear_args& a, int pass) {
+  if (pass == SEG_LINEAR_BWD_WEIGHT) return {a.x, a.x_ld, a.M, a.K, false};
+  return pass == SEG_LINEAR_FWD ? Operand{a.w, a.w_ld, a.N, a.K, true} : Operand{a.w, a.w_ld, a.K, a.N, false};
+}
+inline DmaPlan dma_plan(const seg_linear_args& a, int pass) {
+  DmaPlan d = {0, false, false, 0, 0};
   const Extents e = extents(a, pass);
-  const void *A = pass == SEG_LINEAR_BWD_WEIGHT ? a.dy : a.x, *B = pass == SEG_LINEAR_BWD_WEIGHT ? a.x : a.w;
-  const int64_t al = pass == SEG_LINEAR_BWD_WEIGHT ? a.dy_ld : a.x_ld, bl = pass == SEG_LINEAR_BWD_WEIGHT ? a.x_ld : a.w_ld;
-  if (!aligned16(A) || !aligned16(B) || al % 8 != 0 || bl % 8 != 0 || al > (1 << 21) || bl > (1 << 21) || al <= 0 || bl <= 0) return false;
-  if (e.J % 8 != 0 || (pass == SEG_LINEAR_BWD_WEIGHT ? e.I % 8 != 0 : e.Kd % 8 != 0) || (pass != SEG_LINEAR_BWD_WEIGHT && e.Kd >= (1 << 21))) return false;
-  // tiles far larger than the result waste the matrix cores
-  return e.I >= 64 && e.J >= 64;
+  // (tiles far larger than the result waste the matrix cores)
+  if (a.dtype == SEG_DT_F32 || e.I < 64 || e.J < 64 || e.Kd < 1) return d;
+  const Operand A = operand_a(a, pass), B = operand_b(a, pass);
+  if (A.ld > (1 << 21) || B.ld > (1 << 21) || A.cols > (1 << 21) || B.cols > (1 << 21)) return d;
+  auto fits = [](const Operand& o) { return aligned16(o.p) && o.ld % 8 == 0 && (!o.kc || o.cols % 8 == 0); };
+  d.a = !fits(A);
+  d.b = !fits(B);
+  if (!d.a && !d.b) { d.dma = 1; return d; }
+  if ((double)e.I * e.J * e.Kd < 2147483648.0) return d;
+  d.dma = 2;
+  auto elems = [](const Operand& o) { return o.rows * ((o.cols + 7) / 8 * 8); };
+  d.a_elems = d.a ? elems(A) : 0;
+  d.b_elems = d.b ? elems(B) : 0;
+  return d;
 }
 // up to 64 rows forward, every row of both operands in 16-byte pieces
 inline bool rows_ok(const seg_linear_args& a, int pass) {
@@ -659,7 +706,7 @@ inline bool rows_ok(const seg_linear_args& a, int pass) {
 inline GemmPlan plan_of(const seg_linear_args& a, int pass) {
   const Extents e = extents(a, pass);
   if (rows_ok(a, pass)) return {FEW_ROWS, 1, (e.J + 15) / 16, 1, e.Kd};
-  return gemm_plan(e.I, e.J, e.Kd, a.dtype, dma_ok(a, pass));
+  return gemm_plan(e.I, e.J, e.Kd, a.dtype, dma_plan(a, pass).dma != 0);
 }
 
 // bwd_weight: whether db is part of the product's launch, and the floats of the product's split sums (whole 16 bytes)
@@ -667,7 +714,21 @@ inline bool sums_ride(const seg_linear_args& a) { return a.dw != nullptr && plan
 inline int64_t weight_parts(const seg_linear_args& a) {
   const GemmPlan g = plan_of(a, SEG_LINEAR_BWD_WEIGHT);
   if (a.dw == nullptr || g.splits <= 1) return 0;
-  return ((int64_t)g.splits * a.N * (a.K + (a.db != nullptr && g.kind == TILE_ANY ? 1 : 0)) + 3) / 4 * 4;
+  return ((int64_t)g.splits * a.N * ((a.K + 7) / 8 * 8 + (a.db != nullptr && g.kind == TILE_ANY ? 1 : 0)) + 3) / 4 * 4;
+}
+
+inline int64_t gemm_parts(const seg_linear_args& a, int pass) {            // floats in front of the packed copies
+  if (pass == SEG_LINEAR_BWD_WEIGHT) return weight_parts(a) + (a.db != nullptr && !sums_ride(a) ? (colsum_plan(a.M, a.N).parts * a.N + 3) / 4 * 4 : 0);
+  const GemmPlan g = plan_of(a, pass);
+  const Extents e = extents(a, pass);
+  return g.splits > 1 ? (int64_t)g.splits * e.I * ((e.J + 7) / 8 * 8) : 0;
+}
+inline int64_t pack_offset(const seg_linear_args& a, int pass) { return (gemm_parts(a, pass) * 4 + 15) / 16 * 16; }
+inline int64_t gemm_workspace(const seg_linear_args& a, int pass) {
+  const bool product = pass != SEG_LINEAR_BWD_WEIGHT || a.dw != nullptr;
+  const GemmPlan g = plan_of(a, pass);
+  const DmaPlan d = product && (g.kind == TILE_128 || g.kind == TILE_256) ? dma_plan(a, pass) : DmaPlan{0, false, false, 0, 0};
+  return d.dma == 2 ? pack_offset(a, pass) + (d.a_elems + d.b_elems) * 2 : gemm_parts(a, pass) * 4;
 }
 
 template <int PASS>
@@ -677,10 +738,22 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
   p.I = e.I; p.J = e.J; p.Kd = e.Kd;
   p.ti = g.ti; p.tj = g.tj; p.splits = g.splits; p.kper = g.kper;
   p.part = (float*)a.workspace;
-  p.part_db = p.part + (int64_t)g.splits * e.I * e.J;
+  p.jp = (e.J + 7) / 8 * 8;
+  p.part_db = p.part + (int64_t)g.splits * e.I * p.jp;
   p.act = a.act; p.alpha = a.alpha;
   p.vecio = PASS == SEG_LINEAR_BWD_WEIGHT ? vec_ok(p.out, p.out_ld, 0, SEG_DT_F32)
                                           : vec_ok(p.out, p.out_ld, 0, a.dtype) && vec_ok(p.z, p.z_ld, 0, a.dtype) && vec_ok(p.res, p.res_ld, 0, a.dtype);
+  const DmaPlan d = g.kind == TILE_128 || g.kind == TILE_256 ? dma_plan(a, PASS) : DmaPlan{0, false, false, 0, 0};
+  if (d.dma == 2) {
+    uint16_t* to = (uint16_t*)((char*)a.workspace + pack_offset(a, PASS));
+    auto pack = [&](const Operand& o, uint16_t* dst) {         // (bit copies: either 16-bit type)
+      const int64_t ld8 = (o.cols + 7) / 8 * 8, blocks = (o.rows * (ld8 / 8) + TPB - 1) / TPB;
+      hipLaunchKernelGGL((pack_rows_kernel<half_t>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(TPB), 0, st, (const half_t*)o.p, o.ld, o.rows, o.cols, (half_t*)dst, ld8);
+      return ld8;
+    };
+    if (d.a) { p.a_ld = pack(operand_a(a, PASS), to); p.A = to; }
+    if (d.b) { p.b_ld = pack(operand_b(a, PASS), to + d.a_elems); p.B = to + d.a_elems; }
+  }
   const dim3 grid((unsigned)(g.ti * g.tj), (unsigned)g.splits);
   const int vec = vec_of(p.A, p.a_ld, p.B, p.b_ld, a.dtype);
   seq_dispatch_dtype(a.dtype, [&](auto* tp) {
@@ -720,22 +793,17 @@ int check_linear(const seg_linear_args* a, int pass, const char* name) {
                 "%s: activation %d", name, a->act);
   const Extents e = extents(*a, pass);
   SEG_CHECK_ARG(((e.I + 63) / 64) * ((int64_t)(e.J + 63) / 64) < (int64_t)1 << 24, "%s: result of %lld x %d is too large for one call", name, (long long)e.I, e.J);
-  const GemmPlan g = plan_of(*a, pass);
   SEG_CHECK_ARG(aligned16(a->workspace), "%s: workspace needs 16-byte alignment", name);
-  const bool joins = g.splits > 1 && !(pass == SEG_LINEAR_BWD_WEIGHT && a->dw == nullptr);
-  SEG_CHECK_ARG(a->M == 0 || !joins || a->workspace != nullptr, "%s: workspace is NULL (%lld bytes are needed)", name, (long long)seg_linear_workspace_bytes(a, pass));
+  SEG_CHECK_ARG(a->M == 0 || a->workspace != nullptr || gemm_workspace(*a, pass) == 0, "%s: workspace is NULL (%lld bytes are needed)", name,
+                (long long)gemm_workspace(*a, pass));
   return SEG_OK;
 }
 
 }  // namespace
 
 extern "C" int64_t seg_linear_workspace_bytes(const seg_linear_args* a, int32_t pass) {
-  if (a == nullptr || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
-  const Extents e = extents(*a, pass);
-  const GemmPlan g = plan_of(*a, pass);
-  if (pass == SEG_LINEAR_BWD_WEIGHT) return (weight_parts(*a) + (a->db != nullptr && !sums_ride(*a) ? colsum_plan(a->M, a->N).parts * a->N : 0)) * 4;
-  const int64_t b = g.splits > 1 ? (int64_t)g.splits * e.I * e.J * 4 : 0;
-  return b;
+  if (a == nullptr || a->M <= 0 || a->N <= 0 || a->K <= 0 || pass < SEG_LINEAR_FWD || pass > SEG_LINEAR_BWD_WEIGHT) return 0;
+  return gemm_workspace(*a, pass);
 }
 
 extern "C" int seg_linear_fwd(const seg_linear_args* a, seg_stream_t stream) {
@@ -774,7 +842,6 @@ extern "C" int seg_linear_bwd_weight(const seg_linear_args* a, seg_stream_t stre
   SEG_CHECK_ARG(a->M == 0 || (a->dy != nullptr && (a->dw == nullptr || a->x != nullptr)), "linear_bwd_weight: dy / x is NULL");
   SEG_CHECK_ARG(a->M <= 1 || (a->dy_ld >= a->N && (a->dw == nullptr || a->x_ld >= a->K)), "linear_bwd_weight: row strides below N = %d / K = %d", a->N, a->K);
   SEG_CHECK_ARG(a->dw == nullptr || a->N == 1 || a->dw_ld >= a->K, "linear_bwd_weight: dw_ld below K = %d", a->K);
-  SEG_CHECK_ARG(a->db == nullptr || sums_ride(*a) || a->M == 0 || a->workspace != nullptr, "linear_bwd_weight: db needs the workspace");
   hipStream_t st = (hipStream_t)stream;
   if (a->dw != nullptr) {
     GemmArgs p = {};
