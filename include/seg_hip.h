@@ -589,7 +589,8 @@ int seg_unpack_f32_f32(const void* x, float* y, int64_t npix, int32_t C, int32_t
  * padding.  Row strides (`_ld`) and batch strides (`_bs`) are in ELEMENTS, the channel axis is contiguous; strides may describe
  * slices of wider tensors.  Parameters, statistics, states of the scan and gradients of parameters are fp32, every sum is held in
  * fp32.  Results do not depend on the order of blocks: two runs give the same bits.  Nothing is allocated: workspaces are asked
- * for (`*_workspace_bytes`), need no initialisation and belong to one call in flight.  Inputs and outputs must not overlap unless
+ * for (`*_workspace_bytes`, with the arguments - pointers and strides included - as they will be passed), need no initialisation, are
+ * 16-byte aligned and belong to one call in flight.  Inputs and outputs must not overlap unless
  * an entry point says so.  Extents of zero are calls without work.                                                           */
 enum { SEG_DT_F16 = 0, SEG_DT_BF16 = 1, SEG_DT_F32 = 2 };
 /* activations of the sequence operators: SEG_ACT_NONE / RELU / LEAKY / SIGMOID and                                             */
@@ -672,7 +673,7 @@ int seg_causal_conv_step(const seg_causal_conv_args* a, seg_stream_t stream);
  *   h[t] = exp(delta[t] A[d][s]) h[t-1] + delta[t] Bm[t][s] u[t],   y[t] = (sum_s Cm[t][s] h[t] + D[d] u[t]) * silu(z[t])
  * u, dt, z, y [B][L][D], Bm, Cm [B][L][S] of dtype; A fp32 [D][S]; D, dt_bias fp32 [D] or NULL; z NULL = no gate; state fp32
  * [B][D][S] = h in front of the first row (NULL: zeros); lengths as above: rows behind a length are not read, their y is 0 and the
- * state stays; state_out (NULL: not wanted) may not be state.  saved (NULL: inference) receives what the backward pass needs:
+ * state stays; state_out (NULL: not wanted) may not be state; A and the states are 16-byte aligned.  saved (NULL: inference) receives what the backward pass needs:
  * seg_selective_scan_saved_bytes() bytes.
  * bwd: dy, dstate_out (NULL = 0), saved -> du, ddt, dz, dBm, dCm (of dtype, 0 behind a length), dA, dD, ddt_bias (fp32, stored),
  * dstate; u, dt, z, Bm, Cm, A, D, dt_bias, softplus, lengths as in the forward call.  Gradients that are NULL are not wanted.

@@ -112,9 +112,9 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   const T *A = (const T*)p.A, *B = (const T*)p.B;
   typedef T tv __attribute__((ext_vector_type(S::EPT)));
   u4 ra[2], rb[2];                                             // two steps on their way
-  // A whole step's chunk without a branch: a row that is not there is read from the last one (its results are dropped), and so
-  // is a chunk along i / j where chunks lie inside the operand or outside as a whole.  (Guards here cost the prefetch: the compiler waits for the loads where the guarded
-  // and the unguarded path meet - 22 us instead of 10 for 1111 x 333 x 700, f16.)
+  // A whole step's chunk without a branch: a row that is not there is read from the last one (its results are dropped), and so is a chunk
+  // along i / j where chunks lie inside the operand or outside as a whole.  (Guards here cost the prefetch: the compiler waits for the
+  // loads where the guarded and the unguarded path meet - 22 us instead of 14 for 1111 x 333 x 700, f16.)
   auto fetch = [&](const T* base, int64_t ld, bool kc, int64_t r0, int64_t rend, int64_t k) -> u4 {
     const int64_t row = r0 + tid / KCH;
     const int64_t col = r0 + (tid % ICH) * S::EPT;
@@ -224,15 +224,17 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
 // the layout they have in memory - k-contiguous rows of 128 bytes, or rows of one k with BM / BN columns, which the transposing LDS
 // reads turn into the same fragments - two stages in a ring: a step's loads are in flight while the step before is contracted.
 //
-// LDS swizzle (the DMA writes lane i's 16 bytes at 16 i, so the lane chooses the memory chunk instead): k-contiguous rows of 128 (64)
-// bytes keep chunk c of row r at c ^ ((r >> 1) & 7) (c ^ ((r >> 2) & 3)), so that the 16 rows a ds_read_b128 group touches lie on 16
-// different 16-byte slots; rows of one k keep it at c ^ ((k & 3) << 2), so that the four k rows of a transposing read lie in four
-// different 64-byte quarters.
-
-template <int BK> __device__ __forceinline__ int row_swizzle(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
+// LDS swizzle (the DMA writes lane i's 16 bytes at 16 i, so the lane chooses the memory chunk instead): k-contiguous rows keep chunk c of
+// row r at c ^ ((r >> 1) & 7), so that the 16 rows a ds_read_b128 group touches lie on 16 different 16-byte slots; rows of one k keep it at
+// c ^ ((k & 3) << 2), so that the four k rows of a transposing read lie in four different 64-byte quarters.
+//
+// The matrix cores bound it: 63 % of their cycles busy at 16384 x 4096 x 4096 (1.2 PFLOP/s bf16; the library's own product 1.55), the LDS 25 %.
+// Measured against and dropped: 128 x 256 and 256 x 128 in three stages of 32 at two blocks per CU (4 - 6 % slower: half again the operand
+// traffic), 128 x 128 per wave (the accumulators leave no registers), four stages of 32 (2 % slower).
+constexpr int BK = 64;
 
 // one operand's side of the ring: ROWS tile rows (along i or j) x BK of k, loaded by NWV waves
-template <bool KC, int ROWS, int BK, int NWV> struct TileLoader {
+template <bool KC, int ROWS, int NWV> struct TileLoader {
   static constexpr int NI = ROWS * BK * 2 / 1024 / NWV;        // DMA instructions (1 KiB) per wave and step
   unsigned voff[NI];
   int kchunk[2];                                               // KC: the k chunk a lane fetches in even / odd instructions
@@ -245,14 +247,13 @@ template <bool KC, int ROWS, int BK, int NWV> struct TileLoader {
     const int64_t left = rend - r0;
     const int rows = left < ROWS ? (int)left : ROWS;
     if constexpr (KC) {
-      constexpr int CPR = BK / 8, RPI = 64 / CPR;              // 16-byte chunks per row, rows per instruction
-      static_assert(BK == 32 || NI % 2 == 0, "the swizzle of an instruction depends on its parity only");
+      static_assert(NI % 2 == 0, "the swizzle of an instruction depends on its parity only");
       base = (const unsigned char*)ptr + r0 * ld2;
       rsrc = make_rsrc(base, (int)((rows - 1) * ld2 + (Kd + 7) / 8 * 16));          // rows behind the operand's end start behind this
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int row = (wave * NI + i) * RPI + lane / CPR;
-        const int ch = (lane % CPR) ^ row_swizzle<BK>(row);
+        const int row = (wave * NI + i) * 8 + (lane >> 3);
+        const int ch = (lane & 7) ^ ((row >> 1) & 7);
         kchunk[i & 1] = ch;
         voff[i] = (unsigned)(row * ld2 + ch * 16);
       }
@@ -276,7 +277,7 @@ template <bool KC, int ROWS, int BK, int NWV> struct TileLoader {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         unsigned v = voff[i];
-        if (tail && kchunk[BK == 64 ? i & 1 : 0] * 8 >= rem) v = 0x80000000u;
+        if (tail && kchunk[i & 1] * 8 >= rem) v = 0x80000000u;
         lds_dma16(rsrc, dst + (wave * NI + i) * 1024, v, (int)(k0 * 2));
       }
     } else {
@@ -289,10 +290,10 @@ template <bool KC, int ROWS, int BK, int NWV> struct TileLoader {
   }
 };
 // 32 rows from row0 of an operand's tile, k step ks
-template <bool KC, int ROWS, int BK> __device__ __forceinline__ u4 tile_frag(const unsigned char* s, int row0, int ks, int lane) {
+template <bool KC, int ROWS> __device__ __forceinline__ u4 tile_frag(const unsigned char* s, int row0, int ks, int lane) {
   if constexpr (KC) {
     const int fr = lane & 31, fh = lane >> 5;
-    return *reinterpret_cast<const u4*>(s + (row0 + fr) * (BK * 2) + (((ks * 2 + fh) ^ row_swizzle<BK>(fr)) << 4));
+    return *reinterpret_cast<const u4*>(s + (row0 + fr) * (BK * 2) + (((ks * 2 + fh) ^ ((fr >> 1) & 7)) << 4));
   } else {
     const int tg = lane >> 4, tt = lane & 15, tq = tt >> 2, tp = tt & 3;
     const int ch = (row0 >> 3) + 2 * (tg & 1) + (tp >> 1);
@@ -351,12 +352,12 @@ template <typename T> struct Row8 {                            // eight elements
   }
 };
 
-template <int PASS, typename T, int BM, int BN, int WM, int WN, int BK, int NST, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const GemmArgs p) {
+template <int PASS, typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmArgs p) {
   constexpr bool AKC = PASS != SEG_LINEAR_BWD_WEIGHT, BKC = PASS == SEG_LINEAR_FWD;
   constexpr int NWV = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * BK * 2, SLAB = 32 * 68 * 4;
-  static_assert(TN % 2 == 0 && NWV * SLAB <= NST * STAGE, "the epilogue's slabs take 64 columns and fit the ring");
-  __shared__ __align__(1024) unsigned char smem[NST * STAGE];
+  static_assert(TN % 2 == 0 && NWV * SLAB <= 2 * STAGE, "the epilogue's slabs take 64 columns and fit the ring");
+  __shared__ __align__(1024) unsigned char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // tiles in groups of eight rows of tiles, column by column: the blocks of one XCD share operand panels in both directions
   const int t = xcd_remap(blockIdx.x, p.ti * p.tj);
@@ -365,9 +366,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
   const int j0 = in / gh * BN;
   const int64_t kbeg = blockIdx.y * p.kper, kend = kbeg + p.kper < p.Kd ? kbeg + p.kper : p.Kd;
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_byte_ptr)smem);
-  TileLoader<AKC, BM, BK, NWV> la;
-  TileLoader<BKC, BN, BK, NWV> lb;
-  constexpr int NI = TileLoader<AKC, BM, BK, NWV>::NI + TileLoader<BKC, BN, BK, NWV>::NI, KS = BK / 16;
+  TileLoader<AKC, BM, NWV> la;
+  TileLoader<BKC, BN, NWV> lb;
   la.init(p.A, p.a_ld, i0, p.I, p.Kd, wave, lane);
   lb.init(p.B, p.b_ld, j0, p.J, p.Kd, wave, lane);
   f16v acc[TM][TN];
@@ -384,9 +384,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
   u4 af[2][TM], bf[2][TN];
   auto frags = [&](int set, const unsigned char* sa, int ks) {
 #pragma unroll
-    for (int a = 0; a < TM; ++a) af[set][a] = tile_frag<AKC, BM, BK>(sa, wr + a * 32, ks, lane);
+    for (int a = 0; a < TM; ++a) af[set][a] = tile_frag<AKC, BM>(sa, wr + a * 32, ks, lane);
 #pragma unroll
-    for (int b = 0; b < TN; ++b) bf[set][b] = tile_frag<BKC, BN, BK>(sa + BM * BK * 2, wc + b * 32, ks, lane);
+    for (int b = 0; b < TN; ++b) bf[set][b] = tile_frag<BKC, BN>(sa + BM * BK * 2, wc + b * 32, ks, lane);
   };
   auto contract = [&](int set) {
 #pragma unroll
@@ -399,41 +399,28 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm_tile_kernel(const Gemm
     la.issue(d, k, kend, wave);
     lb.issue(d + BM * BK * 2, k, kend, wave);
   };
-  // wait until at most `later` stages' loads are in flight, i.e. everything older has landed
-  auto landed = [&](bool later) {
-    if (NST > 2 && later) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * NI) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    ring_release_barrier();
-  };
   const int steps = (int)((kend - kbeg + BK - 1) / BK);
-  int64_t knext = kbeg;
-  auto issue_next = [&](int st) {
-    issue(st, knext);
-    knext += BK;
-  };
-#pragma unroll
-  for (int q = 0; q < NST; ++q)
-    if (q < steps) issue_next(q);
-  if (steps >= NST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * NI) : "memory");
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  issue(0, kbeg);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   ring_release_barrier();
+  if (steps > 1) issue(1, kbeg + BK);
   frags(0, smem, 0);
-  int stage = 0;
-  for (int it = 0; it < steps; ++it) {
+  int64_t knext = kbeg + 2 * BK;
+  for (int it = 0; it < steps; ++it, knext += BK) {
+    const int stage = it & 1;
     const unsigned char* sa = smem + stage * STAGE;
 #pragma unroll
-    for (int ks = 1; ks < KS; ++ks) {
+    for (int ks = 1; ks < BK / 16; ++ks) {
       frags(ks & 1, sa, ks);
       contract((ks - 1) & 1);
     }
-    const int next = stage + 1 == NST ? 0 : stage + 1;
     if (it + 1 < steps) {
-      landed(it + NST - 1 < steps);                            // the next stage has landed for every wave, this one has no readers left
-      frags(0, smem + next * STAGE, 0);
-      if (it + NST < steps) issue_next(stage);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      ring_release_barrier();                                  // the next stage has landed for every wave, this one has no readers left
+      frags(0, smem + (stage ^ 1) * STAGE, 0);
+      if (it + 2 < steps) issue(stage, knext);
     }
-    contract((KS - 1) & 1);
-    stage = next;
+    contract((BK / 16 - 1) & 1);
   }
   // Results leave through wave-private slabs of 32 rows x 64 columns in the ring's LDS, so that a store covers whole 128-byte lines:
   // stores straight from the accumulators (32-byte pieces of 32 rows) took 221 us instead of 172 where two tensors are written
@@ -516,6 +503,7 @@ __global__ __launch_bounds__(TPB) void pack_rows_kernel(const T* x, int64_t ld, 
 // ---- a few rows against all the weights (forward, up to 64 rows): the weights' bytes and one memory latency bound it, so they go straight
 // into the matrix instructions' registers, once, with no LDS in between.  A block owns 16 units; its waves share k in steps of 64 bytes per
 // row (lane l: row l % 16, 16 bytes at chunk l / 16), keep four steps' loads in flight and add their sums in the LDS.  MT x 16 rows of x.
+// 4 x 4096 x 1024 bf16: 4.2 us (2 TB/s of weights); the tiled kernel with split sums took 12.
 template <typename T, int MT, int WK>
 __global__ __launch_bounds__(64 * WK) void gemm_rows_kernel(const GemmArgs p) {
   constexpr int EPC = 16 / (int)sizeof(T), STEP = 4 * EPC, UN = MT <= 2 ? 4 : 2;
@@ -633,7 +621,7 @@ inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   // 256 x 256 where such tiles (with k split in ranges of 4096) fill three quarters of the 256 CUs: 233 us against 250 with 128 x 128
   // for 16384 x 4096 x 1024 (f16, GELU, pre-activation kept), 375 against 402 for the backward pass of 16384 x 1024 x 4096 (bf16)
   const int64_t t256 = ((I + 255) / 256) * ((J + 255) / 256);
-  g.kind = !dma ? TILE_ANY : t256 * ((Kd + 4095) / 4096) >= 192 ? TILE_256 : TILE_128;
+  g.kind = !dma ? TILE_ANY : t256 * (Kd > 4096 * 64 ? 64 : (Kd + 4095) / 4096) >= 192 ? TILE_256 : TILE_128;
   const int side = g.kind == TILE_ANY ? 64 : g.kind == TILE_128 ? 128 : 256;
   g.ti = (int)((I + side - 1) / side);
   g.tj = (J + side - 1) / side;
@@ -642,7 +630,7 @@ inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   // f16: 14 us in one launch, 16 in two)
   int64_t s = tiles * 2 > room || tiles == 0 ? 1 : room / tiles;
   if (s > Kd / 512) s = Kd / 512;
-  if (s > 32) s = 32;
+  if (s > 256) s = 256;
   if (s < 1) s = 1;
   const int64_t step = g.kind != TILE_ANY ? 64 : dtype == SEG_DT_F32 ? 16 : 32;
   g.kper = ((Kd + s - 1) / s + step - 1) / step * step;
@@ -659,8 +647,7 @@ inline Extents extents(const seg_linear_args& a, int pass) {
 
 inline int vec_of(const void* A, int64_t a_ld, const void* B, int64_t b_ld, int dt) {
   const int es = (int)dt_size(dt);
-  for (int v = dt == SEG_DT_F32 ? 4 : 8; v > 1; v >>= 1) {
-    if (v == 2) break;
+  for (int v = dt == SEG_DT_F32 ? 4 : 8; v >= 4; v >>= 1) {
     if ((uintptr_t)A % (v * es) == 0 && (uintptr_t)B % (v * es) == 0 && a_ld % v == 0 && b_ld % v == 0) return v;
   }
   return 1;
@@ -668,7 +655,8 @@ inline int vec_of(const void* A, int64_t a_ld, const void* B, int64_t b_ld, int 
 
 // What the LDS-DMA tile kernels take of a pass: 16-bit operands in 16-byte rows (k-contiguous ones also a whole number of 8 inputs),
 // offsets inside a tile below 2 GiB.  A product of 2^32 operations or more whose operands do not fit is worth a packed copy of them
-// (16384 x 4095 x 4095 f16: 2118 us without, 780 with copies; its backward pass 7473 and 1412).  dma: 0 no, 1 as they are, 2 with copies (a, b: which)
+// (16384 x 4095 x 4095 f16: 2118 us without, 780 with copies; its backward pass 7473 and
+// 1412).  dma: 0 no, 1 as they are, 2 with copies (a, b: which)
 struct Operand { const void* p; int64_t ld, rows, cols; bool kc; };
 struct DmaPlan { int dma; bool a, b; int64_t a_elems, b_elems; };
 inline Operand operand_a(const seg_linear_args& a, int pass) {
@@ -770,8 +758,8 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
       }
     } else if (g.kind != TILE_ANY) {
       if constexpr (!std::is_same<T, float>::value) {
-        if (g.kind == TILE_256) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 256, 256, 2, 4, 64, 2, 2>), grid, dim3(512), 0, st, p);
-        else hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 128, 2, 2, 64, 2, 2>), grid, dim3(256), 0, st, p);
+        if (g.kind == TILE_256) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 256, 256, 2, 4>), grid, dim3(512), 0, st, p);
+        else hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 128, 2, 2>), grid, dim3(256), 0, st, p);
       }
     } else if (vec == 4) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 4>), grid, dim3(TPB), 0, st, p);
     else if (vec == 8) {

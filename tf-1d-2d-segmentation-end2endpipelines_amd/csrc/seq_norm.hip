@@ -6,6 +6,9 @@
 // Bandwidth bounds both: the row is read ONCE and kept in registers, so the variance is the two-pass one (no cancellation of
 // sum x^2 - mean^2) at no traffic.  LPR lanes share a row - 8 lanes for the 64-channel rows of a full-resolution level, a wave, or
 // the whole block - with NCH chunks of 8 channels per lane; rows longer than a block's registers are walked in a loop.
+//
+// Measured: forward 4096 x 1024 f16 6.6 us (2.5 TB/s: one memory latency per block is what is left); backward 1 048 576 x 64 f16 75 us
+// (5.4 TB/s; a large copy reaches 4.9) and 4.7 us for the blocks' sums; 5003 x 1111 f32, 4-byte accesses, 17.6 us (3.8 TB/s) and 4.3 us.
 #include "seq_common.h"
 
 namespace {

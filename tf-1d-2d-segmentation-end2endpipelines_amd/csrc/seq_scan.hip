@@ -14,6 +14,11 @@
 // Backward: with dp = dy silu(z) the adjoint g[t] = C[t] dp[t] + a[t+1] g[t+1] runs from the end, over the same chunks in the same way
 // (a chunk's own part of the adjoint in front of it is sum_t (prod_{k<=t} a[k]) C[t] dp[t], which a walk FORWARD in t adds up).  The
 // states are not kept: the forward call saves h in front of every tile, each tile is recomputed from there into registers.
+//
+// Measured: 8 prompts of up to 2048 rows x 2048 channels x 16 states, bf16: main launch 150 us, the chunks' first pass 98 (the main loop
+// issues 35 slots per four states and row - the floor of one exponential and four operations is 32 - and staging another fifth); training
+// step 8 x 1024 x 1024 x 16, f16: forward 33 + 47, backward 36 + 160 us at two waves per SIMD (255 registers); one row of 64 x 2048 x 16
+// 7.7 us (2.2 TB/s of states).
 #include "seq_common.h"
 
 namespace {
