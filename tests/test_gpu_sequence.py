@@ -133,7 +133,7 @@ def test_layer_norm_non_finite_rows_stay_in_their_row():
 
 # --------------------------------------------------------------------------------------------------------------------- linear
 LIN = [(1, 8, 8), (1, 1, 1), (3, 5, 7), (16, 64, 64), (64, 64, 32), (65, 130, 100), (17, 33, 257), (129, 256, 512), (300, 200, 1000), (2, 1000, 4096),
-       (256, 256, 64), (257, 264, 72), (512, 384, 640)]
+       (256, 256, 64), (257, 264, 72), (512, 384, 640), (300, 64, 64), (200, 40, 128), (70, 56, 48)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)

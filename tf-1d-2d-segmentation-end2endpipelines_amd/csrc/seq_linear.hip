@@ -226,12 +226,14 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
 //
 // LDS swizzle (the DMA writes lane i's 16 bytes at 16 i, so the lane chooses the memory chunk instead): k-contiguous rows keep chunk c of
 // row r at c ^ ((r >> 1) & 7), so that the 16 rows a ds_read_b128 group touches lie on 16 different 16-byte slots; rows of one k keep it at
-// c ^ ((k & 3) << 2), so that the four k rows of a transposing read lie in four different 64-byte quarters.
+// c ^ ((k & 3) << 2), so that the four k rows of a transposing read lie in four different 64-byte quarters (rows of 64 columns: two of them
+// fill the banks, c ^ ((k & 2) << 1)).
 //
 // The matrix cores bound it: 63 % of their cycles busy at 16384 x 4096 x 4096 (1.2 PFLOP/s bf16; the library's own product 1.55), the LDS 25 %.
 // Measured against and dropped: 128 x 256 and 256 x 128 in three stages of 32 at two blocks per CU (4 - 6 % slower: half again the operand
 // traffic), 128 x 128 per wave (the accumulators leave no registers), four stages of 32 (2 % slower).
 constexpr int BK = 64;
+template <int ROWS> __device__ __forceinline__ int k_swizzle(int k) { return ROWS == 64 ? (k & 2) << 1 : (k & 3) << 2; }
 
 // one operand's side of the ring: ROWS tile rows (along i or j) x BK of k, loaded by NWV waves
 template <bool KC, int ROWS, int NWV> struct TileLoader {
@@ -264,7 +266,7 @@ template <bool KC, int ROWS, int NWV> struct TileLoader {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int k = (wave * NI + i) * RPI + lane / LPR;
-        const int ch = (lane % LPR) ^ ((k & 3) << 2);
+        const int ch = (lane % LPR) ^ k_swizzle<ROWS>(k);
         voff[i] = (unsigned)(k * ld2 + ch * 16);
       }
     }
@@ -297,7 +299,7 @@ template <bool KC, int ROWS> __device__ __forceinline__ u4 tile_frag(const unsig
   } else {
     const int tg = lane >> 4, tt = lane & 15, tq = tt >> 2, tp = tt & 3;
     const int ch = (row0 >> 3) + 2 * (tg & 1) + (tp >> 1);
-    const unsigned char* a = s + (ks * 16 + 8 * (tg >> 1) + tq) * (ROWS * 2) + ((ch ^ (tq << 2)) << 4) + (tp & 1) * 8;
+    const unsigned char* a = s + (ks * 16 + 8 * (tg >> 1) + tq) * (ROWS * 2) + ((ch ^ k_swizzle<ROWS>(tq)) << 4) + (tp & 1) * 8;
     const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_ptr)a);
     const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_ptr)(a + 4 * ROWS * 2));
     const u2 l = __builtin_bit_cast(u2, lo), h = __builtin_bit_cast(u2, hi);
@@ -614,17 +616,19 @@ inline ColsumPlan colsum_plan(int64_t rows, int cols) {
 }
 
 // ---- plans
-enum { TILE_ANY = 0, TILE_128 = 1, TILE_256 = 2, FEW_ROWS = 3 };
+enum { TILE_ANY = 0, TILE_128 = 1, TILE_256 = 2, FEW_ROWS = 3, TILE_NARROW = 4 };
+inline bool tiled(int kind) { return kind == TILE_128 || kind == TILE_256 || kind == TILE_NARROW; }
 struct GemmPlan { int kind; int ti, tj, splits; int64_t kper; };
 inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   GemmPlan g;
-  // 256 x 256 where such tiles (with k split in ranges of 4096) fill three quarters of the 256 CUs: 233 us against 250 with 128 x 128
+  // 128 x 64 for up to 64 columns (1048576 x 64 x 64, f16: 69 us, 157 with 128 x 128, the bytes' floor 55); 256 x 256 where such tiles
+  // (with k split in ranges of 4096) fill three quarters of the 256 CUs: 233 us against 250 with 128 x 128
   // for 16384 x 4096 x 1024 (f16, GELU, pre-activation kept), 375 against 402 for the backward pass of 16384 x 1024 x 4096 (bf16)
   const int64_t t256 = ((I + 255) / 256) * ((J + 255) / 256);
-  g.kind = !dma ? TILE_ANY : t256 * (Kd > 4096 * 64 ? 64 : (Kd + 4095) / 4096) >= 192 ? TILE_256 : TILE_128;
-  const int side = g.kind == TILE_ANY ? 64 : g.kind == TILE_128 ? 128 : 256;
-  g.ti = (int)((I + side - 1) / side);
-  g.tj = (J + side - 1) / side;
+  g.kind = !dma ? TILE_ANY : J <= 64 ? TILE_NARROW : t256 * (Kd > 4096 * 64 ? 64 : (Kd + 4095) / 4096) >= 192 ? TILE_256 : TILE_128;
+  const int si = g.kind == TILE_ANY ? 64 : g.kind == TILE_256 ? 256 : 128, sj = g.kind == TILE_NARROW ? 64 : si;
+  g.ti = (int)((I + si - 1) / si);
+  g.tj = (J + sj - 1) / sj;
   const int64_t tiles = (int64_t)g.ti * g.tj, room = g.kind == TILE_256 ? 256 : g.kind == TILE_128 ? 512 : 1024;
   // fewer tiles than the card has room for: k is split, down to 512 of it per block (a second launch joins the parts: 1111 x 333 x 700,
   // f16: 14 us in one launch, 16 in two)
@@ -671,14 +675,15 @@ inline DmaPlan dma_plan(const seg_linear_args& a, int pass) {
   DmaPlan d = {0, false, false, 0, 0};
   const Extents e = extents(a, pass);
   // (tiles far larger than the result waste the matrix cores)
-  if (a.dtype == SEG_DT_F32 || e.I < 64 || e.J < 64 || e.Kd < 1) return d;
+  if (a.dtype == SEG_DT_F32 || e.I < 64 || e.J < 48 || e.Kd < 1) return d;
   const Operand A = operand_a(a, pass), B = operand_b(a, pass);
   if (A.ld > (1 << 21) || B.ld > (1 << 21) || A.cols > (1 << 21) || B.cols > (1 << 21)) return d;
   auto fits = [](const Operand& o) { return aligned16(o.p) && o.ld % 8 == 0 && (!o.kc || o.cols % 8 == 0); };
   d.a = !fits(A);
   d.b = !fits(B);
   if (!d.a && !d.b) { d.dma = 1; return d; }
-  if ((double)e.I * e.J * e.Kd < 2147483648.0) return d;
+  // (an element's copy costs what 130 products of it cost the other kernel: 16384 x 63 x 4001 took 47 us without copies, 118 with)
+  if (e.I < 256 || e.J < 256 || (double)e.I * e.J * e.Kd < 2147483648.0) return d;
   d.dma = 2;
   auto elems = [](const Operand& o) { return o.rows * ((o.cols + 7) / 8 * 8); };
   d.a_elems = d.a ? elems(A) : 0;
@@ -715,7 +720,7 @@ inline int64_t pack_offset(const seg_linear_args& a, int pass) { return (gemm_pa
 inline int64_t gemm_workspace(const seg_linear_args& a, int pass) {
   const bool product = pass != SEG_LINEAR_BWD_WEIGHT || a.dw != nullptr;
   const GemmPlan g = plan_of(a, pass);
-  const DmaPlan d = product && (g.kind == TILE_128 || g.kind == TILE_256) ? dma_plan(a, pass) : DmaPlan{0, false, false, 0, 0};
+  const DmaPlan d = product && tiled(g.kind) ? dma_plan(a, pass) : DmaPlan{0, false, false, 0, 0};
   return d.dma == 2 ? pack_offset(a, pass) + (d.a_elems + d.b_elems) * 2 : gemm_parts(a, pass) * 4;
 }
 
@@ -731,7 +736,7 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
   p.act = a.act; p.alpha = a.alpha;
   p.vecio = PASS == SEG_LINEAR_BWD_WEIGHT ? vec_ok(p.out, p.out_ld, 0, SEG_DT_F32)
                                           : vec_ok(p.out, p.out_ld, 0, a.dtype) && vec_ok(p.z, p.z_ld, 0, a.dtype) && vec_ok(p.res, p.res_ld, 0, a.dtype);
-  const DmaPlan d = g.kind == TILE_128 || g.kind == TILE_256 ? dma_plan(a, PASS) : DmaPlan{0, false, false, 0, 0};
+  const DmaPlan d = tiled(g.kind) ? dma_plan(a, PASS) : DmaPlan{0, false, false, 0, 0};
   if (d.dma == 2) {
     uint16_t* to = (uint16_t*)((char*)a.workspace + pack_offset(a, PASS));
     auto pack = [&](const Operand& o, uint16_t* dst) {         // (bit copies: either 16-bit type)
@@ -758,7 +763,8 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
       }
     } else if (g.kind != TILE_ANY) {
       if constexpr (!std::is_same<T, float>::value) {
-        if (g.kind == TILE_256) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 256, 256, 2, 4>), grid, dim3(512), 0, st, p);
+        if (g.kind == TILE_NARROW) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 64, 2, 1>), grid, dim3(128), 0, st, p);
+        else if (g.kind == TILE_256) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 256, 256, 2, 4>), grid, dim3(512), 0, st, p);
         else hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 128, 2, 2>), grid, dim3(256), 0, st, p);
       }
     } else if (vec == 4) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 4>), grid, dim3(TPB), 0, st, p);
