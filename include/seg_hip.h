@@ -591,7 +591,7 @@ int seg_unpack_f32_f32(const void* x, float* y, int64_t npix, int32_t C, int32_t
  * fp32.  Results do not depend on the order of blocks: two runs give the same bits.  Nothing is allocated: workspaces are asked
  * for (`*_workspace_bytes`, with the arguments - pointers and strides included - as they will be passed), need no initialisation, are
  * 16-byte aligned and belong to one call in flight.  Inputs and outputs must not overlap unless
- * an entry point says so.  Extents of zero are calls without work.                                                           */
+ * an entry point says so (the same rows then: one pointer, one row stride).  Extents of zero are calls without work.                                                           */
 enum { SEG_DT_F16 = 0, SEG_DT_BF16 = 1, SEG_DT_F32 = 2 };
 /* activations of the sequence operators: SEG_ACT_NONE / RELU / LEAKY / SIGMOID and                                             */
 enum { SEG_ACT_SILU = 5, SEG_ACT_GELU = 6 };                       /* v sigmoid(v);  v Phi(v) (the error function, no tanh form) */

@@ -770,3 +770,81 @@ def test_gradients_are_difference_quotients():
     directional(scan, {k: t.double() for k, t in i.items()},
                 dict(u=d.du, dt=d.ddt, A=d.dA, B=d.dB, C=d.dC, D=d.dD, z=d.dz, dt_bias=d.ddt_bias, state=d.dstate), g,
                 ("u", "dt", "A", "B", "C", "D", "z", "dt_bias", "state"))
+
+
+# --------------------------------------------------------------------------------------------------- the C level's documented overlaps
+def test_documented_overlaps():
+    """What include/seg_hip.h allows to be the same memory: layer norm's y = x, dx = dy and dx = x (rows in registers and longer ones), linear's
+    y = residual (every kernel, split sums too), the activation gradient's dx = dy.  The Python functions never alias; these are C calls."""
+    ffi = importlib.import_module("tf-1d-2d-segmentation-end2endpipelines_amd._ffi")
+    lib, st = ffi.lib(), torch.cuda.current_stream().cuda_stream
+    g = gen(71)
+    for rows, C in ((5, 64), (3, 2056), (2, 16400)):
+        x, dy, gamma = rnd(g, rows, C).cuda(), rnd(g, rows, C).cuda(), (torch.rand(C, generator=g) + 0.5).cuda()
+        y, mean, rstd = seq.layer_norm(x, gamma, stats=True)
+        dx, dg, db = seq.layer_norm_backward(dy, x, mean, rstd, gamma)
+        t = x.clone()
+        assert lib.seg_layernorm_fwd(t.data_ptr(), C, t.data_ptr(), C, rows, C, 2, gamma.data_ptr(), None, 1e-3, None, None, st) == 0
+        assert torch.equal(t, y)
+        ws = torch.empty(lib.seg_layernorm_bwd_workspace_bytes(rows, C, 2), dtype=torch.uint8, device="cuda")
+        for which in (0, 1):
+            a, b, pg, pb = dy.clone(), x.clone(), torch.empty(C, device="cuda"), torch.empty(C, device="cuda")
+            out = (a, b)[which]
+            assert lib.seg_layernorm_bwd(a.data_ptr(), C, b.data_ptr(), C, out.data_ptr(), C, rows, C, 2, mean.data_ptr(), rstd.data_ptr(), gamma.data_ptr(),
+                                         pg.data_ptr(), pb.data_ptr(), ws.data_ptr(), st) == 0
+            assert torch.equal(out, dx) and torch.equal(pg, dg) and torch.equal(pb, db)
+    for M, N, K, dtype in ((4, 40, 64, torch.float16), (100, 37, 41, torch.float16), (300, 256, 128, torch.bfloat16), (100, 72, 4096, torch.float32), (130, 128, 4096, torch.float16),
+                           (12360, 1032, 136, torch.float16)):
+        x, w, r = rnd(g, M, K, dtype=dtype).cuda(), rnd(g, N, K, dtype=dtype).cuda(), rnd(g, M, N, dtype=dtype).cuda()
+        want = seq.linear(x, w, activation="silu", residual=r)
+        t = r.clone()
+        a = ffi.LinearArgs(M, N, K, seq._DT[dtype], ffi.SEQ_ACT["silu"], 0.0, x.data_ptr(), K, w.data_ptr(), K, None, t.data_ptr(), N, None, 0, t.data_ptr(), N)
+        ws = torch.empty(max(lib.seg_linear_workspace_bytes(a, 0), 16), dtype=torch.uint8, device="cuda")
+        a.workspace = ws.data_ptr()
+        assert lib.seg_linear_fwd(a, st) == 0
+        assert torch.equal(t, want), (M, N, K)
+        dy, r = rnd(g, M, N, dtype=dtype).cuda(), rnd(g, M, K, dtype=dtype).cuda()
+        want = seq.linear_backward(dy, x, w, residual=r, need_dw=False, need_db=False)[0]
+        t = r.clone()
+        a = ffi.LinearArgs(M, K, N, seq._DT[dtype], 0, 0.0, dy.data_ptr(), N, w.data_ptr(), K, None, t.data_ptr(), K, None, 0, t.data_ptr(), K)
+        ws = torch.empty(max(lib.seg_linear_workspace_bytes(a, 1), 16), dtype=torch.uint8, device="cuda")
+        a.workspace = ws.data_ptr()
+        assert lib.seg_linear_bwd_data(a, st) == 0
+        assert torch.equal(t, want), (M, N, K)
+    z, dy = rnd(g, 9, 50).cuda(), rnd(g, 9, 50).cuda()
+    want, t = seq.activation_backward(dy, z, "gelu"), dy.clone()
+    assert lib.seg_linear_act_bwd(t.data_ptr(), 50, z.data_ptr(), 50, t.data_ptr(), 50, 9, 50, 2, ffi.SEQ_ACT["gelu"], 0.0, st) == 0
+    assert torch.equal(t, want)
+    torch.cuda.synchronize()
+
+
+def test_partial_gradients_at_the_c_level():
+    """Gradients that are NULL are not wanted: the others come out as they do together."""
+    ffi = importlib.import_module("tf-1d-2d-segmentation-end2endpipelines_amd._ffi")
+    lib, st = ffi.lib(), torch.cuda.current_stream().cuda_stream
+    B, L, D, S = 2, 70, 24, 16
+    i, dy, dst, g = scan_inputs(72, B, L, D, S, torch.float32)
+    c = {k: t.cuda() for k, t in i.items()}
+    state = c.pop("state")
+    _y, _l, saved = seq.selective_scan(**c, state=state, training=True)
+    dy = dy.cuda()
+    want = seq.selective_scan_backward(dy, c["u"], c["dt"], c["A"], c["B"], c["C"], saved, D=c["D"], z=c["z"], dt_bias=c["dt_bias"])
+    shapes = dict(du=(B, L, D), ddt=(B, L, D), dz=(B, L, D), dBm=(B, L, S), dCm=(B, L, S), dA=(D, S), dD=(D,), ddt_bias=(D,), dstate=(B, D, S))
+    both = dict(zip(shapes, (want.du, want.ddt, want.dz, want.dB, want.dC, want.dA, want.dD, want.ddt_bias, want.dstate)))
+    for name, shape in shapes.items():
+        a = ffi.ScanArgs(B, L, D, S, 2, 1)
+        for n, t in (("u", c["u"]), ("dt", c["dt"]), ("z", c["z"]), ("Bm", c["B"]), ("Cm", c["C"]), ("dy", dy)):
+            setattr(a, n, t.data_ptr())
+            setattr(a, n + "_bs", t.stride(0))
+            setattr(a, n + "_ld", t.stride(1))
+        a.A, a.Dskip, a.dt_bias, a.saved = c["A"].data_ptr(), c["D"].data_ptr(), c["dt_bias"].data_ptr(), saved.data_ptr()
+        out = torch.full(shape, float("nan"), device="cuda")
+        setattr(a, name, out.data_ptr())
+        if len(shape) == 3 and name != "dstate":
+            setattr(a, name + "_bs", shape[1] * shape[2])
+            setattr(a, name + "_ld", shape[2])
+        ws = torch.empty(lib.seg_selective_scan_bwd_workspace_bytes(a), dtype=torch.uint8, device="cuda")
+        a.workspace = ws.data_ptr()
+        assert lib.seg_selective_scan_bwd(a, st) == 0, lib.seg_last_error()
+        torch.cuda.synchronize()
+        assert torch.equal(out, both[name]), name

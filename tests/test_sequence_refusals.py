@@ -208,3 +208,14 @@ def test_selective_scan_arguments(lib):
     refused(lib, lib.seg_selective_scan_step(scan_args(u_bs=7), None), "strides")
     assert lib.seg_selective_scan_fwd(scan_args(B=0), None) == 0
     assert lib.seg_selective_scan_saved_bytes(scan_args()) == 2 * 1 * 8 * 16 * 4
+
+
+def test_results_in_place_keep_the_row_stride(lib):
+    """Where a result may take its operand's memory, rows of another stride would be written while other rows are still read."""
+    refused(lib, lib.seg_layernorm_fwd(FAKE, 8, FAKE, 16, 4, 8, 0, None, None, 1e-3, None, None, None), "stride")
+    b = lib.seg_layernorm_bwd
+    refused(lib, b(FAKE, 8, 2 * FAKE, 8, FAKE, 16, 4, 8, 0, FAKE, FAKE, None, FAKE, FAKE, FAKE, None), "in place")
+    refused(lib, b(FAKE, 8, 2 * FAKE, 8, 2 * FAKE, 16, 4, 8, 0, FAKE, FAKE, None, FAKE, FAKE, FAKE, None), "in place")
+    refused(lib, lib.seg_linear_act_bwd(FAKE, 8, 2 * FAKE, 8, FAKE, 16, 4, 8, 0, 1, 0.0, None), "in place")
+    refused(lib, lib.seg_linear_fwd(linear_args(residual=FAKE, residual_ld=40), None), "in place")
+    refused(lib, lib.seg_linear_bwd_data(linear_args(w_ld=32, residual=FAKE, residual_ld=40), None), "in place")

@@ -807,6 +807,7 @@ extern "C" int seg_linear_fwd(const seg_linear_args* a, seg_stream_t stream) {
   SEG_CHECK_ARG((a->M == 1 || a->x_ld >= a->K) && (a->N == 1 || a->w_ld >= a->K), "linear_fwd: row strides below K = %d", a->K);
   SEG_CHECK_ARG(a->M == 1 || (a->y_ld >= a->N && (a->z == nullptr || a->z_ld >= a->N) && (a->residual == nullptr || a->residual_ld >= 0)),
                 "linear_fwd: row strides below N = %d", a->N);
+  SEG_CHECK_ARG(a->M == 1 || a->residual != a->y || a->residual_ld == a->y_ld, "linear_fwd: y in place of the residual has another row stride");
   GemmArgs p = {};
   p.A = a->x; p.a_ld = a->x_ld; p.B = a->w; p.b_ld = a->w_ld;
   p.bias = a->bias; p.res = a->residual; p.res_ld = a->residual_ld; p.z = a->z; p.z_ld = a->z_ld; p.out = a->y; p.out_ld = a->y_ld;
@@ -823,6 +824,7 @@ extern "C" int seg_linear_bwd_data(const seg_linear_args* a, seg_stream_t stream
   SEG_CHECK_ARG((a->M == 1 || a->x_ld >= a->K) && (a->K == 1 || a->w_ld >= a->N), "linear_bwd_data: row strides of x below %d or of w below %d", a->K, a->N);
   SEG_CHECK_ARG(a->M == 1 || (a->y_ld >= a->N && (a->z == nullptr || a->z_ld >= a->N) && (a->residual == nullptr || a->residual_ld >= 0)),
                 "linear_bwd_data: row strides below N = %d", a->N);
+  SEG_CHECK_ARG(a->M == 1 || a->residual != a->y || a->residual_ld == a->y_ld, "linear_bwd_data: y in place of the residual has another row stride");
   GemmArgs p = {};
   p.A = a->x; p.a_ld = a->x_ld; p.B = a->w; p.b_ld = a->w_ld;
   p.res = a->residual; p.res_ld = a->residual_ld; p.z = a->z; p.z_ld = a->z_ld; p.out = a->y; p.out_ld = a->y_ld;
@@ -888,6 +890,7 @@ extern "C" int seg_linear_act_bwd(const void* dy, int64_t dy_ld, const void* z, 
   if (rows == 0) return SEG_OK;
   SEG_CHECK_ARG(dy != nullptr && z != nullptr && dx != nullptr, "linear_act_bwd: dy / z / dx is NULL");
   SEG_CHECK_ARG(rows == 1 || (dy_ld >= C && z_ld >= C && dx_ld >= C), "linear_act_bwd: row strides below the %d channels", C);
+  SEG_CHECK_ARG(rows == 1 || dx != dy || dx_ld == dy_ld, "linear_act_bwd: dx in place of dy has another row stride");
   seq_dispatch_dtype(dtype, [&](auto* tp) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
     const int64_t blocks = (rows * ((C + 7) / 8) + TPB - 1) / TPB;

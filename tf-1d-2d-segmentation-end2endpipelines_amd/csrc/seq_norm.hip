@@ -345,6 +345,7 @@ extern "C" int seg_layernorm_fwd(const void* x, int64_t x_ld, void* y, int64_t y
   SEG_CHECK_ARG(rows <= 1 || (x_ld >= C && y_ld >= C), "layernorm_fwd: row strides below the %d channels", C);
   if (rows == 0) return SEG_OK;
   SEG_CHECK_ARG(x != nullptr && y != nullptr, "layernorm_fwd: x / y is NULL");
+  SEG_CHECK_ARG(y != x || rows == 1 || y_ld == x_ld, "layernorm_fwd: y in place of x has another row stride");
   hipStream_t st = (hipStream_t)stream;
   seq_dispatch_dtype(dtype, [&](auto* tp) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
@@ -380,6 +381,7 @@ extern "C" int seg_layernorm_bwd(const void* dy, int64_t dy_ld, const void* x, i
   const bool params = dgamma != nullptr || dbeta != nullptr;
   SEG_CHECK_ARG(rows == 0 || (dy != nullptr && x != nullptr && mean != nullptr && rstd != nullptr), "layernorm_bwd: dy / x / mean / rstd is NULL");
   SEG_CHECK_ARG(rows == 0 || !params || workspace != nullptr, "layernorm_bwd: dgamma / dbeta need the workspace");
+  SEG_CHECK_ARG(rows <= 1 || dx == nullptr || ((dx != dy || dx_ld == dy_ld) && (dx != x || dx_ld == x_ld)), "layernorm_bwd: dx in place of dy / x has another row stride");
   hipStream_t st = (hipStream_t)stream;
   float* part = params ? (float*)workspace : nullptr;
   const int64_t nblk = rows > 0 ? ln_bwd_blocks(rows, C) : 0;
