@@ -848,3 +848,39 @@ def test_partial_gradients_at_the_c_level():
         assert lib.seg_selective_scan_bwd(a, st) == 0, lib.seg_last_error()
         torch.cuda.synchronize()
         assert torch.equal(out, both[name]), name
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("wide_side", [136, 56])
+def test_linear_every_number_of_steps(wide_side, dtype):
+    """Contractions of one step of the tile kernels' ring to several rounds of it, whole and ragged, in the three passes."""
+    g = gen(81)
+    for L in (1, 8, 64, 72, 128, 192, 200, 256, 264, 320, 512, 576, 1030):
+        a, b = rnd(g, 136, L, dtype=dtype), rnd(g, wide_side, L, dtype=dtype)
+        want, s = a.double() @ b.double().t(), a.double().abs() @ b.double().abs().t()
+        R.assert_close(seq.linear(a.cuda(), b.cuda()), want, s, L + 4, f"fwd {L}")
+        bt, at = b.t().contiguous(), a.t().contiguous()
+        none = torch.zeros(136, wide_side, dtype=dtype, device="cuda")
+        R.assert_close(seq.linear_backward(a.cuda(), none, bt.cuda(), need_dw=False, need_db=False)[0], want, s, L + 4, f"dx {L}")
+        none = torch.zeros(136, wide_side, dtype=dtype, device="cuda")
+        dw, db = seq.linear_backward(at.cuda(), bt.cuda(), none, need_dx=False)[1:]
+        R.assert_close(dw, want, s, L + 4, f"dw {L}")
+        R.assert_close(db, at.double().sum(0), at.double().abs().sum(0), L + 4, f"db {L}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", [(3, 40, 30008), (64, 64, 24576), (33, 16, 9000), (40, 4104, 520), (16, 40, 4096), (5, 2048, 5000), (17, 24, 4100)])
+def test_linear_few_rows_and_long_contractions(M, N, K, dtype):
+    """Both sides of the limits of the kernel for few rows, and sums split over many ranges (joined by several threads per element)."""
+    g = gen(82)
+    x, w, b, r = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype, scale=K ** -0.5), rnd(g, N), rnd(g, M, N, dtype=dtype)
+    y, pre = seq.linear(x.cuda(), w.cuda(), b.cuda(), activation="relu", residual=r.cuda(), preactivation=True)
+    z64, s = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t() + b.double().abs()
+    R.assert_close(pre, z64, s, K + 4, "z")
+    R.assert_close(y, z64.clamp(min=0) + r.double(), s + r.double().abs(), K + 6, "y")
+    # the same contraction as a weight gradient: K rows
+    dy, xt = x.t().contiguous(), w.t().contiguous()
+    dw, db = seq.linear_backward(dy.cuda(), xt.cuda(), torch.zeros(M, N, dtype=dtype, device="cuda"), need_dx=False)[1:]
+    R.assert_close(dw, x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t(), K + 4, "dw")
+    R.assert_close(db, x.double().sum(1), x.double().abs().sum(1), K + 4, "db")
+    assert torch.equal(dw, seq.linear_backward(dy.cuda(), xt.cuda(), torch.zeros(M, N, dtype=dtype, device="cuda"), need_dx=False)[1])

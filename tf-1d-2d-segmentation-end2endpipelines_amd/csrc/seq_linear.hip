@@ -222,7 +222,9 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
 
 // ---- the tile kernel for 16-bit operands whose rows take 16-byte accesses: BM x BN tiles, 64 of k per step, both operands by LDS-DMA in
 // the layout they have in memory - k-contiguous rows of 128 bytes, or rows of one k with BM / BN columns, which the transposing LDS
-// reads turn into the same fragments - two stages in a ring: a step's loads are in flight while the step before is contracted.
+// reads turn into the same fragments - NST stages in a ring: a step's loads are in flight while NST - 1 steps before it are contracted.  Two
+// stages where other blocks of the CU hide a load's latency (or the tile fills the LDS), four where a block has its CU to itself:
+// 2048 x 2048 x 2048 f16 25 us and 28 with two, 256 x 16384 x 4096 43 and 49, weight gradient of 1048576 x 64 x 64 46 and 57.
 //
 // LDS swizzle (the DMA writes lane i's 16 bytes at 16 i, so the lane chooses the memory chunk instead): k-contiguous rows keep chunk c of
 // row r at c ^ ((r >> 1) & 7), so that the 16 rows a ds_read_b128 group touches lie on 16 different 16-byte slots; rows of one k keep it at
@@ -354,12 +356,19 @@ template <typename T> struct Row8 {                            // eight elements
   }
 };
 
-template <int PASS, typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmArgs p) {
+// until at most `left` more stages of PER loads each are on their way (the DMA's loads land in order; left < NST)
+template <int PER, int NST> __device__ __forceinline__ void wait_stages(int left) {
+  if (NST > 3 && left >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * PER) : "memory");
+  else if (NST > 2 && left == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
+  else if (left == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+template <int PASS, typename T, int BM, int BN, int WM, int WN, int NST>
+__global__ __launch_bounds__(64 * WM * WN, NST == 2 ? 2 : 1) void gemm_tile_kernel(const GemmArgs p) {
   constexpr bool AKC = PASS != SEG_LINEAR_BWD_WEIGHT, BKC = PASS == SEG_LINEAR_FWD;
   constexpr int NWV = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * BK * 2, SLAB = 32 * 68 * 4;
-  static_assert(TN % 2 == 0 && NWV * SLAB <= 2 * STAGE, "the epilogue's slabs take 64 columns and fit the ring");
-  __shared__ __align__(1024) unsigned char smem[2 * STAGE];
+  static_assert(TN % 2 == 0 && NWV * SLAB <= NST * STAGE && NST <= 4, "the epilogue's slabs take 64 columns and fit the ring");
+  __shared__ __align__(1024) unsigned char smem[NST * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // tiles in groups of eight rows of tiles, column by column: the blocks of one XCD share operand panels in both directions
   const int t = xcd_remap(blockIdx.x, p.ti * p.tj);
@@ -402,27 +411,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmAr
     lb.issue(d + BM * BK * 2, k, kend, wave);
   };
   const int steps = (int)((kend - kbeg + BK - 1) / BK);
-  issue(0, kbeg);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  constexpr int PER = TileLoader<AKC, BM, NWV>::NI + TileLoader<BKC, BN, NWV>::NI;
+  const int ahead = steps < NST ? steps : NST;
+#pragma unroll
+  for (int st = 0; st < NST; ++st)
+    if (st < ahead) issue(st, kbeg + st * BK);
+  wait_stages<PER, NST>(ahead - 1);
   ring_release_barrier();
-  if (steps > 1) issue(1, kbeg + BK);
   frags(0, smem, 0);
-  int64_t knext = kbeg + 2 * BK;
+  int64_t knext = kbeg + NST * BK;
+  int stage = 0;
   for (int it = 0; it < steps; ++it, knext += BK) {
-    const int stage = it & 1;
     const unsigned char* sa = smem + stage * STAGE;
+    const int next = stage + 1 < NST ? stage + 1 : 0;
 #pragma unroll
     for (int ks = 1; ks < BK / 16; ++ks) {
       frags(ks & 1, sa, ks);
       contract((ks - 1) & 1);
     }
     if (it + 1 < steps) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      wait_stages<PER, NST>(steps - it - 2 < NST - 2 ? steps - it - 2 : NST - 2);
       ring_release_barrier();                                  // the next stage has landed for every wave, this one has no readers left
-      frags(0, smem + (stage ^ 1) * STAGE, 0);
-      if (it + 2 < steps) issue(stage, knext);
+      frags(0, smem + next * STAGE, 0);
+      if (it + NST < steps) issue(stage, knext);
     }
     contract((BK / 16 - 1) & 1);
+    stage = next;
   }
   // Results leave through wave-private slabs of 32 rows x 64 columns in the ring's LDS, so that a store covers whole 128-byte lines:
   // stores straight from the accumulators (32-byte pieces of 32 rows) took 221 us instead of 172 where two tensors are written
@@ -561,21 +575,37 @@ __global__ __launch_bounds__(64 * WK) void gemm_rows_kernel(const GemmArgs p) {
   }
 }
 
-// the split ranges of k added in order, then the epilogue
-template <int PASS, typename T>
+// the split ranges of k added in a fixed order, then the epilogue: R threads per element, thread r adds ranges r, r + R, ..
+template <int PASS, typename T, int R>
 __global__ __launch_bounds__(TPB) void gemm_join_kernel(const GemmArgs p) {
+  constexpr int EPB = TPB / R;
+  __shared__ float sh[R > 1 ? TPB : 1];
+  const int r = threadIdx.x / EPB, c = threadIdx.x % EPB;
   const int64_t n = p.I * p.J, all = n + (p.db != nullptr ? p.I : 0);
-  for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < all; e += (int64_t)gridDim.x * TPB) {
-    float v = 0.f;
-    if (PASS == SEG_LINEAR_BWD_WEIGHT && e >= n) {
-      for (int s = 0; s < p.splits; ++s) v += p.part_db[s * p.I + e - n];
-      p.db[e - n] = v;
-      continue;
-    }
-    const int64_t i = e / p.J;
+  for (int64_t e0 = (int64_t)blockIdx.x * EPB; e0 < all; e0 += (int64_t)gridDim.x * EPB) {
+    const int64_t e = e0 + c, i = e / p.J;
     const int j = (int)(e - i * p.J);
-    for (int s = 0; s < p.splits; ++s) v += p.part[(s * p.I + i) * p.jp + j];
-    epilogue1<PASS, T>(p, i, j, v);
+    const bool bias = PASS == SEG_LINEAR_BWD_WEIGHT && e >= n;
+    float v = 0.f;
+    if (e < all) {
+      const float* q = bias ? p.part_db + (e - n) : p.part + i * p.jp + j;
+      const int64_t ld = bias ? p.I : p.I * p.jp;
+#pragma unroll 4
+      for (int s = r; s < p.splits; s += R) v += q[s * ld];
+    }
+    if constexpr (R > 1) {
+      __syncthreads();
+      sh[threadIdx.x] = v;
+      __syncthreads();
+      if (r == 0) {
+#pragma unroll
+        for (int k = 1; k < R; ++k) v += sh[k * EPB + c];
+      }
+    }
+    if (r == 0 && e < all) {
+      if (bias) p.db[e - n] = v;
+      else epilogue1<PASS, T>(p, i, j, v);
+    }
   }
 }
 
@@ -629,12 +659,20 @@ inline GemmPlan gemm_plan(int64_t I, int J, int64_t Kd, int dtype, bool dma) {
   const int si = g.kind == TILE_ANY ? 64 : g.kind == TILE_256 ? 256 : 128, sj = g.kind == TILE_NARROW ? 64 : si;
   g.ti = (int)((I + si - 1) / si);
   g.tj = (J + sj - 1) / sj;
-  const int64_t tiles = (int64_t)g.ti * g.tj, room = g.kind == TILE_256 ? 256 : g.kind == TILE_128 ? 512 : 1024;
-  // fewer tiles than the card has room for: k is split, down to 512 of it per block (a second launch joins the parts: 1111 x 333 x 700,
-  // f16: 14 us in one launch, 16 in two)
+  const int64_t tiles = (int64_t)g.ti * g.tj, room = g.kind == TILE_ANY ? 1024 : 256, most = Kd / 512;
+  // fewer tiles than the card has room for: k is split, down to 512 of it per block, and a second launch joins the parts (1111 x 333 x 700,
+  // f16: 14 us in one launch, 16 in two).  Half a microsecond per step of 64 and block against 5 us for the second launch and 8 bytes
+  // per element and range written and read again (at 4 TB/s): as many ranges as level the two.  Against filling every CU twice
+  // (f16): 2048 x 2048 x 2048 42 -> 25 us, 1024 x 1024 x 1024 18.6 -> 14.3, 128 x 4096 x 4096 21.1 -> 19.2
   int64_t s = tiles * 2 > room || tiles == 0 ? 1 : room / tiles;
-  if (s > Kd / 512) s = Kd / 512;
+  if (s > most) s = most;
   if (s > 256) s = 256;
+  if (g.kind == TILE_128 || g.kind == TILE_NARROW) {
+    const double us = 0.55 * (double)Kd / 64, join = (double)I * J * 2e-6;
+    const int64_t level = (int64_t)(sqrt(us / join) + 0.5);
+    if (s > level) s = level;
+    if (s > 1 && us / s + 5 + s * join > us) s = 1;
+  }
   if (s < 1) s = 1;
   const int64_t step = g.kind != TILE_ANY ? 64 : dtype == SEG_DT_F32 ? 16 : 32;
   g.kper = ((Kd + s - 1) / s + step - 1) / step * step;
@@ -690,11 +728,18 @@ inline DmaPlan dma_plan(const seg_linear_args& a, int pass) {
   d.b_elems = d.b ? elems(B) : 0;
   return d;
 }
-// up to 64 rows forward, every row of both operands in 16-byte pieces
+// Up to 64 rows forward, every row of both operands in 16-byte pieces, go to gemm_rows_kernel where one launch gains more than its blocks
+// lose: a block walks all of k (16 rows f16: 1.7 us per 1024 of it, four times that for 64 rows) and reads all of x again.  Against the
+// kernels with split sums (f16): 16 x 4096 x 4096 10 us and 14, 32 x 1024 x 4096 13 and 14, 64 x 4096 x 1024 10 and 13.4; beyond the two
+// limits 64 x 64 x 65536 276 and 14, 32 x 256 x 16384 44 and 14, 64 x 16384 x 4096 74 and 31, 32 x 8192 x 8192 45 and 27.  fp32 has
+// no faster way for many units: 1 x 16384 x 4096 57 and 89, 16 x 4096 x 16384 69 and 96.
 inline bool rows_ok(const seg_linear_args& a, int pass) {
   if (pass != SEG_LINEAR_FWD || a.M > 64) return false;
   const int64_t u = a.dtype == SEG_DT_F32 ? 4 : 8;
-  return aligned16(a.x) && aligned16(a.w) && a.x_ld % u == 0 && a.w_ld % u == 0 && a.K % u == 0;
+  if (!(aligned16(a.x) && aligned16(a.w) && a.x_ld % u == 0 && a.w_ld % u == 0 && a.K % u == 0)) return false;
+  const int64_t groups = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  if (a.dtype == SEG_DT_F32 && groups == 1 && a.N >= 2048) return true;
+  return groups * a.K * (int64_t)dt_size(a.dtype) <= 16384 && groups * a.K * a.N <= (int64_t)1 << 25;
 }
 inline GemmPlan plan_of(const seg_linear_args& a, int pass) {
   const Extents e = extents(a, pass);
@@ -763,17 +808,24 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
       }
     } else if (g.kind != TILE_ANY) {
       if constexpr (!std::is_same<T, float>::value) {
-        if (g.kind == TILE_NARROW) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 64, 2, 1>), grid, dim3(128), 0, st, p);
-        else if (g.kind == TILE_256) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 256, 256, 2, 4>), grid, dim3(512), 0, st, p);
-        else hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, 128, 128, 2, 2>), grid, dim3(256), 0, st, p);
+        // a block that has its CU to itself keeps three steps on their way instead of one
+        const bool deep = (int64_t)g.ti * g.tj * g.splits <= 256;
+#define TILE_CASE(bm, bn, wm, wn, nst) hipLaunchKernelGGL((gemm_tile_kernel<PASS, T, bm, bn, wm, wn, nst>), grid, dim3(64 * wm * wn), 0, st, p)
+        if (g.kind == TILE_256) TILE_CASE(256, 256, 2, 4, 2);
+        else if (g.kind == TILE_NARROW) { if (deep) TILE_CASE(128, 64, 2, 1, 4); else TILE_CASE(128, 64, 2, 1, 2); }
+        else { if (deep) TILE_CASE(128, 128, 2, 2, 4); else TILE_CASE(128, 128, 2, 2, 2); }
+#undef TILE_CASE
       }
     } else if (vec == 4) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 4>), grid, dim3(TPB), 0, st, p);
     else if (vec == 8) {
       if constexpr (!std::is_same<T, float>::value) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 8>), grid, dim3(TPB), 0, st, p);
     } else hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 1>), grid, dim3(TPB), 0, st, p);
     if (g.splits > 1) {
-      const int64_t blocks = (p.I * (p.J + (p.db != nullptr ? 1 : 0)) + TPB - 1) / TPB;
-      hipLaunchKernelGGL((gemm_join_kernel<PASS, T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(TPB), 0, st, p);
+      const bool wide = g.splits >= 32;
+      const int64_t per = wide ? TPB / 8 : TPB, blocks = (p.I * (p.J + (p.db != nullptr ? 1 : 0)) + per - 1) / per;
+      const dim3 jg((unsigned)(blocks < 4096 ? blocks : 4096));
+      if (wide) hipLaunchKernelGGL((gemm_join_kernel<PASS, T, 8>), jg, dim3(TPB), 0, st, p);
+      else hipLaunchKernelGGL((gemm_join_kernel<PASS, T, 1>), jg, dim3(TPB), 0, st, p);
     }
   });
   return SEG_OK;
