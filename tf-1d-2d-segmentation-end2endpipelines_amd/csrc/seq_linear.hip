@@ -76,10 +76,10 @@ __device__ __forceinline__ void store_sums(const GemmArgs& p, const f16v& acc, i
 
 // ---- the kernel for every size, stride and type: 64 x 64 tiles, four waves of one 32 x 32 tile each, operands through registers into the
 // LDS in the order they have in memory - rows of BK along k (LD elements apart), or BK rows of 64 along i / j (LDT apart: the four rows of
-// a transposing 16-bit read fall into four 64-byte quarters of the banks; 32-bit fragments are single elements either way).  VEC: elements
-// per memory access - what the addresses' alignment allows; the ends of rows and of k go element by element.
+// a transposing 16-bit read fall into four 64-byte quarters of the banks; 32-bit fragments are single elements there, rows that are four
+// apart lie in different halves of them).  VEC: elements per memory access - what the addresses' alignment allows; the ends of rows and of k go element by element.
 template <typename T> struct AnyStep { static constexpr int BK = 32, EPT = 8, LD = 40, LDT = 96, SIZE = 32 * 96; };
-template <> struct AnyStep<float> { static constexpr int BK = 16, EPT = 4, LD = 20, LDT = 68, SIZE = 64 * 20; };
+template <> struct AnyStep<float> { static constexpr int BK = 16, EPT = 4, LD = 20, LDT = 72, SIZE = 64 * 20; };
 
 // 16 bytes of elements, kept in their memory format until they are put into the LDS (unpacked earlier they would be waited for earlier)
 template <typename T, int VEC> __device__ __forceinline__ u4 load_elems(const T* p) {
@@ -143,7 +143,15 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
     const u2 l = __builtin_bit_cast(u2, lo), h = __builtin_bit_cast(u2, hi);
     return u4{l[0], l[1], h[0], h[1]};
   };
-  auto elem = [&](const T* s, bool kc, int row0, int k) -> T { return kc ? s[(row0 + fr) * S::LD + k] : s[k * S::LDT + row0 + fr]; };
+  // fp32: four of k, the two halves of a wave taking k0 + 0 .. 3 and k0 + 4 .. 7 (both operands in the same order): 16-byte reads, where
+  // single elements took 172 us instead of 149 (2048 x 2048 x 2048, fp32; the matrix rate's floor 112)
+  auto elem4 = [&](const T* s, bool kc, int row0, int k0) -> f4 {
+    if (kc) return __builtin_bit_cast(f4, ld16(s + (row0 + fr) * S::LD + k0 + 4 * fh));
+    f4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = s[(k0 + 4 * fh + e) * S::LDT + row0 + fr];
+    return v;
+  };
   f16v acc, accb;
 #pragma unroll
   for (int q = 0; q < 16; ++q) acc[q] = accb[q] = 0.f;
@@ -154,10 +162,13 @@ __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
     const T *sa = smem[buf][0], *sb = smem[buf][1];
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-      for (int ks = 0; ks < S::BK / 2; ++ks) {
-        const float a = elem(sa, AKC, wi, 2 * ks + fh);
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, elem(sb, BKC, wj, 2 * ks + fh), acc, 0, 0, 0);
-        if (PASS == SEG_LINEAR_BWD_WEIGHT && sums) accb = __builtin_amdgcn_mfma_f32_32x32x2f32(a, 1.f, accb, 0, 0, 0);
+      for (int ks = 0; ks < S::BK / 8; ++ks) {
+        const f4 a = elem4(sa, AKC, wi, 8 * ks), b = elem4(sb, BKC, wj, 8 * ks);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
+          if (PASS == SEG_LINEAR_BWD_WEIGHT && sums) accb = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], 1.f, accb, 0, 0, 0);
+        }
       }
     } else {
 #pragma unroll
