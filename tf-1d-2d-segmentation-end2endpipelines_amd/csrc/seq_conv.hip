@@ -22,15 +22,7 @@ struct ConvDims { int B, L, D, act; };
 template <typename T, bool VEC> struct Raw {
   typedef T tv __attribute__((ext_vector_type(8)));
   tv v;
-  __device__ __forceinline__ void load(const T* p, int n) {
-    if constexpr (VEC) {
-      v = tv{};
-      if (n > 0) v = *reinterpret_cast<const tv*>(p);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (T)0.f;
-    }
-  }
+  __device__ __forceinline__ void load(const T* p, int n) { v = raw_load8<T, VEC>(p, n); }
   __device__ __forceinline__ float operator[](int j) const { return (float)v[j]; }
 };
 // rows of xx = [state; x]: r < 0 is state row K - 1 + r.  x rows at or behind the length are not read

@@ -77,27 +77,20 @@ __device__ __forceinline__ void store_sums(const GemmArgs& p, const f16v& acc, i
 // ---- the kernel for every size, stride and type: 64 x 64 tiles, four waves of one 32 x 32 tile each, operands through registers into the
 // LDS in the order they have in memory - rows of BK along k (LD elements apart), or BK rows of 64 along i / j (LDT apart: the four rows of
 // a transposing 16-bit read fall into four 64-byte quarters of the banks; 32-bit fragments are single elements there, rows that are four
-// apart lie in different halves of them).  VEC: elements per memory access - what the addresses' alignment allows; the ends of rows and of k go element by element.
+// apart lie in different halves of them).  VEC: 16-byte rows; otherwise the same accesses at
+// any element's address.  The ends of rows and of k go element by element.
 template <typename T> struct AnyStep { static constexpr int BK = 32, EPT = 8, LD = 40, LDT = 96, SIZE = 32 * 96; };
 template <> struct AnyStep<float> { static constexpr int BK = 16, EPT = 4, LD = 20, LDT = 72, SIZE = 64 * 20; };
 
 // 16 bytes of elements, kept in their memory format until they are put into the LDS (unpacked earlier they would be waited for earlier)
-template <typename T, int VEC> __device__ __forceinline__ u4 load_elems(const T* p) {
-  constexpr int EPT = AnyStep<T>::EPT;
-  if constexpr (VEC == EPT) return ld16(p);
-  else if constexpr (VEC * sizeof(T) == 8) {
-    const u2 a = *reinterpret_cast<const u2*>(p), b = *reinterpret_cast<const u2*>(p + VEC);
-    return u4{a[0], a[1], b[0], b[1]};
-  } else {
-    typedef T tv __attribute__((ext_vector_type(EPT)));
-    tv v;
-#pragma unroll
-    for (int t = 0; t < EPT; ++t) v[t] = p[t];
-    return __builtin_bit_cast(u4, v);
-  }
+template <typename T, bool VEC> __device__ __forceinline__ u4 load_elems(const T* p) {
+  if constexpr (VEC) return ld16(p);
+  u4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
 }
 
-template <int PASS, typename T, int VEC>
+template <int PASS, typename T, bool VEC>
 __global__ __launch_bounds__(TPB) void gemm_any_kernel(const GemmArgs p) {
   typedef AnyStep<T> S;
   constexpr bool AKC = PASS != SEG_LINEAR_BWD_WEIGHT, BKC = PASS == SEG_LINEAR_FWD;
@@ -356,10 +349,7 @@ template <typename T> struct Row8 {                            // eight elements
   tv v;
   __device__ __forceinline__ void load(const T* p, int n, bool vec) {
     if (vec) v = *reinterpret_cast<const tv*>(p);
-    else {
-#pragma unroll
-      for (int t = 0; t < 8; ++t) v[t] = t < n ? p[t] : (T)0.f;
-    }
+    else v = raw_load8<T, false>(p, n);
   }
   __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
@@ -518,12 +508,8 @@ __global__ __launch_bounds__(TPB) void pack_rows_kernel(const T* x, int64_t ld, 
   const int64_t n = rows * (ld8 / 8);
   for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < n; e += (int64_t)gridDim.x * TPB) {
     const int64_t r = e / (ld8 / 8), c = (e - r * (ld8 / 8)) * 8;
-    typedef T tv __attribute__((ext_vector_type(8)));
-    tv v;
-    const T* p = x + r * ld + c;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) v[t] = c + t < cols ? p[t] : (T)0.f;
-    *reinterpret_cast<tv*>(o + r * ld8 + c) = v;
+    const auto v = raw_load8<T, false>(x + r * ld + c, (int)(cols - c));
+    st16(o + r * ld8 + c, __builtin_bit_cast(u4, v));
   }
 }
 
@@ -698,14 +684,6 @@ inline Extents extents(const seg_linear_args& a, int pass) {
   return {a.M, a.K, a.N};
 }
 
-inline int vec_of(const void* A, int64_t a_ld, const void* B, int64_t b_ld, int dt) {
-  const int es = (int)dt_size(dt);
-  for (int v = dt == SEG_DT_F32 ? 4 : 8; v >= 4; v >>= 1) {
-    if ((uintptr_t)A % (v * es) == 0 && (uintptr_t)B % (v * es) == 0 && a_ld % v == 0 && b_ld % v == 0) return v;
-  }
-  return 1;
-}
-
 // What the LDS-DMA tile kernels take of a pass: 16-bit operands in 16-byte rows (k-contiguous ones also a whole number of 8 inputs),
 // offsets inside a tile below 2 GiB.  A product of 2^32 operations or more whose operands do not fit is worth a packed copy of them
 // (16384 x 4095 x 4095 f16: 2118 us without, 780 with copies; its backward pass 7473 and
@@ -804,7 +782,7 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
     if (d.b) { p.b_ld = pack(operand_b(a, PASS), to + d.a_elems); p.B = to + d.a_elems; }
   }
   const dim3 grid((unsigned)(g.ti * g.tj), (unsigned)g.splits);
-  const int vec = vec_of(p.A, p.a_ld, p.B, p.b_ld, a.dtype);
+  const bool vec = vec_ok(p.A, p.a_ld, 0, a.dtype) && vec_ok(p.B, p.b_ld, 0, a.dtype);
   seq_dispatch_dtype(a.dtype, [&](auto* tp) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
     if (g.kind == FEW_ROWS) {
@@ -827,10 +805,8 @@ int run_gemm(const seg_linear_args& a, GemmArgs& p, hipStream_t st) {
         else { if (deep) TILE_CASE(128, 128, 2, 2, 4); else TILE_CASE(128, 128, 2, 2, 2); }
 #undef TILE_CASE
       }
-    } else if (vec == 4) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 4>), grid, dim3(TPB), 0, st, p);
-    else if (vec == 8) {
-      if constexpr (!std::is_same<T, float>::value) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 8>), grid, dim3(TPB), 0, st, p);
-    } else hipLaunchKernelGGL((gemm_any_kernel<PASS, T, 1>), grid, dim3(TPB), 0, st, p);
+    } else if (vec) hipLaunchKernelGGL((gemm_any_kernel<PASS, T, true>), grid, dim3(TPB), 0, st, p);
+    else hipLaunchKernelGGL((gemm_any_kernel<PASS, T, false>), grid, dim3(TPB), 0, st, p);
     if (g.splits > 1) {
       const bool wide = g.splits >= 32;
       const int64_t per = wide ? TPB / 8 : TPB, blocks = (p.I * (p.J + (p.db != nullptr ? 1 : 0)) + per - 1) / per;

@@ -125,15 +125,7 @@ template <bool VEC> __device__ __forceinline__ void load_chan(const float* p, in
 template <typename T, bool VEC> struct Raw {
   typedef T tv __attribute__((ext_vector_type(8)));
   tv v;
-  __device__ __forceinline__ void load(const T* p, int n) {
-    if constexpr (VEC) {
-      if (n > 0) v = *reinterpret_cast<const tv*>(p);
-      else v = tv{};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (T)0.f;
-    }
-  }
+  __device__ __forceinline__ void load(const T* p, int n) { v = raw_load8<T, VEC>(p, n); }
   __device__ __forceinline__ float operator[](int j) const { return (float)v[j]; }
 };
 template <typename T, int G> struct RawStates {
@@ -285,6 +277,7 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_arg
 }
 
 // the chunks in order: in place, a chunk's own last state becomes the state in front of it
+constexpr int JOIN = 8;          // chunks whose parts are on their way together (1 x 100000 x 64 x 16, 1563 chunks: 535 us one at a time, 200)
 __global__ __launch_bounds__(256) void scan_join_kernel(const seg_scan_args p, int nch, float* start, const float* sumd) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)p.D * p.S;
   const int b = blockIdx.y;
@@ -292,16 +285,23 @@ __global__ __launch_bounds__(256) void scan_join_kernel(const seg_scan_args p, i
   const int64_t d = e / p.S;
   const float A2 = p.A[e] * LOG2E;
   float h = p.state != nullptr ? p.state[b * n + e] : 0.f;
-  for (int k = 0; k < nch; ++k) {
-    const int64_t o = (int64_t)b * nch + k;
-    if (k == nch - 1) {                                        // (its own last state was not computed: nothing starts behind it)
-      start[o * n + e] = h;
-      return;
-    }
-    const float own = start[o * n + e];
-    start[o * n + e] = h;
-    h = fmaf(exp2_f(A2 * sumd[o * p.D + d]), h, own);
+  const int64_t o0 = (int64_t)b * nch;
+  for (int k0 = 0; k0 < nch - 1; k0 += JOIN) {
+    float own[JOIN], a[JOIN];
+#pragma unroll
+    for (int k = 0; k < JOIN; ++k)
+      if (k0 + k < nch - 1) {
+        own[k] = start[(o0 + k0 + k) * n + e];
+        a[k] = sumd[(o0 + k0 + k) * p.D + d];
+      }
+#pragma unroll
+    for (int k = 0; k < JOIN; ++k)
+      if (k0 + k < nch - 1) {
+        start[(o0 + k0 + k) * n + e] = h;
+        h = fmaf(exp2_f(A2 * a[k]), h, own[k]);
+      }
   }
+  start[(o0 + nch - 1) * n + e] = h;                           // (the last chunk's own last state was not computed: nothing starts behind it)
 }
 // the same for the adjoint, from the last chunk: a chunk's own part becomes the adjoint that enters it from behind
 __global__ __launch_bounds__(256) void scan_join_bwd_kernel(const seg_scan_args p, int nch, float* adj, const float* sumd) {
@@ -311,16 +311,23 @@ __global__ __launch_bounds__(256) void scan_join_bwd_kernel(const seg_scan_args 
   const int64_t d = e / p.S;
   const float A2 = p.A[e] * LOG2E;
   float q = p.dstate_out != nullptr ? p.dstate_out[b * n + e] : 0.f;
-  for (int k = nch - 1; k >= 0; --k) {
-    const int64_t o = (int64_t)b * nch + k;
-    if (k == 0) {                                              // (its own part was not computed: nothing lies in front of it)
-      adj[o * n + e] = q;
-      return;
-    }
-    const float own = adj[o * n + e];
-    adj[o * n + e] = q;
-    q = fmaf(exp2_f(A2 * sumd[o * p.D + d]), q, own);
+  const int64_t o0 = (int64_t)b * nch;
+  for (int k0 = nch - 1; k0 > 0; k0 -= JOIN) {
+    float own[JOIN], a[JOIN];
+#pragma unroll
+    for (int k = 0; k < JOIN; ++k)
+      if (k0 - k > 0) {
+        own[k] = adj[(o0 + k0 - k) * n + e];
+        a[k] = sumd[(o0 + k0 - k) * p.D + d];
+      }
+#pragma unroll
+    for (int k = 0; k < JOIN; ++k)
+      if (k0 - k > 0) {
+        adj[(o0 + k0 - k) * n + e] = q;
+        q = fmaf(exp2_f(A2 * a[k]), q, own[k]);
+      }
   }
+  adj[o0 * n + e] = q;                                         // (the first chunk's own part was not computed: nothing lies in front of it)
 }
 
 // dp = dy silu(z) of a piece
