@@ -596,7 +596,7 @@ enum { SEG_DT_F16 = 0, SEG_DT_BF16 = 1, SEG_DT_F32 = 2 };
 /* activations of the sequence operators: SEG_ACT_NONE / RELU / LEAKY / SIGMOID and                                             */
 enum { SEG_ACT_SILU = 5, SEG_ACT_GELU = 6 };                       /* v sigmoid(v);  v Phi(v) (the error function, no tanh form) */
 
-/* Layer normalisation over the C channels of every row: y = (x - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps), biased
+/* Layer normalisation over the C (<= 2^30) channels of every row: y = (x - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps), biased
  * variance.  gamma / beta NULL = 1 / 0; mean / rstd (fp32 [rows]) NULL = not wanted.  y may be x.                              */
 int seg_layernorm_fwd(const void* x, int64_t x_ld, void* y, int64_t y_ld, int64_t rows, int32_t C, int32_t dtype, const float* gamma,
                       const float* beta, float eps, float* mean, float* rstd, seg_stream_t stream);

@@ -941,3 +941,16 @@ def test_layer_norm_long_rows_and_few_blocks(rows, C, dtype):
     R.assert_close(dx, rs * (gd - gd.mean(1, keepdim=True) - xh * (gd * xh).mean(1, keepdim=True)), rs * (gd.abs() + 2 * gd.abs().mean(1, keepdim=True) * (1 + xh.abs())), n, "dx")
     R.assert_close(dg, (d64 * xh).sum(0), (d64.abs() * (xh.abs() + 1)).sum(0), n + rows, "dgamma")
     R.assert_close(db, d64.sum(0), d64.abs().sum(0), n + rows, "dbeta")
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+def test_linear_forward_from_packed_copies(dtype):
+    """A forward product large enough for copies of operands that no 16-byte access fits (2^32 products), NaN beside them."""
+    g = gen(95)
+    M, N, K = 16392, 523, 519
+    x, w, b = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype), rnd(g, N).cuda()
+    X, W = wide(x, 3, 2), wide(w, 1, 4)
+    x, w = x.cuda(), w.cuda()
+    z64, s = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t() + b.double().abs()
+    for args in ((x, w), (X, W), (x, W)):
+        R.assert_close(seq.linear(*args, b, activation="relu"), z64.clamp(min=0).cpu(), s.cpu(), K + 6, "y")

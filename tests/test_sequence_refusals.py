@@ -219,3 +219,8 @@ def test_results_in_place_keep_the_row_stride(lib):
     refused(lib, lib.seg_linear_act_bwd(FAKE, 8, 2 * FAKE, 8, FAKE, 16, 4, 8, 0, 1, 0.0, None), "in place")
     refused(lib, lib.seg_linear_fwd(linear_args(residual=FAKE, residual_ld=40), None), "in place")
     refused(lib, lib.seg_linear_bwd_data(linear_args(w_ld=32, residual=FAKE, residual_ld=40), None), "in place")
+
+
+def test_layernorm_row_length_limit(lib):
+    refused(lib, lib.seg_layernorm_fwd(FAKE, 1 << 31, 2 * FAKE, 1 << 31, 4, (1 << 30) + 1, 0, None, None, 1e-3, None, None, None), "2^30")
+    refused(lib, lib.seg_layernorm_bwd(FAKE, 1 << 31, 2 * FAKE, 1 << 31, None, 0, 4, (1 << 30) + 1, 0, FAKE, FAKE, None, FAKE, FAKE, FAKE, None), "2^30")

@@ -319,11 +319,7 @@ template <int PASS, typename T> __device__ __forceinline__ void epilogue8(const 
   if constexpr (PASS == SEG_LINEAR_BWD_WEIGHT) {
     float* o = (float*)p.out + i * p.out_ld + j;
     if (vec) store8<float>(o, v);
-    else {
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-        if (t < n) o[t] = v[t];
-    }
+    else row_store8<float, false>(o, n, v);
   } else {
     if constexpr (PASS == SEG_LINEAR_FWD) {
 #pragma unroll
@@ -685,9 +681,8 @@ inline Extents extents(const seg_linear_args& a, int pass) {
 }
 
 // What the LDS-DMA tile kernels take of a pass: 16-bit operands in 16-byte rows (k-contiguous ones also a whole number of 8 inputs),
-// offsets inside a tile below 2 GiB.  A product of 2^32 operations or more whose operands do not fit is worth a packed copy of them
-// (16384 x 4095 x 4095 f16: 2118 us without, 780 with copies; its backward pass 7473 and
-// 1412).  dma: 0 no, 1 as they are, 2 with copies (a, b: which)
+// offsets inside a tile below 2 GiB.  A large product whose operands do not fit is worth a packed copy of them (16384 x 4095 x 4095 f16:
+// 2012 us without, 553 with; its gradients 2439 and 550, 2838 and 598).  dma: 0 no, 1 as they are, 2 with copies (a, b: which)
 struct Operand { const void* p; int64_t ld, rows, cols; bool kc; };
 struct DmaPlan { int dma; bool a, b; int64_t a_elems, b_elems; };
 inline Operand operand_a(const seg_linear_args& a, int pass) {
@@ -709,8 +704,12 @@ inline DmaPlan dma_plan(const seg_linear_args& a, int pass) {
   d.a = !fits(A);
   d.b = !fits(B);
   if (!d.a && !d.b) { d.dma = 1; return d; }
-  // (an element's copy costs what 130 products of it cost the other kernel: 16384 x 63 x 4001 took 47 us without copies, 118 with)
-  if (e.I < 256 || e.J < 256 || (double)e.I * e.J * e.Kd < 2147483648.0) return d;
+  // A copy pays where enough products share it, sooner for operands along i / j, which the other kernel transposes at a quarter of the
+  // tile kernel's pace.  Without and with (f16): forward 8192 x 519 x 523 24 and 28 us, 16384 x 1001 x 1003 103 and 59, 16384 x 63 x 4001
+  // 43 and 77; data gradients 2000 x 1001 x 777 37 and 25, 500 x 301 x 1203 14 and 17; weight gradients 46 and 27, 18 and 19
+  const double products = (double)e.I * e.J * e.Kd;
+  if (pass == SEG_LINEAR_FWD ? e.I < 256 || products < 4294967296.0 : products < 1073741824.0) return d;
+  if (e.J < 256) return d;
   d.dma = 2;
   auto elems = [](const Operand& o) { return o.rows * ((o.cols + 7) / 8 * 8); };
   d.a_elems = d.a ? elems(A) : 0;
