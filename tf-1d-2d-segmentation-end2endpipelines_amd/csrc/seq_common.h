@@ -1,5 +1,5 @@
-// Shared pieces of the sequence operators (seq_norm.hip, seq_linear.hip, seq_scan.hip): element types fp16 / bf16 / fp32, vector
-// access with a scalar form for rows that no 16-byte access fits, activations, and the ordered reduction of per-block partial rows.
+// Shared pieces of the sequence operators (seq_norm.hip, seq_linear.hip, seq_conv.hip, seq_scan.hip): element types fp16 / bf16 / fp32,
+// row access in pieces of eight at aligned and at any addresses, activations, and the ordered reduction of per-block partial rows.
 #pragma once
 #include "seg_common.h"
 #include <math.h>
