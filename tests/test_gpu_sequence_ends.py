@@ -1,0 +1,108 @@
+"""GPU: the sequence operators at the ends of their ranges - infinities and NaN in activations, constant rows, empty and very long
+extents, gradients of weights whose every row counts."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs an MI355X", allow_module_level=True)
+
+from segamd import sequence as seq
+
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+IDS = ["f16", "bf16", "f32"]
+INF = float("inf")
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rnd(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+# rows, units and inputs that every kernel of the product meets: few rows, any size, 128 x 64, 128 x 128 and 256 x 256 tiles
+KERNELS = [(4, 64, 64), (100, 40, 33), (200, 64, 64), (130, 136, 64), (12360, 1032, 136)]
+ACTIVATIONS = ["relu", "leaky_relu", "sigmoid", "silu", "gelu"]
+
+
+# ---------------------------------------------------------------------------------------------------- activations at infinity
+@pytest.mark.parametrize("name", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_activations_of_infinity_are_their_limits(name, dtype):
+    """z = bias here (x is zero).  At +-inf an activation takes its limit; a finite value next to them keeps its own.  1e-5: an exponential's
+    argument of up to 40 carries 40 half steps of 2^-24 each way, a few times over; one step of the type where it is stored."""
+    for M, N, K in KERNELS:
+        v = torch.tensor([INF, -INF, 3e38, -3e38, 1e4, -1e4, 40.0, -40.0]).repeat(N // 8)
+        want = {"relu": torch.relu, "leaky_relu": lambda t: torch.where(t > 0, t, t * 0.3), "sigmoid": torch.sigmoid,
+                "silu": lambda t: torch.where(t < -1e3, 0.0, t * torch.sigmoid(t)),
+                "gelu": lambda t: torch.where(t < -1e3, 0.0, 0.5 * t * torch.special.erfc(-t * 0.5 ** 0.5))}[name](v.double()).to(dtype).float()
+        y, z = seq.linear(torch.zeros(M, K, dtype=dtype, device="cuda"), torch.ones(N, K, dtype=dtype, device="cuda"), v.cuda(), activation=name,
+                          preactivation=True)
+        assert torch.equal(z.cpu(), v.to(dtype).expand(M, N))
+        assert torch.allclose(y.float().cpu(), want.expand(M, N), rtol=max(1e-5, torch.finfo(dtype).eps), atol=2.0 ** -24), (M, N, K)
+
+
+@pytest.mark.parametrize("name", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_slopes_at_infinity_are_their_limits(name, dtype):
+    """A kept pre-activation that overflowed its type: the gradient through it is the one through any large value of that sign."""
+    g = gen(61)
+    for M, K, N in KERNELS:
+        dy, w, x = rnd(g, M, N, dtype=dtype), rnd(g, N, K, dtype=dtype), rnd(g, M, K, dtype=dtype)
+        z = rnd(g, M, K, dtype=dtype)
+        far = torch.rand(M, K, generator=g).cuda()
+        big, z = (torch.where(far < 0.2, v, torch.where(far > 0.8, -v, z.float())).to(dtype) for v in (1e4, INF))
+        assert torch.isinf(z).any()
+        got, want = (seq.linear_backward(dy, x, w, z=t, activation=name, need_dw=False, need_db=False)[0] for t in (z, big))
+        assert torch.isfinite(got).all() and torch.equal(got, want), (M, N, K)
+        d = torch.ones_like(z)
+        got = seq.activation_backward(d, z, name)
+        assert torch.equal(got, seq.activation_backward(d, big, name))
+        up, down = {"relu": (1, 0), "leaky_relu": (1, 0.3), "sigmoid": (0, 0), "silu": (1, 0), "gelu": (1, 0)}[name]
+        assert torch.equal(got[z == INF], torch.full_like(got[z == INF], up)) and torch.equal(got[z == -INF], torch.full_like(got[z == -INF], down))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("D", [24, 13])
+def test_causal_conv_at_infinity(D, dtype):
+    """The convolution's silu at +-inf (by way of the bias): limits forward, finite gradients backward."""
+    g = gen(62)
+    B, L, K = 2, 37, 4
+    x, dy, w, st = rnd(g, B, L, D, dtype=dtype), rnd(g, B, L, D, dtype=dtype), rnd(g, K, D), rnd(g, B, K - 1, D, dtype=dtype)
+    far = torch.arange(D).cuda() % 3
+    big, bias = (torch.where(far == 0, v, torch.where(far == 1, -v, 0.1)).cuda() for v in (torch.tensor(1e4).cuda(), torch.tensor(INF).cuda()))
+    y, _ = seq.causal_conv(x, w, bias, activation="silu", state=st)
+    want, _ = seq.causal_conv(x, w, big, activation="silu", state=st)
+    assert torch.equal(y[..., far != 0], want[..., far != 0]) and torch.isposinf(y[..., far == 0]).all() and not y[..., far == 1].any()
+    for p, q in zip(seq.causal_conv_backward(dy, x, w, bias, activation="silu", state=st), seq.causal_conv_backward(dy, x, w, big, activation="silu", state=st)):
+        assert torch.isfinite(p).all() and torch.equal(p, q)
+    ys = seq.causal_conv_step(x[:, 0], st.clone(), w, bias, activation="silu")
+    assert torch.equal(ys, y[:, 0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("B,L,D,S", [(2, 40, 24, 5), (1, 300, 13, 16), (1, 150, 20, 40)])
+def test_selective_scan_gates_at_infinity(B, L, D, S, dtype):
+    """A gate of -inf shuts (outputs and gradients as with any gate far below zero); one of +inf leaves dz finite."""
+    g = gen(63)
+    u, dt, z, dy = (rnd(g, B, L, D, dtype=dtype) for _ in range(4))
+    Bm, Cm = rnd(g, B, L, S, dtype=dtype), rnd(g, B, L, S, dtype=dtype)
+    A, skip = -(torch.rand(D, S, generator=g) + 0.2).cuda(), rnd(g, D)
+    far = torch.rand(B, L, D, generator=g).cuda()
+    shut = far < 0.2
+    big, low = (torch.where(shut, v, z.float()).to(dtype) for v in (-1e4, -INF))
+    y, last, saved = seq.selective_scan(u, dt, A, Bm, Cm, D=skip, z=low, training=True)
+    want, _, _ = seq.selective_scan(u, dt, A, Bm, Cm, D=skip, z=big, training=True)
+    assert torch.equal(y, want) and not y[shut].any()
+    for p, q in zip(*(seq.selective_scan_backward(dy, u, dt, A, Bm, Cm, saved, D=skip, z=t) for t in (low, big))):
+        assert p is None or (torch.isfinite(p).all() and torch.equal(p, q))
+    big, high = (torch.where(shut, v, z.float()).to(dtype) for v in (1e4, INF))
+    p, q = (seq.selective_scan_backward(dy, u, dt, A, Bm, Cm, saved, D=skip, z=t).dz for t in (high, big))
+    assert torch.isfinite(p).all() and torch.equal(p, q)
+    st = rnd(g, B, D, S)
+    p, q = (seq.selective_scan_step(u[:, 0], dt[:, 0], A, Bm[:, 0], Cm[:, 0], st, D=skip, z=t, new_state=torch.empty_like(st))
+            for t in (torch.full_like(z[:, 0], -INF), torch.full_like(z[:, 0], -1e4)))
+    assert torch.equal(p, q) and not p.any()

@@ -87,12 +87,19 @@ template <typename T, bool VEC> __device__ __forceinline__ void row_store8(T* p,
 }
 
 __device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
-// h = Phi(-|v|) = erfc(|v| / sqrt 2) / 2 and e = exp(-v^2 / 2).  erfc(x) exp(x^2) = t P(t) with t = 1 / (1 + 0.3 x), P of degree 8 fitted to a
-// relative error of 2e-8 on 0 <= x <= 9.5 (behind it both factors are 0 in 32 bits): the left tail keeps its relative precision, which
-// 1 + erf loses, at about 20 instructions - half of the library's erff, and the derivative's Gaussian comes with it.
-__device__ __forceinline__ float phi_neg(float v, float& e) {
+// At +-inf the activations and their slopes take their limits: a factor v meets one that is 0 in 32 bits from |v| = 100 on, and inf * 0
+// would be NaN.  The factor is cut far behind that - no finite v changes its result -, and a NaN stays one by way of the other factor.
+constexpr float ACT_FAR = 128.f;
+__device__ __forceinline__ float silu_f(float v) { return __builtin_amdgcn_fmed3f(v, -ACT_FAR, INFINITY) * sigmoid_f(v); }
+__device__ __forceinline__ float silu_slope_f(float v) { const float s = sigmoid_f(v); return s * (1.f + __builtin_amdgcn_fmed3f(v, -ACT_FAR, ACT_FAR) * (1.f - s)); }
+// Phi(-|v|) = erfc(|v| / sqrt 2) / 2 = Q e with e = exp(-v^2 / 2), and ve = |v| e.  erfc(x) exp(x^2) = t P(t) with t = 1 / (1 + 0.3 x), P of degree 8
+// fitted to a relative error of 2e-8 on 0 <= x <= 9.5 (behind it both factors are 0 in 32 bits): the left tail keeps its relative precision,
+// which 1 + erf loses, at about 20 instructions - half of the library's erff, and the derivative's Gaussian comes with it.
+// 0 <= ve <= 0.61: cut to [0, 1] - a modifier of the product's instruction - it is what it was, but for inf * 0, which becomes 0.
+__device__ __forceinline__ float phi_neg(float v, float& e, float& ve) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.21213203435596426f, fabsf(v), 1.f));
   e = __builtin_amdgcn_exp2f(-0.72134752044448170f * v * v);
+  ve = __builtin_amdgcn_fmed3f(fabsf(v) * e, 0.f, 1.f);
   float P = -0.12943415125844135f;
   P = fmaf(P, t, 0.48509680347354195f);
   P = fmaf(P, t, -0.5112271909366609f);
@@ -102,7 +109,7 @@ __device__ __forceinline__ float phi_neg(float v, float& e) {
   P = fmaf(P, t, 0.1484823543501283f);
   P = fmaf(P, t, 0.17069194623730768f);
   P = fmaf(P, t, 0.16918961408577482f);
-  return 0.5f * t * P * e;
+  return 0.5f * t * P;
 }
 
 __device__ __forceinline__ float seq_act(float v, int act, float alpha) {
@@ -110,8 +117,8 @@ __device__ __forceinline__ float seq_act(float v, int act, float alpha) {
     case SEG_ACT_RELU: return v > 0.f ? v : 0.f;
     case SEG_ACT_LEAKY: return v > 0.f ? v : v * alpha;
     case SEG_ACT_SIGMOID: return sigmoid_f(v);
-    case SEG_ACT_SILU: return v * sigmoid_f(v);
-    case SEG_ACT_GELU: { float e; const float h = phi_neg(v, e); return fmaf(-fabsf(v), h, fmaxf(v, 0.f)); }      // v Phi(v)
+    case SEG_ACT_SILU: return silu_f(v);
+    case SEG_ACT_GELU: { float e, ve; const float Q = phi_neg(v, e, ve); return fmaf(-Q, ve, fmaxf(v, 0.f)); }      // v Phi(v)
     default: return v;
   }
 }
@@ -121,8 +128,12 @@ __device__ __forceinline__ float seq_act_slope(float v, int act, float alpha) {
     case SEG_ACT_RELU: return v > 0.f ? 1.f : 0.f;
     case SEG_ACT_LEAKY: return v > 0.f ? 1.f : alpha;
     case SEG_ACT_SIGMOID: { const float s = sigmoid_f(v); return s * (1.f - s); }
-    case SEG_ACT_SILU: { const float s = sigmoid_f(v); return s * (1.f + v * (1.f - s)); }
-    case SEG_ACT_GELU: { float e; const float h = phi_neg(v, e); return fmaf(v * 0.39894228040143268f, e, v < 0.f ? h : 1.f - h); }
+    case SEG_ACT_SILU: return silu_slope_f(v);
+    case SEG_ACT_GELU: {                                       // g: the slope at -|v|; the two add up to 1
+      float e, ve;
+      const float Q = phi_neg(v, e, ve), g = fmaf(ve, -0.39894228040143268f, Q * e);
+      return v < 0.f ? g : 1.f - g;
+    }
     default: return 1.f;
   }
 }

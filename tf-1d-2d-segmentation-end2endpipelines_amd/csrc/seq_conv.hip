@@ -40,7 +40,7 @@ __device__ __forceinline__ int conv_len(const seg_causal_conv_args& p, int b) {
   const int n = p.lengths[b];
   return n < 0 ? 0 : n > p.L ? p.L : n;
 }
-__device__ __forceinline__ float conv_act(float v, int act) { return act == SEG_ACT_SILU ? v * sigmoid_f(v) : v; }
+__device__ __forceinline__ float conv_act(float v, int act) { return act == SEG_ACT_SILU ? silu_f(v) : v; }
 
 // threads: 32 channel groups of 8 x 8 runs of RUNS rows; grid (channels / 256, runs / 8, B).  A run's rows are all on their way before the
 // first is used: one memory latency per run
@@ -132,8 +132,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const seg_causal_conv_arg
             float v = bias[j];
 #pragma unroll
             for (int k = 0; k < K; ++k) v = fmaf(w[k][j], x[i + k][j], v);
-            const float s = sigmoid_f(v);
-            d[j] *= s * (1.f + v * (1.f - s));
+            d[j] *= silu_slope_f(v);
           }
           d[j] = r < len ? d[j] : 0.f;
           dv[K - 1][j] = d[j];

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_arg
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 y[j] = fmaf(skip[j], cu[i][j], sy[r][q0c + j]);
-                if (p.z != nullptr) y[j] *= cz[i][j] * sigmoid_f(cz[i][j]);
+                if (p.z != nullptr) y[j] *= silu_f(cz[i][j]);
               }
             }
             row_store8<T, VEC>((T*)p.y + b * p.y_bs + t * p.y_ld + tc, tn, y);
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256) void scan_join_bwd_kernel(const seg_scan_args 
 // dp = dy silu(z) of a piece
 template <typename T, bool VEC>
 __device__ __forceinline__ float dp_of(const seg_scan_args& p, const Raw<T, VEC>& dy, const Raw<T, VEC>& z, int j) {
-  return p.z != nullptr ? dy[j] * z[j] * sigmoid_f(z[j]) : dy[j];
+  return p.z != nullptr ? dy[j] * silu_f(z[j]) : dy[j];
 }
 
 // a chunk's own part of the adjoint in front of it, and its sum of delta (chunks 1 ..: blockIdx.y + 1)
@@ -619,8 +619,7 @@ __global__ __launch_bounds__(Lay<G>::NT, 2) void scan_bwd_kernel(const seg_scan_
           if (p.dz != nullptr) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float z = cz[i][j], sg = sigmoid_f(z);
-              o[j] = cy[i][j] * fmaf(skip[j], cu[i][j], x[j][3]) * sg * (1.f + z * (1.f - sg));
+              o[j] = cy[i][j] * fmaf(skip[j], cu[i][j], x[j][3]) * silu_slope_f(cz[i][j]);
             }
             row_store8<T, VEC>((T*)p.dz + b * p.dz_bs + t * p.dz_ld + tc, tn, o);
           }
@@ -698,7 +697,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const seg_scan_args p) {
     if (p.Dskip != nullptr) y = fmaf(p.Dskip[d], u, y);
     if (p.z != nullptr) {
       const float z = (float)((const T*)p.z)[b * p.z_bs + d];
-      y *= z * sigmoid_f(z);
+      y *= silu_f(z);
     }
     ((T*)p.y)[b * p.y_bs + d] = (T)y;
   }
