@@ -595,7 +595,8 @@ int seg_unpack_f32_f32(const void* x, float* y, int64_t npix, int32_t C, int32_t
 enum { SEG_DT_F16 = 0, SEG_DT_BF16 = 1, SEG_DT_F32 = 2 };
 /* activations of the sequence operators: SEG_ACT_NONE / RELU / LEAKY / SIGMOID and                                             */
 enum { SEG_ACT_SILU = 5, SEG_ACT_GELU = 6 };                       /* v sigmoid(v);  v Phi(v) (the error function, no tanh form) */
-/* at +-inf they and their slopes take their limits (silu(-inf) = gelu(-inf) = 0; a pre-activation that overflowed its type has a slope)  */
+/* at +-inf they and their slopes take their limits (silu(-inf) = gelu(-inf) = 0; a pre-activation that overflowed its type has a
+ * slope); a NaN stays one, in SEG_ACT_RELU too                                                                                */
 
 /* Layer normalisation over the C (<= 2^30) channels of every row: y = (x - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps), biased
  * variance.  gamma / beta NULL = 1 / 0; mean / rstd (fp32 [rows]) NULL = not wanted.  y may be x.                              */

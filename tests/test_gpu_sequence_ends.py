@@ -106,3 +106,23 @@ def test_selective_scan_gates_at_infinity(B, L, D, S, dtype):
     p, q = (seq.selective_scan_step(u[:, 0], dt[:, 0], A, Bm[:, 0], Cm[:, 0], st, D=skip, z=t, new_state=torch.empty_like(st))
             for t in (torch.full_like(z[:, 0], -INF), torch.full_like(z[:, 0], -1e4)))
     assert torch.equal(p, q) and not p.any()
+
+
+# ------------------------------------------------------------------------------------------------------------ NaN through relu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_relu_keeps_nan(dtype):
+    """max(NaN, 0) is NaN, as for every other activation: a row that went wrong shows.  Its slope there is torch's (the gradient passes)."""
+    g = gen(64)
+    for M, N, K in KERNELS:
+        x, w, b = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype), rnd(g, N)
+        want = seq.linear(x, w, b, activation="relu")
+        x[M // 2, K // 2] = float("nan")
+        y = seq.linear(x, w, b, activation="relu")
+        on = torch.arange(M, device="cuda") == M // 2
+        assert torch.isnan(y[on]).all() and torch.equal(y[~on], want[~on]), (M, N, K)
+    z, dy = rnd(g, 9, 21, dtype=dtype), rnd(g, 9, 21, dtype=dtype)
+    z[4, 3], z[5, 6], z[5, 7] = float("nan"), 0.0, -0.0
+    v = z.float().cpu().requires_grad_()
+    with torch.enable_grad():
+        slope, = torch.autograd.grad(torch.relu(v).sum(), v)
+    assert torch.equal(seq.activation_backward(dy, z, "relu").float().cpu(), dy.float().cpu() * slope)

@@ -114,7 +114,7 @@ __device__ __forceinline__ float phi_neg(float v, float& e, float& ve) {
 
 __device__ __forceinline__ float seq_act(float v, int act, float alpha) {
   switch (act) {
-    case SEG_ACT_RELU: return v > 0.f ? v : 0.f;
+    case SEG_ACT_RELU: return v <= 0.f ? 0.f : v;              // (a NaN stays one, here and in the slope: the gradient passes, as torch's)
     case SEG_ACT_LEAKY: return v > 0.f ? v : v * alpha;
     case SEG_ACT_SIGMOID: return sigmoid_f(v);
     case SEG_ACT_SILU: return silu_f(v);
@@ -125,7 +125,7 @@ __device__ __forceinline__ float seq_act(float v, int act, float alpha) {
 // derivative from the activation's INPUT
 __device__ __forceinline__ float seq_act_slope(float v, int act, float alpha) {
   switch (act) {
-    case SEG_ACT_RELU: return v > 0.f ? 1.f : 0.f;
+    case SEG_ACT_RELU: return v <= 0.f ? 0.f : 1.f;
     case SEG_ACT_LEAKY: return v > 0.f ? 1.f : alpha;
     case SEG_ACT_SIGMOID: { const float s = sigmoid_f(v); return s * (1.f - s); }
     case SEG_ACT_SILU: return silu_slope_f(v);
