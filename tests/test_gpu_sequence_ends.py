@@ -126,3 +126,21 @@ def test_relu_keeps_nan(dtype):
     with torch.enable_grad():
         slope, = torch.autograd.grad(torch.relu(v).sum(), v)
     assert torch.equal(seq.activation_backward(dy, z, "relu").float().cpu(), dy.float().cpu() * slope)
+
+
+# ------------------------------------------------------------------------------------------------------------- constant rows
+@pytest.mark.parametrize("C", [1, 3, 37, 64, 200, 512, 1111, 2048, 2056, 5000, 16384, 20001, 100003])
+def test_layer_norm_of_constant_rows_is_beta(C):
+    """Rows without variance, of values whose sums round: the mean is the value, y is beta, rstd 1 / sqrt(eps) (three roundings)."""
+    g = gen(C)
+    v = torch.cat([torch.tensor([0.1, 1000.1, -3.3e-5, 7.7e7, 0.0]), torch.randn(20, generator=g) * 10.0 ** torch.randint(-3, 4, (20,), generator=g)])
+    x = v[:, None].expand(-1, C).contiguous().cuda()
+    gamma, beta = rnd(g, C), rnd(g, C)
+    for off in (0, 1):                                          # rows that 16-byte accesses fit, and rows at any address
+        rows = torch.empty(25, C + off, device="cuda")[:, off:].copy_(x) if off else x
+        y, mean, rstd = seq.layer_norm(rows, gamma, beta, eps=1e-3, stats=True)
+        assert torch.equal(mean.cpu(), v)
+        assert torch.equal(y, beta.expand_as(y))
+        assert torch.allclose(rstd.cpu(), torch.full((25,), 1e-3 ** -0.5), rtol=3 * 2.0 ** -23, atol=0)
+    dx, dg, _ = seq.layer_norm_backward(x, x, mean, rstd, gamma)
+    assert not dg.any()
