@@ -144,3 +144,20 @@ def test_layer_norm_of_constant_rows_is_beta(C):
         assert torch.allclose(rstd.cpu(), torch.full((25,), 1e-3 ** -0.5), rtol=3 * 2.0 ** -23, atol=0)
     dx, dg, _ = seq.layer_norm_backward(x, x, mean, rstd, gamma)
     assert not dg.any()
+
+
+# ------------------------------------------------------------------------------------------------------------- empty extents
+@pytest.mark.parametrize("shape", [(4, 0), (0, 4), (2, 0, 3), (1, 0)])
+def test_empty_leading_axes(shape):
+    """Extents of zero anywhere in front of the channels are calls without work; gradients of parameters are zero."""
+    x = torch.empty(shape + (8,), dtype=torch.float16, device="cuda")
+    y, mean, rstd = seq.layer_norm(x, stats=True)
+    assert y.shape == x.shape and mean.shape == shape == rstd.shape
+    dx, dg, db = seq.layer_norm_backward(x, x, mean, rstd)
+    assert dx.shape == x.shape and dg.shape == (8,) and not dg.any() and not db.any()
+    w = torch.ones(6, 8, dtype=torch.float16, device="cuda")
+    y, z = seq.linear(x, w, activation="gelu", preactivation=True, residual=torch.empty(shape + (6,), dtype=torch.float16, device="cuda"))
+    assert y.shape == z.shape == shape + (6,)
+    dx, dw, db = seq.linear_backward(y, x, w, z=x, activation="gelu", residual=x)
+    assert dx.shape == x.shape and dw.shape == (6, 8) and not dw.any() and not db.any()
+    assert seq.activation_backward(x, x, "silu").shape == x.shape

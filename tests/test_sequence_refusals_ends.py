@@ -36,3 +36,14 @@ def test_extents_that_an_int32_does_not_hold(call):
     """They would reach the C level as their low 32 bits, 8 here: refused in front of it (tensors without memory, on torch's meta device)."""
     with pytest.raises(ValueError, match="2147483647"):
         call(lambda *shape: T(*shape, device="meta"))
+
+
+# ------------------------------------------------------------------------------------------------------------- empty extents
+@pytest.mark.parametrize("shape", [(4, 0), (0, 4), (3, 0, 5), (2, 5, 0), (0, 0)])
+def test_empty_leading_axes_are_calls_without_work(shape):
+    """An extent of zero in any place in front of the channels passes the checks of strides (there are no rows to be spaced)."""
+    x, y, w = T(*shape, 8), T(*shape, 6), T(6, 8)
+    for f in (lambda: seq.layer_norm(x), lambda: seq.layer_norm_backward(x, x, T(*shape), T(*shape)), lambda: seq.linear(x, w, residual=y),
+              lambda: seq.linear_backward(y, x, w, z=x, activation="gelu", residual=x), lambda: seq.activation_backward(x, x, "silu")):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            f()

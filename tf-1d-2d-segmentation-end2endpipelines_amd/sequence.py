@@ -99,6 +99,8 @@ def _rows(what, name, t):
         _fail(what, f"{name}: the channel axis must be contiguous (strides {strides})")
     if len(shape) == 2:
         rows, ld = shape[0], strides[0]
+    elif 0 in shape[:-1]:
+        return 0, c
     else:
         rows, ld, first = 1, c, True
         for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
