@@ -161,3 +161,20 @@ def test_empty_leading_axes(shape):
     dx, dw, db = seq.linear_backward(y, x, w, z=x, activation="gelu", residual=x)
     assert dx.shape == x.shape and dw.shape == (6, 8) and not dw.any() and not db.any()
     assert seq.activation_backward(x, x, "silu").shape == x.shape
+
+
+# ------------------------------------------------------------------------------------------------------------ long sequences
+def test_causal_conv_of_millions_of_rows():
+    """More rows than one axis of a grid of row blocks takes (65535 blocks of 128 or, backward, 64): whole numbers, so every sum is exact."""
+    g = torch.Generator("cuda").manual_seed(65)
+    L, D, K = 65535 * 128 + 4099, 8, 3
+    x, dy = (torch.randint(-2, 3, (1, L, D), device="cuda", generator=g).half() for _ in range(2))
+    w = torch.tensor([[1.0], [-2.0], [3.0]], device="cuda").expand(K, D).contiguous()
+    y, st = seq.causal_conv(x, w)
+    xx = torch.cat([torch.zeros(1, K - 1, D, dtype=torch.float16, device="cuda"), x], 1)
+    assert torch.equal(y, sum(xx[:, k:k + L] * w[k, 0].half() for k in range(K))) and torch.equal(st, x[:, -(K - 1):])
+    dx, dw, db, _ = seq.causal_conv_backward(dy, x, w, torch.zeros(D, device="cuda"))
+    dd = torch.cat([dy, torch.zeros(1, K - 1, D, dtype=torch.float16, device="cuda")], 1)
+    assert torch.equal(dx, sum(dd[:, K - 1 - k:K - 1 - k + L] * w[k, 0].half() for k in range(K)))
+    assert torch.equal(dw.long(), torch.stack([(xx[0, k:k + L].long() * dy[0].long()).sum(0) for k in range(K)]))
+    assert torch.equal(db.long(), dy[0].long().sum(0))

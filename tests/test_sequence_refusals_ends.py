@@ -47,3 +47,31 @@ def test_empty_leading_axes_are_calls_without_work(shape):
               lambda: seq.linear_backward(y, x, w, z=x, activation="gelu", residual=x), lambda: seq.activation_backward(x, x, "silu")):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             f()
+
+
+# --------------------------------------------------------------------------------------------------------------- C level
+FAKE = 1 << 20            # a pointer that would fault if anything read it
+
+
+def refused(rc, text):
+    assert rc == -1
+    assert text in ffi.lib().seg_last_error().decode(), ffi.lib().seg_last_error()
+
+
+def test_causal_conv_length_limit():
+    """Long sequences do not end at one grid axis of 65535 blocks of 64 rows; the workspace is counted in 64 bits."""
+    lib = ffi.lib()
+
+    def args(B, L, x=None):
+        a = ffi.CausalConvArgs(B, L, 8, 4, 0, 0, x, 0, 8, FAKE)
+        a.y, a.y_ld = FAKE, 8
+        return a
+    refused(lib.seg_causal_conv_fwd(args(1, (1 << 30) + 1, FAKE), None), "2^30")
+    refused(lib.seg_causal_conv_fwd(args(32768, 65535 * 64 + 1, FAKE), None), "sequences of")
+    refused(lib.seg_causal_conv_fwd(args(128, 1 << 30, FAKE), None), "sequences of")
+    refused(lib.seg_causal_conv_fwd(args(127, 1 << 30), None), "NULL")
+    refused(lib.seg_causal_conv_fwd(args(32767, 65535 * 64 + 1), None), "NULL")
+    for L in (0, 1, 64, 65, 65535 * 64, 65535 * 64 + 1, 1 << 30):
+        blocks = max(1, -(-L // 64))
+        least, most = 3 * blocks * 5 * 8 * 4, 3 * (blocks + 512) * 5 * 8 * 4
+        assert least <= lib.seg_causal_conv_bwd_workspace_bytes(args(3, L)) <= (least if blocks <= 65535 else most), L

@@ -16,8 +16,6 @@ namespace {
 constexpr int RUN = 16, RUN_SMALL = 8;          // rows per thread, forward / backward and small grids
 constexpr int MAXK = 8;
 
-struct ConvDims { int B, L, D, act; };
-
 // eight channels of a row in their memory format; n <= 0: zeros
 template <typename T, bool VEC> struct Raw {
   typedef T tv __attribute__((ext_vector_type(8)));
@@ -42,12 +40,16 @@ __device__ __forceinline__ int conv_len(const seg_causal_conv_args& p, int b) {
 }
 __device__ __forceinline__ float conv_act(float v, int act) { return act == SEG_ACT_SILU ? silu_f(v) : v; }
 
-// threads: 32 channel groups of 8 x 8 runs of RUNS rows; grid (channels / 256, runs / 8, B).  A run's rows are all on their way before the
+__device__ __forceinline__ unsigned conv_row_block(int split) { return (blockIdx.z & ((1u << split) - 1)) * gridDim.y + blockIdx.y; }
+
+// threads: 32 channel groups of 8 x 8 runs of RUNS rows; grid (channels / 256, blocks of 8 runs, B).  An axis
+// ends at 65535 blocks: more of them are cut into 2^split pieces, which share the third axis with B (on one axis with the channels, by a
+// division: the prompt 54.5 us instead of 51.5).  A run's rows are all on their way before the
 // first is used: one memory latency per run
 template <typename T, bool VEC, int K, int RUNS>
-__global__ __launch_bounds__(256) void conv_fwd_kernel(const seg_causal_conv_args p) {
-  const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8, b = blockIdx.z;
-  const int64_t run = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5);
+__global__ __launch_bounds__(256) void conv_fwd_kernel(const seg_causal_conv_args p, int split) {
+  const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8, b = blockIdx.z >> split;
+  const int64_t run = (int64_t)conv_row_block(split) * 8 + (threadIdx.x >> 5);
   if (c >= p.D) return;
   const int len = conv_len(p, b), n = p.D - c;
   const int64_t t0l = run * RUNS;
@@ -92,10 +94,10 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(const seg_causal_conv_arg
 // The same run of rows backward: dv of rows t0 .. t0 + RUNS + K - 2 (each from its own window), dx[t] from the K dv behind it; dw / db
 // from the run's own rows only, summed over the block's eight runs in LDS: part[block along rows and B][K + 1][D].
 template <typename T, bool VEC, int K>
-__global__ __launch_bounds__(256) void conv_bwd_kernel(const seg_causal_conv_args p, float* part) {
+__global__ __launch_bounds__(256) void conv_bwd_kernel(const seg_causal_conv_args p, int split, float* part) {
   constexpr int RUNS = RUN_SMALL;
-  const int cg = threadIdx.x & 31, c = (blockIdx.x * 32 + cg) * 8, b = blockIdx.z;
-  const int64_t run = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5), t0l = run * RUNS;
+  const int cg = threadIdx.x & 31, c = (blockIdx.x * 32 + cg) * 8, b = blockIdx.z >> split;
+  const int64_t run = (int64_t)conv_row_block(split) * 8 + (threadIdx.x >> 5), t0l = run * RUNS;
   const int len = conv_len(p, b), n = c < p.D ? p.D - c : 0;
   float dw[K + 1][8];
 #pragma unroll
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const seg_causal_conv_arg
   }
   if (part == nullptr) return;
   __shared__ float sh[8][32][9];
-  const int64_t row = ((int64_t)b * gridDim.y + blockIdx.y) * (K + 1);
+  const int64_t row = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * (K + 1);
   const int ol = threadIdx.x >> 3, oj = threadIdx.x & 7, oc = (blockIdx.x * 32 + ol) * 8 + oj;
 #pragma unroll
   for (int k = 0; k <= K; ++k) {
@@ -233,9 +235,16 @@ inline bool conv_vec(const seg_causal_conv_args& a, bool bwd) {
   if (bwd) return ok && vec_ok(a.dy, a.dy_ld, a.dy_bs, a.dtype) && vec_ok(a.dx, a.dx_ld, a.dx_bs, a.dtype) && vec_ok(a.dstate, 0, 0, a.dtype) && vec_ok(a.dstate_out, 0, 0, a.dtype);
   return ok && vec_ok(a.y, a.y_ld, a.y_bs, a.dtype) && vec_ok(a.state_out, 0, 0, a.dtype);
 }
-inline dim3 conv_grid(const seg_causal_conv_args& a, int run) {
-  const int64_t runs = ((int64_t)a.L + run - 1) / run, yb = (runs + 7) / 8;
-  return dim3((unsigned)((a.D + 255) / 256), (unsigned)(yb < 1 ? 1 : yb), (unsigned)a.B);
+struct ConvGrid {
+  dim3 blocks;
+  int split;
+  int64_t parts() const { return (int64_t)blocks.y * blocks.z; }           // partial rows of dw / db
+};
+inline ConvGrid conv_grid(const seg_causal_conv_args& a, int run) {
+  const int64_t runs = ((int64_t)a.L + run - 1) / run, blocks = runs <= 8 ? 1 : (runs + 7) / 8;
+  int split = 0;
+  while (blocks > (int64_t)65535 << split) ++split;
+  return {dim3((unsigned)(((int64_t)a.D + 255) / 256), (unsigned)((blocks + (1 << split) - 1) >> split), (unsigned)a.B << split), split};
 }
 
 int check_conv(const seg_causal_conv_args* a, const char* name) {
@@ -245,7 +254,8 @@ int check_conv(const seg_causal_conv_args* a, const char* name) {
   SEG_CHECK_ARG(a->K >= 1 && a->K <= MAXK, "%s: K = %d (1 .. %d)", name, a->K, MAXK);
   SEG_CHECK_ARG(a->act == SEG_ACT_NONE || a->act == SEG_ACT_SILU, "%s: activation %d (none or silu)", name, a->act);
   SEG_CHECK_ARG(a->B <= 65535, "%s: %d sequences in one call (65535 at most)", name, a->B);
-  SEG_CHECK_ARG(a->L <= 65535 * 8 * RUN_SMALL, "%s: %d rows in one call (%d at most)", name, a->L, 65535 * 8 * RUN_SMALL);
+  SEG_CHECK_ARG(a->L <= (1 << 30), "%s: %d rows in one call (2^30 at most)", name, a->L);
+  SEG_CHECK_ARG((int64_t)a->B << conv_grid(*a, RUN_SMALL).split <= 65535, "%s: %d sequences of %d rows in one call (65535 for each 2^22 rows begun)", name, a->B, a->L);
   SEG_CHECK_ARG(a->w != nullptr, "%s: w is NULL", name);
   return SEG_OK;
 }
@@ -261,9 +271,9 @@ extern "C" int seg_causal_conv_fwd(const seg_causal_conv_args* a, seg_stream_t s
   conv_dispatch(*a, conv_vec(*a, false), [&](auto* tp, auto V, auto Kc) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
     // runs of 16 rows read the window's edges half as often as runs of 8; too few of them to fill the card are halved
-    const dim3 grid = conv_grid(*a, RUN);
-    if ((int64_t)grid.x * grid.y * grid.z >= 1024) hipLaunchKernelGGL((conv_fwd_kernel<T, V(), Kc(), RUN>), grid, dim3(256), 0, (hipStream_t)stream, *a);
-    else hipLaunchKernelGGL((conv_fwd_kernel<T, V(), Kc(), RUN_SMALL>), conv_grid(*a, RUN_SMALL), dim3(256), 0, (hipStream_t)stream, *a);
+    const ConvGrid g = conv_grid(*a, RUN), small = conv_grid(*a, RUN_SMALL);
+    if (g.blocks.x * g.parts() >= 1024) hipLaunchKernelGGL((conv_fwd_kernel<T, V(), Kc(), RUN>), g.blocks, dim3(256), 0, (hipStream_t)stream, *a, g.split);
+    else hipLaunchKernelGGL((conv_fwd_kernel<T, V(), Kc(), RUN_SMALL>), small.blocks, dim3(256), 0, (hipStream_t)stream, *a, small.split);
   });
   SEG_CHECK_LAUNCH("causal_conv_fwd");
   return SEG_OK;
@@ -271,7 +281,7 @@ extern "C" int seg_causal_conv_fwd(const seg_causal_conv_args* a, seg_stream_t s
 
 extern "C" int64_t seg_causal_conv_bwd_workspace_bytes(const seg_causal_conv_args* a) {
   if (a == nullptr || a->B <= 0 || a->L < 0 || a->D <= 0 || a->K < 1) return 0;
-  return (int64_t)a->B * conv_grid(*a, RUN_SMALL).y * (a->K + 1) * a->D * 4;
+  return conv_grid(*a, RUN_SMALL).parts() * (a->K + 1) * a->D * 4;
 }
 
 extern "C" int seg_causal_conv_bwd(const seg_causal_conv_args* a, seg_stream_t stream) {
@@ -283,13 +293,13 @@ extern "C" int seg_causal_conv_bwd(const seg_causal_conv_args* a, seg_stream_t s
   SEG_CHECK_ARG(a->dx == nullptr || (a->dx != a->dy && a->dx != a->x), "causal_conv_bwd: dx may not be dy or x");
   hipStream_t st = (hipStream_t)stream;
   float* part = params ? (float*)a->workspace : nullptr;
-  const dim3 grid = conv_grid(*a, RUN_SMALL);
+  const ConvGrid g = conv_grid(*a, RUN_SMALL);
   if (a->B > 0)
     conv_dispatch(*a, conv_vec(*a, true), [&](auto* tp, auto V, auto Kc) {
       typedef typename std::remove_pointer<decltype(tp)>::type T;
-      hipLaunchKernelGGL((conv_bwd_kernel<T, V(), Kc()>), grid, dim3(256), 0, st, *a, part);
+      hipLaunchKernelGGL((conv_bwd_kernel<T, V(), Kc()>), g.blocks, dim3(256), 0, st, *a, g.split, part);
     });
-  const int64_t parts = (int64_t)a->B * grid.y, ld = (int64_t)(a->K + 1) * a->D;
+  const int64_t parts = a->B > 0 ? g.parts() : 0, ld = (int64_t)(a->K + 1) * a->D;
   launch_colsum_pair(part, parts, ld, (int64_t)a->K * a->D, a->dw, a->D, a->db, st);
   SEG_CHECK_LAUNCH("causal_conv_bwd");
   return SEG_OK;
