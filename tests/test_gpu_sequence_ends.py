@@ -178,3 +178,16 @@ def test_causal_conv_of_millions_of_rows():
     assert torch.equal(dx, sum(dd[:, K - 1 - k:K - 1 - k + L] * w[k, 0].half() for k in range(K)))
     assert torch.equal(dw.long(), torch.stack([(xx[0, k:k + L].long() * dy[0].long()).sum(0) for k in range(K)]))
     assert torch.equal(db.long(), dy[0].long().sum(0))
+
+
+def test_layer_norm_backward_of_very_long_rows():
+    """More columns than one grid of column sums takes (2^32 threads in a row of blocks)."""
+    C = (1 << 27) + 5
+    g = torch.Generator("cuda").manual_seed(66)
+    x, dy = (torch.randint(-2, 3, (2, C), device="cuda", generator=g, dtype=torch.int8).half() for _ in range(2))
+    mean, rstd = torch.tensor([0.5, -0.25], device="cuda"), torch.tensor([2.0, 0.5], device="cuda")
+    _dx, dgamma, dbeta = seq.layer_norm_backward(dy, x, mean, rstd)
+    for lo in range(0, C, 1 << 25):                             # every value is a whole number of 1/8: exact
+        s = slice(lo, min(C, lo + (1 << 25)))
+        assert torch.equal(dbeta[s], dy[:, s].float().sum(0)), lo
+        assert torch.equal(dgamma[s], (dy[:, s].float() * ((x[:, s].float() - mean[:, None]) * rstd[:, None])).sum(0)), lo

@@ -190,6 +190,14 @@ __global__ __launch_bounds__(16 * R) void colsum_parts_kernel(const ColsumSet s0
   }
 }
 inline void launch_colsum_sets(const ColsumSet& s0, const ColsumSet& s1, hipStream_t st) {
+  // An axis of a grid takes fewer than 2^32 threads (a larger one comes out as its low 32 bits, without an error): more columns go by pieces.
+  constexpr int64_t MOST = (int64_t)1 << 24;
+  if (s0.cols + s1.cols > 2 * MOST) {
+    for (const ColsumSet* s : {&s0, &s1})
+      for (int64_t c = 0; c < s->cols; c += MOST)
+        launch_colsum_sets({s->part == nullptr ? nullptr : s->part + c, s->nparts, s->ld, s->cols - c < MOST ? s->cols - c : MOST, s->out + c}, {nullptr, 0, 0, 0, nullptr}, st);
+    return;
+  }
   const int64_t b0 = (s0.cols + 15) / 16, b1 = (s1.cols + 15) / 16, most = s0.nparts > s1.nparts ? s0.nparts : s1.nparts;
   if (b0 + b1 == 0) return;
   // many parts: four times the threads on the same columns (1024 parts of 128 columns: 20 us with 16 rows of threads)
