@@ -191,3 +191,16 @@ def test_layer_norm_backward_of_very_long_rows():
         s = slice(lo, min(C, lo + (1 << 25)))
         assert torch.equal(dbeta[s], dy[:, s].float().sum(0)), lo
         assert torch.equal(dgamma[s], (dy[:, s].float() * ((x[:, s].float() - mean[:, None]) * rstd[:, None])).sum(0)), lo
+
+
+@pytest.mark.parametrize("M", [1, 16])
+def test_linear_with_very_many_units(M):
+    """More units than a grid of the few-rows kernel takes (2^32 threads in a row of blocks of 512, 16 units each): whole numbers, exact."""
+    N, K = (1 << 27) + 48, 4
+    g = torch.Generator("cuda").manual_seed(68)
+    x = torch.randint(-2, 3, (M, K), device="cuda", generator=g).float()
+    w = torch.randint(-2, 3, (N, K), device="cuda", generator=g, dtype=torch.int8).float()
+    y = seq.linear(x, w, activation="relu")
+    for lo in range(0, N, 1 << 25):
+        s = slice(lo, min(N, lo + (1 << 25)))
+        assert torch.equal(y[:, s], torch.relu(x @ w[s].t())), lo

@@ -720,13 +720,14 @@ inline DmaPlan dma_plan(const seg_linear_args& a, int pass) {
 // lose: a block walks all of k (16 rows f16: 1.7 us per 1024 of it, four times that for 64 rows) and reads all of x again.  Against the
 // kernels with split sums (f16): 16 x 4096 x 4096 10 us and 14, 32 x 1024 x 4096 13 and 14, 64 x 4096 x 1024 10 and 13.4; beyond the two
 // limits 64 x 64 x 65536 276 and 14, 32 x 256 x 16384 44 and 14, 64 x 16384 x 4096 74 and 31, 32 x 8192 x 8192 45 and 27.  fp32 has
-// no faster way for many units: 1 x 16384 x 4096 57 and 89, 16 x 4096 x 16384 69 and 96.
+// no faster way for many units: 1 x 16384 x 4096 57 and 89, 16 x 4096 x 16384 69 and 96 (up to 2^26: blocks of 512 threads own 16 units,
+// and an axis of a grid takes fewer than 2^32 threads).
 inline bool rows_ok(const seg_linear_args& a, int pass) {
   if (pass != SEG_LINEAR_FWD || a.M > 64) return false;
   const int64_t u = a.dtype == SEG_DT_F32 ? 4 : 8;
   if (!(aligned16(a.x) && aligned16(a.w) && a.x_ld % u == 0 && a.w_ld % u == 0 && a.K % u == 0)) return false;
   const int64_t groups = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-  if (a.dtype == SEG_DT_F32 && groups == 1 && a.N >= 2048) return true;
+  if (a.dtype == SEG_DT_F32 && groups == 1 && a.N >= 2048 && a.N <= 1 << 26) return true;
   return groups * a.K * (int64_t)dt_size(a.dtype) <= 16384 && groups * a.K * a.N <= (int64_t)1 << 25;
 }
 inline GemmPlan plan_of(const seg_linear_args& a, int pass) {
