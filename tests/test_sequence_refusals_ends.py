@@ -75,3 +75,20 @@ def test_causal_conv_length_limit():
         blocks = max(1, -(-L // 64))
         least, most = 3 * blocks * 5 * 8 * 4, 3 * (blocks + 512) * 5 * 8 * 4
         assert least <= lib.seg_causal_conv_bwd_workspace_bytes(args(3, L)) <= (least if blocks <= 65535 else most), L
+
+
+def test_grids_that_would_wrap_are_refused():
+    """An axis of a grid takes fewer than 2^32 threads and wraps without an error: refused in front of the launch."""
+    lib = ffi.lib()
+    a = ffi.CausalConvArgs(65535, 1, 1 << 20, 1, 0, 0, FAKE, 1 << 20, 1 << 20, FAKE)
+    a.y, a.y_bs, a.y_ld = FAKE, 1 << 20, 1 << 20
+    refused(lib.seg_causal_conv_step(a, None), "too many")
+    for B, D, S, f in ((65535, 1 << 13, 64, lib.seg_selective_scan_step), (4, 1 << 28, 16, lib.seg_selective_scan_step), (1, 1 << 28, 64, lib.seg_selective_scan_fwd),
+                       (1, 1 << 30, 16, lib.seg_selective_scan_fwd), (1, 1 << 28, 33, lib.seg_selective_scan_bwd)):
+        a = ffi.ScanArgs(B, 1, D, S, 0, 1)
+        for n, c in (("u", D), ("dt", D), ("Bm", S), ("Cm", S), ("y", D), ("dy", D)):
+            setattr(a, n, FAKE)
+            setattr(a, n + "_bs", c)
+            setattr(a, n + "_ld", c)
+        a.A = a.state = a.saved = a.workspace = FAKE
+        refused(f(a, None), "too many")

@@ -190,7 +190,7 @@ __global__ __launch_bounds__(16 * R) void colsum_parts_kernel(const ColsumSet s0
   }
 }
 inline void launch_colsum_sets(const ColsumSet& s0, const ColsumSet& s1, hipStream_t st) {
-  // An axis of a grid takes fewer than 2^32 threads (a larger one comes out as its low 32 bits, without an error): more columns go by pieces.
+  // (2^21 blocks of 1024 threads: more columns go by pieces, see grid_takes below)
   constexpr int64_t MOST = (int64_t)1 << 24;
   if (s0.cols + s1.cols > 2 * MOST) {
     for (const ColsumSet* s : {&s0, &s1})
@@ -211,6 +211,8 @@ inline void launch_colsum_pair(const float* part, int64_t nparts, int64_t ld, in
   launch_colsum_sets(a, b, st);
 }
 
+// an axis of a grid takes fewer than 2^32 threads: a larger one comes out as its low 32 bits, without an error
+inline bool grid_takes(int64_t threads) { return threads < (int64_t)1 << 32; }
 inline size_t dt_size(int dt) { return dt == SEG_DT_F32 ? 4 : 2; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // whether 8-element vector accesses fit a tensor's rows (NULL: not there, fits)

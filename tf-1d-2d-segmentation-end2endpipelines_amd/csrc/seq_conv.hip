@@ -310,7 +310,8 @@ extern "C" int seg_causal_conv_step(const seg_causal_conv_args* a, seg_stream_t 
   if (a->B == 0) return SEG_OK;
   SEG_CHECK_ARG(a->x != nullptr && a->y != nullptr, "causal_conv_step: x / y is NULL");
   SEG_CHECK_ARG(a->B == 1 || (a->x_bs >= a->D && a->y_bs >= a->D), "causal_conv_step: row strides below the %d channels", a->D);
-  const int64_t n = (int64_t)a->B * ((a->D + 7) / 8);
+  const int64_t n = (int64_t)a->B * (((int64_t)a->D + 7) / 8);
+  SEG_CHECK_ARG(grid_takes(n + 255), "causal_conv_step: %d sequences of %d channels are too many for one call (2^35 elements)", a->B, a->D);
   conv_dispatch(*a, conv_vec(*a, false), [&](auto* tp, auto V, auto Kc) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
     hipLaunchKernelGGL((conv_step_kernel<T, V(), Kc()>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, *a);

@@ -771,6 +771,8 @@ int check_scan(const seg_scan_args* a, const char* name) {
   SEG_CHECK_ARG(a->S >= 1 && a->S <= MAXS, "%s: %d states (1 .. %d)", name, a->S, MAXS);
   SEG_CHECK_ARG(a->B <= 65535, "%s: %d sequences in one call (65535 at most)", name, a->B);
   SEG_CHECK_ARG(a->L <= (1 << 30), "%s: %d rows in one call (2^30 at most)", name, a->L);
+  const int64_t G = scan_group(a->S), cb = scan_cb(a->S);
+  SEG_CHECK_ARG(grid_takes((a->D + cb - 1) / cb * cb * G), "%s: %d channels of %d states are too many for one call (2^32 pieces of four states)", name, a->D, a->S);
   SEG_CHECK_ARG(a->A != nullptr, "%s: A is NULL", name);
   SEG_CHECK_ARG(((uintptr_t)a->A & 15) == 0 && ((uintptr_t)a->state & 15) == 0 && ((uintptr_t)a->state_out & 15) == 0 && ((uintptr_t)a->saved & 15) == 0 &&
                 ((uintptr_t)a->dstate_out & 15) == 0 && ((uintptr_t)a->dstate & 15) == 0, "%s: A / state / saved need 16-byte alignment", name);
@@ -888,6 +890,8 @@ extern "C" int seg_selective_scan_step(const seg_scan_args* a, seg_stream_t stre
   SEG_CHECK_ARG(a->u != nullptr && a->dt != nullptr && a->Bm != nullptr && a->Cm != nullptr && a->y != nullptr, "selective_scan_step: u / dt / Bm / Cm / y is NULL");
   SEG_CHECK_ARG(a->B == 1 || (a->u_bs >= a->D && a->dt_bs >= a->D && (a->z == nullptr || a->z_bs >= a->D) && a->Bm_bs >= a->S && a->Cm_bs >= a->S && a->y_bs >= a->D),
                 "selective_scan_step: row strides below the channels / states");
+  SEG_CHECK_ARG(grid_takes((int64_t)a->B * a->D * scan_group(a->S) + 255), "selective_scan_step: %d sequences of %d channels of %d states are too many for one call (2^32 pieces of four states)",
+                a->B, a->D, a->S);
   scan_dispatch(*a, [&](auto* tp, auto Gc) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
     constexpr int G = Gc();
