@@ -92,3 +92,22 @@ def test_grids_that_would_wrap_are_refused():
             setattr(a, n + "_ld", c)
         a.A = a.state = a.saved = a.workspace = FAKE
         refused(f(a, None), "too many")
+
+
+# ------------------------------------------------------------------------------------------------------------- derivatives
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor's tangent would be lost without a word; outside a dual level, and for operands without one, nothing changes."""
+    from torch.autograd import forward_ad as fwd
+    x, w = torch.ones(4, 8), torch.ones(6, 8)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for f in (lambda: seq.layer_norm(d), lambda: seq.linear(d, w), lambda: seq.linear(x, fwd.make_dual(w, torch.ones_like(w))),
+                  lambda: seq.activation_backward(d, x, "silu"), lambda: seq.causal_conv(d[None], T(4, 8)), lambda: seq.causal_conv_step(d, T(4, 3, 8), T(4, 8)),
+                  lambda: seq.selective_scan(d[None], T(1, 4, 8), T(8, 4), T(1, 4, 4), T(1, 4, 4)),
+                  lambda: seq.selective_scan_step(d, T(4, 8), T(8, 4), T(4, 4), T(4, 4), T(4, 8, 4))):
+            with pytest.raises(ValueError, match="tangent"):
+                f()
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            seq.linear(x, w)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        seq.linear(x, w)

@@ -5,7 +5,7 @@ Every function enqueues kernels of libseg_hip.so on the current stream of its te
 it allocates (outputs, workspaces) comes from torch's allocator on that stream, so calls can be captured into a graph.  Rows are
 channels-last ([..., C], [B, L, D]) in fp16, bf16 or fp32; they may be slices of wider tensors as long as the channel axis is
 contiguous.  Parameters, statistics, scan states and gradients of parameters are fp32.  Gradients are explicit functions, as everywhere
-in this package: nothing is recorded by torch.autograd, and a call on tensors that ask for it raises.
+in this package: nothing is recorded by torch.autograd, and a call on tensors that ask for it - or carry a forward-mode tangent - raises.
 
 Weights are stored the way the matrix cores read them: `linear` takes [units, inputs] (a Keras Dense kernel transposed), `causal_conv`
 [K, D] (a Keras depthwise kernel without its last axis), tap K - 1 on the current row.
@@ -17,6 +17,7 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ffi
 from ._ffi import SEQ_ACT, CausalConvArgs, LinearArgs, ScanArgs
@@ -128,6 +129,10 @@ def _no_grad(what, *ts):
         for t in ts:
             if t is not None and t.requires_grad:
                 _fail(what, "a tensor requires grad, but nothing here is recorded by torch.autograd: detach it and call the *_backward function")
+    if getattr(forward_ad, "_current_level", 0) >= 0:           # (inside a dual level; torch without that name: always looked at)
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail(what, "a tensor carries a forward-mode tangent, which would be lost")
 
 
 def _ptr(t):
