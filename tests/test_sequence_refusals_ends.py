@@ -111,3 +111,25 @@ def test_forward_mode_tangents_are_refused():
             seq.linear(x, w)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         seq.linear(x, w)
+
+
+def test_a_new_state_that_requires_grad_is_refused():
+    """It is written, so it gets the check that state gets; torch.no_grad() lifts both."""
+    for f in (lambda n: seq.causal_conv_step(T(2, 8), T(2, 3, 8), T(4, 8), new_state=n(2, 3, 8)),
+              lambda n: seq.selective_scan_step(T(2, 8), T(2, 8), T(8, 4), T(2, 4), T(2, 4), T(2, 8, 4), new_state=n(2, 8, 4))):
+        with pytest.raises(ValueError, match="requires grad"):
+            f(lambda *s: T(*s, requires_grad=True))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            f(lambda *s: T(*s, requires_grad=True))
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            f(T)
+
+
+def test_saved_states_that_require_grad_are_refused():
+    t = T(2, 5, 8)
+    args = (t, t, t, T(8, 4), T(2, 5, 4), T(2, 5, 4))
+    n = 2 * 1 * 8 * 4
+    with pytest.raises(ValueError, match="requires grad"):
+        seq.selective_scan_backward(*args, T(n, requires_grad=True))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        seq.selective_scan_backward(*args, T(n))

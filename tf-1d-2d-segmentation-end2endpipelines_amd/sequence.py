@@ -412,7 +412,7 @@ def causal_conv_step(x, state, w, bias=None, activation: Optional[str] = None, n
     new = _new_state(what, state, new_state)
     if B > 1 and x.stride(0) < d:
         _fail(what, f"x: rows overlap (strides {x.stride()}); call .contiguous()")
-    _no_grad(what, x, w, bias, state)
+    _no_grad(what, x, w, bias, state, new_state)
     di = _gpu(what, x)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     a = CausalConvArgs(B, 1, d, K, dt, act, _ptr(x), x.stride(0), d, _ptr(w), _ptr(bias), _ptr(state), None, _ptr(y), d, d, _ptr(new))
@@ -526,7 +526,7 @@ def selective_scan_backward(dy, u, dt, A, B, C, saved, D=None, z=None, dt_bias=N
     lib = _ffi.lib()
     a = _scan_args(nb, L, d, S, dtc, softplus, u, dt, z, B, C, A, D, dt_bias, None, lengths, st)
     _param(what, "saved", saved, u, (lib.seg_selective_scan_saved_bytes(a) // 4,))
-    _no_grad(what, dy, u, dt, A, B, C, D, z, dt_bias, dstate)
+    _no_grad(what, dy, u, dt, A, B, C, D, z, dt_bias, dstate, saved)
     di = _gpu(what, u)
     dev = u.device
 
@@ -563,7 +563,7 @@ def selective_scan_step(u, dt, A, B, C, state, D=None, z=None, dt_bias=None, sof
     new = _new_state(what, state, new_state)
     if state.data_ptr() % 16 or new.data_ptr() % 16:
         _fail(what, "state must be 16-byte aligned")
-    _no_grad(what, u, dt, A, B, C, D, z, dt_bias, state)
+    _no_grad(what, u, dt, A, B, C, D, z, dt_bias, state, new_state)
     di = _gpu(what, u)
     y = torch.empty_like(u, memory_format=torch.contiguous_format)
     a = ScanArgs(nb, 1, d, S, dtc, 1 if softplus else 0, u.data_ptr(), st[0][0], 0, dt.data_ptr(), st[1][0], 0, _ptr(z), st[2][0], 0, B.data_ptr(), st[3][0], 0,
