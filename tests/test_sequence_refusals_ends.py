@@ -133,3 +133,16 @@ def test_saved_states_that_require_grad_are_refused():
         seq.selective_scan_backward(*args, T(n, requires_grad=True))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         seq.selective_scan_backward(*args, T(n))
+
+
+def test_many_rows_and_large_tensors_are_no_large_extents():
+    """Rows of layer_norm and linear count in 64 bits; a tensor of more than 2^31 elements has no large extent by that alone."""
+    def m(*shape):
+        return T(*shape, device="meta")
+    for f in (lambda: seq.layer_norm(m(BIG, 8)), lambda: seq.linear(m(BIG, 8), m(4, 8)), lambda: seq.linear(m(2, 1 << 17), m(1 << 17, 1 << 17)),
+              lambda: seq.causal_conv(m(1 << 10, 1 << 11, 1 << 12), m(4, 1 << 12)),
+              lambda: seq.selective_scan(m(1 << 10, 1 << 11, 1 << 12), m(1 << 10, 1 << 11, 1 << 12), m(1 << 12, 4), m(1 << 10, 1 << 11, 4), m(1 << 10, 1 << 11, 4))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            f()
+    with pytest.raises(ValueError, match="2147483647"):
+        seq.causal_conv(m(BIG, 0, 8), m(1, 8))

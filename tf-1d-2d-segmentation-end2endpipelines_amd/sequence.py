@@ -84,18 +84,18 @@ def _param(what, name, t, ref, shape, dtype=torch.float32):
     _fail(what, f"{name} must be contiguous (strides {t.stride()})")
 
 
-def _extents(what, *ns):
-    """ctypes would hand on the low 32 bits of a larger one."""
-    if max(ns) > MAX_EXTENT:
-        _fail(what, f"an extent of {max(ns)} (at most {MAX_EXTENT} channels, units, rows of a sequence or sequences)")
+def _extents(what, t):
+    """ctypes would hand on the low 32 bits of a larger extent.  (No extent of a tensor of few elements is large, unless it has none.)"""
+    if not 0 < t.numel() <= MAX_EXTENT and max(t.shape) > MAX_EXTENT:
+        _fail(what, f"an extent of {max(t.shape)} (at most {MAX_EXTENT} channels, units, rows of a sequence or sequences)")
 
 
 def _rows(what, name, t):
     """(rows, row stride) of [..., C] whose leading axes collapse into one."""
     shape, strides = t.shape, t.stride()
     c = shape[-1]
-    if c > MAX_EXTENT:
-        _extents(what, c)
+    if c > MAX_EXTENT:                                           # (rows: int64)
+        _extents(what, t)
     if c > 1 and strides[-1] != 1:
         _fail(what, f"{name}: the channel axis must be contiguous (strides {strides})")
     if len(shape) == 2:
@@ -228,7 +228,7 @@ def _linear_args(what, x, w, activation, alpha):
         _fail(what, "x must be [..., inputs] and w [units, inputs]")
     if min(w.shape) < 1:
         _fail(what, f"w has shape {tuple(w.shape)}")
-    _extents(what, w.shape[0])
+    _extents(what, w)
     if w.dtype != x.dtype or w.device != x.device:
         _fail(what, f"w is {w.dtype} on {w.device}, expected {x.dtype} on {x.device}")
     _n, w_ld = _rows(what, "w", w)
@@ -335,7 +335,7 @@ def _conv_common(what, x, w, bias, activation, state, rank):
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         _fail(what, "w must be [K, D]")
     K, d, B = w.shape[0], x.shape[-1], x.shape[0]
-    _extents(what, *x.shape)
+    _extents(what, x)
     if not 1 <= K <= MAX_TAPS:
         _fail(what, f"{K} taps (1 .. {MAX_TAPS})")
     if activation not in (None, "none", "linear", "silu"):
@@ -443,7 +443,7 @@ def _scan_common(what, u, dt, A, B, C_, D, z, dt_bias, rank):
     if not isinstance(A, torch.Tensor) or A.dim() != 2:
         _fail(what, "A must be [D, S]")
     d, S, nb = shape[-1], A.shape[1], shape[0]
-    _extents(what, *shape)
+    _extents(what, u)
     if not 1 <= S <= MAX_STATES:
         _fail(what, f"{S} states per channel (1 .. {MAX_STATES})")
     _param(what, "A", A, u, (d, S))
