@@ -153,7 +153,7 @@ __device__ __forceinline__ float delta_of(const seg_scan_args& p, float dt, floa
 template <typename T, bool VEC, int G, bool MAIN>
 __global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_args p, int clen, int nch, float* start, float* sumd) {
   typedef Lay<G> Y;
-  __shared__ float2 sdu[TT][Y::CB];
+  __shared__ __align__(16) float2 sdu[TT][Y::CB];              // (written two channels, 16 bytes, at a time)
   __shared__ __align__(16) float sB[TT * Y::SP], sC[MAIN ? TT * Y::SP : 1];
   __shared__ __align__(16) float sy[MAIN ? TT : 1][Y::CB];
   const int tid = threadIdx.x, g = tid % G, c = tid / G, b = blockIdx.z, chunk = blockIdx.y;
@@ -340,7 +340,7 @@ __device__ __forceinline__ float dp_of(const seg_scan_args& p, const Raw<T, VEC>
 template <typename T, bool VEC, int G>
 __global__ __launch_bounds__(Lay<G>::NT) void scan_bwd_local_kernel(const seg_scan_args p, int clen, int nch, float* adj, float* sumd) {
   typedef Lay<G> Y;
-  __shared__ float2 sdp[TT][Y::CB];
+  __shared__ __align__(16) float2 sdp[TT][Y::CB];              // (written two channels, 16 bytes, at a time)
   __shared__ __align__(16) float sC[TT * Y::SP];
   const int tid = threadIdx.x, g = tid % G, c = tid / G, b = blockIdx.z, chunk = blockIdx.y + 1;
   const int c0 = blockIdx.x * Y::CB, d = c0 + c, len = scan_len(p, b);
