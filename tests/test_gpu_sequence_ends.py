@@ -204,3 +204,34 @@ def test_linear_with_very_many_units(M):
     for lo in range(0, N, 1 << 25):
         s = slice(lo, min(N, lo + (1 << 25)))
         assert torch.equal(y[:, s], torch.relu(x @ w[s].t())), lo
+
+
+# ------------------------------------------------------------------------------------- gradients of weights: every row counts
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", [(131080, 520, 264), (131075, 520, 264), (20011, 136, 264), (100003, 64, 72), (8201, 519, 523), (5003, 24, 40), (65, 300, 1000)])
+def test_weight_gradients_of_whole_numbers(M, N, K, dtype):
+    """Products and sums of whole numbers up to 4 M < 2^24 are exact in 32 bits: a lost, doubled or misplaced row, range of rows or partial
+    sum shows.  Every tile kernel, split ranges that end inside a step, operands that are copied, and the kernel for every size."""
+    g = torch.Generator("cuda").manual_seed(M + N)
+    x, dy = (torch.randint(-2, 3, (M, c), device="cuda", generator=g).to(dtype) for c in (K, N))
+    w = torch.zeros(N, K, dtype=dtype, device="cuda")
+    _none, dw, db = seq.linear_backward(dy, x, w, need_dx=False)
+    want, sums = dy.double().t().contiguous() @ x.double(), dy.double().sum(0)
+    assert torch.equal(dw.double(), want) and torch.equal(db.double(), sums)
+    assert torch.equal(seq.linear_backward(dy, x, w, need_dx=False, need_db=False)[1], dw)
+    assert torch.equal(seq.linear_backward(dy, x, w, need_dx=False, need_dw=False)[2], db)
+
+
+@pytest.mark.parametrize("n", [64, 20])
+def test_weight_gradients_of_rows_past_32_bits(n):
+    """Only the last rows of an operand of more than 2^31 elements count (the others' gradient is zero): the same bits as those rows alone."""
+    D = 1032
+    rows = (1 << 31) // D + 77
+    g = torch.Generator("cuda").manual_seed(67)
+    x = torch.randint(-2, 3, (rows, D), device="cuda", generator=g, dtype=torch.int8).half()
+    dy = torch.zeros(rows, n, dtype=torch.float16, device="cuda")
+    dy[-70:] = torch.randint(-2, 3, (70, n), device="cuda", generator=g).half()
+    w = torch.zeros(n, D, dtype=torch.float16, device="cuda")
+    _none, dw, db = seq.linear_backward(dy, x, w, need_dx=False)
+    want = dy[-70:].double().t().contiguous() @ x[-70:].double()
+    assert torch.equal(dw.double(), want) and torch.equal(db.double(), dy[-70:].double().sum(0))
