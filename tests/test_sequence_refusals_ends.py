@@ -146,3 +146,21 @@ def test_many_rows_and_large_tensors_are_no_large_extents():
             f()
     with pytest.raises(ValueError, match="2147483647"):
         seq.causal_conv(m(BIG, 0, 8), m(1, 8))
+
+
+def test_channel_limit():
+    """Channel indices of a last block reach 256 behind the last channel: they hold in 32 bits up to 2^30 channels."""
+    lib = ffi.lib()
+    D = (1 << 30) + 1
+    a = ffi.CausalConvArgs(1, 1, D, 2, 0, 0, FAKE, D, D, FAKE)
+    a.y, a.y_bs, a.y_ld, a.dy, a.dy_bs, a.dy_ld, a.workspace = FAKE, D, D, FAKE, D, D, FAKE
+    for f in (lib.seg_causal_conv_fwd, lib.seg_causal_conv_bwd, lib.seg_causal_conv_step):
+        refused(f(a, None), "D 1073741825")
+    a = ffi.ScanArgs(1, 1, D, 1, 0, 1)
+    for n, c in (("u", D), ("dt", D), ("Bm", 1), ("Cm", 1), ("y", D), ("dy", D)):
+        setattr(a, n, FAKE)
+        setattr(a, n + "_bs", c)
+        setattr(a, n + "_ld", c)
+    a.A = a.state = a.saved = a.workspace = FAKE
+    for f in (lib.seg_selective_scan_fwd, lib.seg_selective_scan_bwd, lib.seg_selective_scan_step):
+        refused(f(a, None), "D 1073741825")

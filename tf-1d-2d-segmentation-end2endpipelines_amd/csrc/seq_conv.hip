@@ -250,7 +250,7 @@ inline ConvGrid conv_grid(const seg_causal_conv_args& a, int run) {
 int check_conv(const seg_causal_conv_args* a, const char* name) {
   SEG_CHECK_ARG(a != nullptr, "%s: args is NULL", name);
   SEG_CHECK_ARG(a->dtype >= SEG_DT_F16 && a->dtype <= SEG_DT_F32, "%s: dtype %d", name, a->dtype);
-  SEG_CHECK_ARG(a->B >= 0 && a->L >= 0 && a->D > 0, "%s: B %d, L %d, D %d", name, a->B, a->L, a->D);
+  SEG_CHECK_ARG(a->B >= 0 && a->L >= 0 && a->D > 0 && a->D <= (1 << 30), "%s: B %d, L %d, D %d (2^30 at most)", name, a->B, a->L, a->D);
   SEG_CHECK_ARG(a->K >= 1 && a->K <= MAXK, "%s: K = %d (1 .. %d)", name, a->K, MAXK);
   SEG_CHECK_ARG(a->act == SEG_ACT_NONE || a->act == SEG_ACT_SILU, "%s: activation %d (none or silu)", name, a->act);
   SEG_CHECK_ARG(a->B <= 65535, "%s: %d sequences in one call (65535 at most)", name, a->B);

@@ -767,7 +767,7 @@ inline bool scan_vec(const seg_scan_args& a, bool bwd) {
 int check_scan(const seg_scan_args* a, const char* name) {
   SEG_CHECK_ARG(a != nullptr, "%s: args is NULL", name);
   SEG_CHECK_ARG(a->dtype >= SEG_DT_F16 && a->dtype <= SEG_DT_F32, "%s: dtype %d", name, a->dtype);
-  SEG_CHECK_ARG(a->B >= 0 && a->L >= 0 && a->D > 0, "%s: B %d, L %d, D %d", name, a->B, a->L, a->D);
+  SEG_CHECK_ARG(a->B >= 0 && a->L >= 0 && a->D > 0 && a->D <= (1 << 30), "%s: B %d, L %d, D %d (2^30 at most)", name, a->B, a->L, a->D);
   SEG_CHECK_ARG(a->S >= 1 && a->S <= MAXS, "%s: %d states (1 .. %d)", name, a->S, MAXS);
   SEG_CHECK_ARG(a->B <= 65535, "%s: %d sequences in one call (65535 at most)", name, a->B);
   SEG_CHECK_ARG(a->L <= (1 << 30), "%s: %d rows in one call (2^30 at most)", name, a->L);

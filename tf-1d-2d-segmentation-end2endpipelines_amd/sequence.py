@@ -351,7 +351,7 @@ def _conv_common(what, x, w, bias, activation, state, rank):
 def causal_conv(x, w, bias=None, activation: Optional[str] = None, state=None, lengths=None):
     """Per channel: v[t] = bias + sum_k w[k] xx[t + k] over xx = [state; x], y = act(v).  x [B, L, D], w fp32 [K, D] (K <= 8), bias fp32
     [D], activation None or "silu", state [B, K - 1, D] (None: zeros), lengths int32 [B]: rows behind a length are not read, their y is 0.
-    At most 65535 sequences (fewer by a power of two from 2^22 rows each on) of 2^30 rows in one call.
+    At most 65535 sequences (fewer by a power of two from 2^22 rows each on) of 2^30 rows and 2^30 channels in one call.
     Returns (y, the state that goes on: the last K - 1 rows in front of each length)."""
     what = "causal_conv"
     dt, act, B, d, K = _conv_common(what, x, w, bias, activation, state, 3)
@@ -485,7 +485,7 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus: bool 
 
     u, dt, z [B, L, D], B, C [B, L, S] of one type; A fp32 [D, S] (negative rates), D, dt_bias fp32 [D]; state fp32 [B, D, S] in front of
     the first row (None: zeros); lengths int32 [B]: rows behind a length are not read, their y is 0 and the state stays what it was.
-    At most 65535 sequences of 2^30 rows in one call.
+    At most 65535 sequences of 2^30 rows and 2^30 channels in one call.
     Returns (y, last state), with training=True (y, last state, saved) - `saved` is what selective_scan_backward needs."""
     what = "selective_scan"
     dtc, nb, d, S, st = _scan_common(what, u, dt, A, B, C, D, z, dt_bias, 3)
