@@ -235,3 +235,14 @@ def test_weight_gradients_of_rows_past_32_bits(n):
     _none, dw, db = seq.linear_backward(dy, x, w, need_dx=False)
     want = dy[-70:].double().t().contiguous() @ x[-70:].double()
     assert torch.equal(dw.double(), want) and torch.equal(db.double(), dy[-70:].double().sum(0))
+
+
+def test_activation_backward_of_the_longest_row():
+    """2^31 - 3 channels: their pieces of eight are counted in 64 bits."""
+    C = (1 << 31) - 3
+    g = torch.Generator("cuda").manual_seed(69)
+    z = torch.randint(-2, 3, (1, C), device="cuda", generator=g, dtype=torch.int8).half()
+    dx = seq.activation_backward(z, z, "relu")
+    for lo in range(0, C, 1 << 29):
+        s = slice(lo, min(C, lo + (1 << 29)))
+        assert torch.equal(dx[:, s], torch.relu(z[:, s])), lo

@@ -905,7 +905,7 @@ namespace {
 template <typename T, bool VEC>
 __global__ __launch_bounds__(TPB) void act_bwd_kernel(const T* dy, int64_t dy_ld, const T* z, int64_t z_ld, T* dx, int64_t dx_ld, int64_t rows, int C,
                                                       int act, float alpha) {
-  const int chunks = (C + 7) / 8;
+  const int chunks = (int)(((int64_t)C + 7) / 8);
   const int64_t n = rows * chunks;
   for (int64_t e = (int64_t)blockIdx.x * TPB + threadIdx.x; e < n; e += (int64_t)gridDim.x * TPB) {
     const int64_t r = e / chunks;
@@ -932,7 +932,7 @@ extern "C" int seg_linear_act_bwd(const void* dy, int64_t dy_ld, const void* z, 
   SEG_CHECK_ARG(rows == 1 || dx != dy || dx_ld == dy_ld, "linear_act_bwd: dx in place of dy has another row stride");
   seq_dispatch_dtype(dtype, [&](auto* tp) {
     typedef typename std::remove_pointer<decltype(tp)>::type T;
-    const int64_t blocks = (rows * ((C + 7) / 8) + TPB - 1) / TPB;
+    const int64_t blocks = (rows * (((int64_t)C + 7) / 8) + TPB - 1) / TPB;
     const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
     if (C % 8 == 0 && vec_ok(dy, dy_ld, 0, dtype) && vec_ok(z, z_ld, 0, dtype) && vec_ok(dx, dx_ld, 0, dtype))
       hipLaunchKernelGGL((act_bwd_kernel<T, true>), grid, dim3(TPB), 0, (hipStream_t)stream, (const T*)dy, dy_ld, (const T*)z, z_ld, (T*)dx, dx_ld, rows, C, act, alpha);
