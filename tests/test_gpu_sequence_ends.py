@@ -246,3 +246,32 @@ def test_activation_backward_of_the_longest_row():
     for lo in range(0, C, 1 << 29):
         s = slice(lo, min(C, lo + (1 << 29)))
         assert torch.equal(dx[:, s], torch.relu(z[:, s])), lo
+
+
+# ------------------------------------------------------------------------------------------------------------ growing states
+@pytest.mark.parametrize("S", [4, 16])
+def test_selective_scan_of_growing_states(S):
+    """Steps of the wrong sign make states grow by e^1.5 a row (softplus=False, dt = -1): what is still zero stays zero however far a whole
+    chunk's factor lies past 32 bits, and so do gradients that have not begun.  Inputs in the last 20 rows, dy in the first 20."""
+    g = gen(70)
+    B, L, D = 2, 600, 24
+    u, dt, dy = torch.zeros(B, L, D), -torch.ones(B, L, D), torch.zeros(B, L, D)
+    u[:, -20:], dy[:, :20] = torch.randn(B, 20, D, generator=g), torch.randn(B, 20, D, generator=g)
+    A = -1.5 * torch.ones(D, S)
+    Bm, Cm = torch.randn(B, L, S, generator=g), torch.randn(B, L, S, generator=g)
+    ref = [t.double().requires_grad_() for t in (u, dt, A, Bm, Cm)]
+    args = [t.cuda() for t in (u, dt, A, Bm, Cm)]
+    y, last, saved = seq.selective_scan(*args, softplus=False, training=True)
+    d = seq.selective_scan_backward(dy.cuda(), *args, saved, softplus=False)
+    h, ys = torch.zeros(B, D, S, dtype=torch.float64), []
+    with torch.enable_grad():
+        for t in range(L):
+            h = torch.exp(ref[1][:, t, :, None] * ref[2]) * h + (ref[1][:, t] * ref[0][:, t])[..., None] * ref[3][:, t, None]
+            ys.append((h * ref[4][:, t, None]).sum(-1))
+        want = torch.autograd.grad(torch.stack(ys, 1), ref, dy.double())
+    # one sign of every factor e^1.5 and random signs of the terms: relative to the largest value, 20 rows x 8 roundings
+    for name, got, exact in (("y", y, torch.stack(ys, 1)), ("state", last, h)) + tuple(zip(("du", "ddt", "dA", "dB", "dC"), (d.du, d.ddt, d.dA, d.dB, d.dC), want)):
+        got, exact = got.double().cpu(), exact.detach()
+        assert torch.isfinite(got).all(), name
+        assert float((got - exact).abs().max()) <= 160 * 2.0 ** -24 * float(exact.abs().max()), name
+    assert torch.isfinite(d.dstate).all()

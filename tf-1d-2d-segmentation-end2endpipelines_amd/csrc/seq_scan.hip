@@ -40,8 +40,9 @@ template <int G> struct Lay {
 };
 
 __device__ __forceinline__ float exp2_f(float v) { return __builtin_amdgcn_exp2f(v); }
-// max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1], with a small RELATIVE error for every v: log(1 + e) = e P(e), P of degree 8 fitted to
-// 3e-8 on [0, 1] - half the instructions of a logarithm whose argument's lost bits are corrected
+// max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1]: log(1 + e) = e P(e), P of degree 8 fitted to 3e-8 on [0, 1] - half the instructions of a
+// logarithm whose argument's lost bits are corrected.  Relative error, measured in half steps of 2^-24: 3 around zero, about |v| in the left
+// tail (the exponential's argument is rounded: 15 at -16, 61 at -80), 1 to the right
 __device__ __forceinline__ float softplus_f(float v) {
   const float e = __expf(-fabsf(v));
   float P = 0.0052326812f;
@@ -276,6 +277,8 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_fwd_kernel(const seg_scan_arg
   }
 }
 
+// A chunk's whole factor lies past 32 bits where states grow (softplus off and steps of the wrong sign): what is still zero stays zero there
+__device__ __forceinline__ float carried(float factor, float h, float own) { return h != 0.f ? fmaf(factor, h, own) : own; }
 // the chunks in order: in place, a chunk's own last state becomes the state in front of it
 constexpr int JOIN = 8;          // chunks whose parts are on their way together (1 x 100000 x 64 x 16, 1563 chunks: 535 us one at a time, 200)
 __global__ __launch_bounds__(256) void scan_join_kernel(const seg_scan_args p, int nch, float* start, const float* sumd) {
@@ -298,7 +301,7 @@ __global__ __launch_bounds__(256) void scan_join_kernel(const seg_scan_args p, i
     for (int k = 0; k < JOIN; ++k)
       if (k0 + k < nch - 1) {
         start[(o0 + k0 + k) * n + e] = h;
-        h = fmaf(exp2_f(A2 * a[k]), h, own[k]);
+        h = carried(exp2_f(A2 * a[k]), h, own[k]);
       }
   }
   start[(o0 + nch - 1) * n + e] = h;                           // (the last chunk's own last state was not computed: nothing starts behind it)
@@ -324,7 +327,7 @@ __global__ __launch_bounds__(256) void scan_join_bwd_kernel(const seg_scan_args 
     for (int k = 0; k < JOIN; ++k)
       if (k0 - k > 0) {
         adj[(o0 + k0 - k) * n + e] = q;
-        q = fmaf(exp2_f(A2 * a[k]), q, own[k]);
+        q = carried(exp2_f(A2 * a[k]), q, own[k]);
       }
   }
   adj[o0 * n + e] = q;                                         // (the first chunk's own part was not computed: nothing lies in front of it)
@@ -365,33 +368,51 @@ __global__ __launch_bounds__(Lay<G>::NT) void scan_bwd_local_kernel(const seg_sc
     }
     rC.load((const T*)p.Cm, p.Cm_bs, p.Cm_ld, b, t0, len, p.S);
   };
-  if (tbeg < tlive) fetch(tbeg);
-  for (int t0 = tbeg; t0 < tlive; t0 += TT) {
-    if (worker) {
+  // GROWN: the factors from their logarithms' sum, terms of zero left out
+  auto walk = [&](auto GROWN) {
+    if (tbeg < tlive) fetch(tbeg);
+    for (int t0 = tbeg; t0 < tlive; t0 += TT) {
+      if (worker) {
 #pragma unroll
-      for (int i = 0; i < Y::PIECES; ++i) {
-        const int r = row0 + i * Y::ROWS;
+        for (int i = 0; i < Y::PIECES; ++i) {
+          const int r = row0 + i * Y::ROWS;
 #pragma unroll
-        for (int j = 0; j < 8; j += 2)
-          *reinterpret_cast<f4*>(&sdp[r][q0c + j]) = f4{delta_of(p, rt[i][j], bias[j], t0 + r < len), dp_of<T, VEC>(p, ry[i], rz[i], j),
-                                                       delta_of(p, rt[i][j + 1], bias[j + 1], t0 + r < len), dp_of<T, VEC>(p, ry[i], rz[i], j + 1)};
+          for (int j = 0; j < 8; j += 2)
+            *reinterpret_cast<f4*>(&sdp[r][q0c + j]) = f4{delta_of(p, rt[i][j], bias[j], t0 + r < len), dp_of<T, VEC>(p, ry[i], rz[i], j),
+                                                         delta_of(p, rt[i][j + 1], bias[j + 1], t0 + r < len), dp_of<T, VEC>(p, ry[i], rz[i], j + 1)};
+        }
       }
-    }
-    rC.put(sC);
-    if (t0 + TT < tlive) fetch(t0 + TT);
-    __syncthreads();
+      rC.put(sC);
+      if (t0 + TT < tlive) fetch(t0 + TT);
+      __syncthreads();
 #pragma unroll 4
-    for (int r = 0; r < TT; ++r) {
-      const float2 dd = sdp[r][c];
-      const f4 C4 = *reinterpret_cast<const f4*>(sC + r * Y::SP + 4 * g);
-      dsum += dd.x;
+      for (int r = 0; r < TT; ++r) {
+        const float2 dd = sdp[r][c];
+        const f4 C4 = *reinterpret_cast<const f4*>(sC + r * Y::SP + 4 * g);
+        dsum += dd.x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        P[i] *= exp2_f(dd.x * A2[i]);
-        q[i] = fmaf(P[i], C4[i] * dd.y, q[i]);
+        for (int i = 0; i < 4; ++i) {
+          const float x = C4[i] * dd.y;
+          if constexpr (GROWN()) {
+            if (x != 0.f) q[i] = fmaf(exp2_f(dsum * A2[i]), x, q[i]);
+          } else {
+            P[i] *= exp2_f(dd.x * A2[i]);
+            q[i] = fmaf(P[i], x, q[i]);
+          }
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
+  };
+  walk(std::false_type{});
+  // (a product that has left 32 bits stays outside of them; the block's other lanes keep what they have)
+  const bool far = !(P[0] + P[1] + P[2] + P[3] < INFINITY);
+  if (__syncthreads_or(far)) {
+    const f4 near = q;
+    dsum = 0.f;
+    q = f4{0.f, 0.f, 0.f, 0.f};
+    walk(std::true_type{});
+    if (!far) q = near;
   }
   if (!live) return;
   const int64_t o = ((int64_t)b * nch + chunk) * p.D + d;
