@@ -643,7 +643,8 @@ int seg_linear_act_bwd(const void* dy, int64_t dy_ld, const void* z, int64_t z_l
                        int32_t dtype, int32_t act, float alpha, seg_stream_t stream);
 
 /* Short causal convolution per channel: v[t] = bias + sum_k w[k] * xx[t + k], xx = [state (K - 1 rows); x], y[t] = act(v[t]).
- * B <= 65535 (fewer by a power of two for L above 2^22), L <= 2^30; w fp32 [K][D], 1 <= K <= 8; bias fp32 [D] or NULL; act NONE or SILU; state [B][K-1][D] of dtype (dense) or NULL = zeros;
+ * B <= 65535 (fewer by a power of two for L above 2^22), L <= 2^30, D <= 2^30; w fp32 [K][D], 1 <= K <= 8; bias fp32 [D] or NULL; act NONE or
+ * SILU; state [B][K-1][D] of dtype (dense) or NULL = zeros;
  * lengths int32 [B] or NULL: rows t >= lengths[b] (clamped to [0, L]) are not read, their y is 0.  state_out (NULL: not wanted)
  * = the last K - 1 rows of xx in front of lengths[b]; it may not be state.
  * bwd: from dy (rows behind a length not read) and dstate_out (gradient of state_out, NULL = 0): dx (0 behind a length), dw, db (fp32,
@@ -673,7 +674,8 @@ int seg_causal_conv_step(const seg_causal_conv_args* a, seg_stream_t stream);
 /* Selective state space scan.  Per sequence b, channel d and state s (1 <= S <= 64), with delta = softplus(dt + dt_bias) (softplus
  * == 0: dt + dt_bias itself):
  *   h[t] = exp(delta[t] A[d][s]) h[t-1] + delta[t] Bm[t][s] u[t],   y[t] = (sum_s Cm[t][s] h[t] + D[d] u[t]) * silu(z[t])
- * B <= 65535, L <= 2^30; u, dt, z, y [B][L][D], Bm, Cm [B][L][S] of dtype; A fp32 [D][S]; D, dt_bias fp32 [D] or NULL; z NULL = no gate; state fp32
+ * B <= 65535, L <= 2^30, D <= 2^30, fewer than 2^32 pieces of four states (S as the next of 4, 8, 16, 32, 64) in a row of D channels - step: in B D;
+ * u, dt, z, y [B][L][D], Bm, Cm [B][L][S] of dtype; A fp32 [D][S]; D, dt_bias fp32 [D] or NULL; z NULL = no gate; state fp32
  * [B][D][S] = h in front of the first row (NULL: zeros); lengths as above: rows behind a length are not read, their y is 0 and the
  * state stays; state_out (NULL: not wanted) may not be state; A and the states are 16-byte aligned.  saved (NULL: inference) receives what the backward pass needs:
  * seg_selective_scan_saved_bytes() bytes.
