@@ -95,7 +95,9 @@ constexpr float ACT_FAR = 128.f;
 __device__ __forceinline__ float silu_f(float v) { return __builtin_amdgcn_fmed3f(v, -ACT_FAR, INFINITY) * sigmoid_f(v); }
 __device__ __forceinline__ float silu_slope_f(float v) {
   const float s = sigmoid_f(v);
-  return s * (1.f + __builtin_amdgcn_fmed3f(v, -ACT_FAR, ACT_FAR) * (1.f - s));
+  float far = ACT_FAR;
+  asm("" : "+s"(far));                                         // (one scalar register for both ends: as literals either end costs a move each time)
+  return s * (1.f + __builtin_amdgcn_fmed3f(v, -far, far) * (1.f - s));
 }
 // Phi(-|v|) = erfc(|v| / sqrt 2) / 2 = Q e with e = exp(-v^2 / 2), and ve = |v| e.  erfc(x) exp(x^2) = t P(t) with t = 1 / (1 + 0.3 x), P of degree 8
 // fitted to a relative error of 2e-8 on 0 <= x <= 9.5 (behind it both factors are 0 in 32 bits), at about 20 instructions - half of the
