@@ -6,9 +6,9 @@
 // Bandwidth bounds all three.  A thread owns 8 neighbouring channels (one 16-byte access per row) and walks a run of rows with the
 // window of K rows in registers, so every row is read once per run plus K - 1 rows at its edges.
 //
-// Measured: forward 8 x 4096 x 2048 bf16, K = 4, half of the sequences shorter, 48 us (the bytes' floor with whole sequences is 55);
-// backward 16 x 1024 x 512 f16 21 us for 50 MB: about 44 operations per element are 10 us of the vector ALUs, and its 220 registers leave
-// two waves per SIMD to hide the loads behind them.
+// Measured: forward 8 x 4096 x 2048 bf16, K = 4, half of the sequences shorter, 49 us (the bytes' floor 41, with whole sequences 55);
+// backward 16 x 1024 x 512 f16 21 us for 50 MB: 57 instructions per element (11 rows recomputed for 8) are 12 us of the vector ALUs, and
+// its 227 registers leave two waves per SIMD to hide the loads behind them.  K = 8 takes 313 us for 8 x 4096 x 2048 (120 with K = 4, the bytes 82).
 #include "seq_common.h"
 
 namespace {
