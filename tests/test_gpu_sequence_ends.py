@@ -275,3 +275,45 @@ def test_selective_scan_of_growing_states(S):
         assert torch.isfinite(got).all(), name
         assert float((got - exact).abs().max()) <= 160 * 2.0 ** -24 * float(exact.abs().max()), name
     assert torch.isfinite(d.dstate).all()
+
+
+@pytest.mark.parametrize("C", [64, 1111, 4096, 20001])
+def test_layer_norm_of_rows_far_from_zero(C):
+    """Offsets far above the spread: the mean is off by its own rounding alone (half a step, 2^-24 of it), beside the roundings of sums of the
+    spread (a lane's channels and 8 to combine them, twice; xhat, rstd and the result 8)."""
+    g = gen(71 + C)
+    x = (torch.randn(9, C, generator=g) * torch.tensor([0.1, 1.0, 3.0])[:, None].repeat(3, 1) + torch.tensor([1000.0, -300.0, 70.0])[:, None].repeat_interleave(3, 0)).float()
+    gamma, beta = torch.rand(C, generator=g) + 0.5, torch.randn(C, generator=g)
+    y, mean, rstd = seq.layer_norm(x.cuda(), gamma.cuda(), beta.cuda(), stats=True)
+    d = x.double()
+    m = d.mean(1, keepdim=True)
+    r = (((d - m) ** 2).mean(1, keepdim=True) + 1e-3) ** -0.5
+    n, u = 2 * (max(64, C // 256 + 1) + 8) + 8, 2.0 ** -24
+    off = m.abs() * u + n * u * (d - m).abs().mean(1, keepdim=True)                      # of the mean
+    xh = ((d - m) * r).abs()
+    assert float(((mean.double().cpu() - m[:, 0]).abs() / off[:, 0]).max()) <= 1
+    assert float(((rstd.double().cpu()[:, None] / r - 1).abs() / (n * u + (off * r) ** 2)).max()) <= 1
+    want = (d - m) * r * gamma.double() + beta.double()
+    bound = (off * r + xh * (n * u + (off * r) ** 2)) * gamma.double() + 4 * u * (want.abs() + beta.double().abs() + xh * gamma.double())
+    assert float(((y.double().cpu() - want).abs() / bound).max()) <= 1
+
+
+def test_causal_conv_of_several_long_sequences():
+    """Row blocks past one axis share the third with the sequences: every sequence's rows, lengths and states are its own."""
+    g = torch.Generator("cuda").manual_seed(72)
+    B, L, D, K = 3, 65535 * 64 + 130, 8, 4
+    x, dy = (torch.randint(-2, 3, (B, L, D), device="cuda", generator=g).half() for _ in range(2))
+    st, dst = (torch.randint(-2, 3, (B, K - 1, D), device="cuda", generator=g).half() for _ in range(2))
+    w = torch.tensor([1.0, -2.0, 3.0, -1.0], device="cuda")[:, None].expand(K, D).contiguous()
+    lengths = torch.tensor([L, 70, L - 65], dtype=torch.int32, device="cuda")
+    y, new = seq.causal_conv(x, w, state=st, lengths=lengths)
+    dx, dw, _db, dstate = seq.causal_conv_backward(dy, x, w, state=st, lengths=lengths, dstate=dst)
+    sums = torch.zeros(K, D, dtype=torch.long, device="cuda")
+    for b, n in enumerate(lengths.tolist()):
+        xx, dd = torch.cat([st[b], x[b, :n]]), torch.cat([torch.zeros(K - 1, D, dtype=torch.float16, device="cuda"), dy[b, :n], torch.zeros(K - 1, D, dtype=torch.float16, device="cuda")])
+        assert torch.equal(y[b, :n], sum(xx[k:k + n] * w[k, 0].half() for k in range(K))) and not y[b, n:].any() and torch.equal(new[b], xx[n:])
+        dxx = sum(dd[K - 1 - k:K - 1 - k + n + K - 1] * w[k, 0].half() for k in range(K))
+        dxx[n:] += dst[b]
+        assert torch.equal(dx[b, :n], dxx[K - 1:]) and not dx[b, n:].any() and torch.equal(dstate[b], dxx[:K - 1])
+        sums += torch.stack([(xx[k:k + n].long() * dy[b, :n].long()).sum(0) for k in range(K)])
+    assert torch.equal(dw.long(), sums)
