@@ -317,3 +317,36 @@ def test_causal_conv_of_several_long_sequences():
         assert torch.equal(dx[b, :n], dxx[K - 1:]) and not dx[b, n:].any() and torch.equal(dstate[b], dxx[:K - 1])
         sums += torch.stack([(xx[k:k + n].long() * dy[b, :n].long()).sum(0) for k in range(K)])
     assert torch.equal(dw.long(), sums)
+
+
+@pytest.mark.parametrize("name", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_nan_goes_through_every_activation(name, dtype):
+    g = gen(73)
+    for M, N, K in KERNELS:
+        b = rnd(g, N)
+        b[N // 3] = float("nan")
+        y = seq.linear(rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype), b, activation=name)
+        on = torch.arange(N, device="cuda") == N // 3
+        assert torch.isnan(y[:, on]).all() and not torch.isnan(y[:, ~on]).any(), (M, N, K)
+    z, dy = rnd(g, 9, 21, dtype=dtype), rnd(g, 9, 21, dtype=dtype)
+    z[4, 3] = float("nan")
+    d = seq.activation_backward(dy, z, name)
+    assert not torch.isnan(d[z == z]).any() and (name in ("relu", "leaky_relu") or torch.isnan(d[4, 3]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_nan_goes_through_the_convolution_and_the_gate(dtype):
+    """A NaN stays in its channel (and, in the convolution, in the rows whose window holds it)."""
+    g = gen(74)
+    x, w = rnd(g, 2, 40, 24, dtype=dtype), rnd(g, 4, 24)
+    x[1, 10, 5] = float("nan")
+    y, _ = seq.causal_conv(x, w, activation="silu")
+    want = torch.zeros_like(y, dtype=torch.bool)
+    want[1, 10:14, 5] = True
+    assert torch.equal(torch.isnan(y), want)
+    u, dt, z = (rnd(g, 2, 40, 24, dtype=dtype) for _ in range(3))
+    Bm, Cm, A = rnd(g, 2, 40, 16, dtype=dtype), rnd(g, 2, 40, 16, dtype=dtype), -torch.rand(24, 16, generator=g).cuda()
+    z[0, 7, 3] = float("nan")
+    y, last = seq.selective_scan(u, dt, A, Bm, Cm, z=z)
+    assert torch.equal(torch.isnan(y), torch.isnan(z)) and torch.isfinite(last).all()
